@@ -19,6 +19,7 @@
 #include "ral/nccl_dyn.h"
 #include "../../include/disc_b200_ral.h"
 #include "kernels/attention.h"
+#include "kernels/kv8.h"
 #include "kernels/observer.h"
 #include "kernels/qconv.h"
 #include "kernels/qgemm.h"
@@ -437,6 +438,131 @@ int32_t disc_b200_attention(const disc_b200_attention_args* a, void* stream) {
   const char* detail = nullptr;
   const cudaError_t st = disc_b200::attention_launch(p, static_cast<cudaStream_t>(stream), &detail);
   return finish(st, "attention", detail);
+}
+
+namespace {
+disc_b200::KvBlocksParams kv_blocks_params(const disc_b200_kv_blocks_args* a) {
+  disc_b200::KvBlocksParams p;
+  p.tokens = a->tokens;
+  p.lens = a->lens;
+  p.table = a->table;
+  p.free_list = a->free_list;
+  p.free_count = a->free_count;
+  p.requests = a->requests;
+  p.table_width = a->table_width;
+  p.num_blocks = a->num_blocks;
+  p.block_size = a->block_size;
+  p.max_tokens = a->max_tokens;
+  p.slots = a->slots;
+  p.positions = a->positions;
+  p.q_start = a->q_start;
+  p.q_lens = a->q_lens;
+  p.kv_lens = a->kv_lens;
+  return p;
+}
+
+disc_b200::Kv8Cache kv8_cache(const disc_b200_kv8_cache& a) {
+  disc_b200::Kv8Cache c;
+  c.k = a.k;
+  c.v = a.v;
+  c.k_scale = a.k_scale;
+  c.v_scale = a.v_scale;
+  c.num_blocks = a.num_blocks;
+  c.kv_heads = a.kv_heads;
+  c.block_size = a.block_size;
+  c.dim = a.dim;
+  return c;
+}
+}  // namespace
+
+int32_t disc_b200_kv_blocks_extend(const disc_b200_kv_blocks_args* a, void* stream) {
+  if (!a) {
+    g_last_error = "kv_blocks_extend: null args";
+    return 1;
+  }
+  const char* detail = nullptr;
+  const cudaError_t st =
+      disc_b200::kv_blocks_extend_launch(kv_blocks_params(a), static_cast<cudaStream_t>(stream), &detail);
+  return finish(st, "kv_blocks_extend", detail);
+}
+
+int32_t disc_b200_kv_blocks_trim(const disc_b200_kv_blocks_args* a, void* stream) {
+  if (!a) {
+    g_last_error = "kv_blocks_trim: null args";
+    return 1;
+  }
+  const char* detail = nullptr;
+  const cudaError_t st =
+      disc_b200::kv_blocks_trim_launch(kv_blocks_params(a), static_cast<cudaStream_t>(stream), &detail);
+  return finish(st, "kv_blocks_trim", detail);
+}
+
+int32_t disc_b200_kv8_append(const disc_b200_kv8_append_args* a, void* stream) {
+  if (!a) {
+    g_last_error = "kv8_append: null args";
+    return 1;
+  }
+  disc_b200::Kv8AppendParams p;
+  p.qkv = a->qkv;
+  p.tokens = a->tokens;
+  p.ld_qkv = a->ld_qkv;
+  p.q_heads = a->q_heads;
+  p.q_out = a->q_out;
+  p.slots = a->slots;
+  p.positions = a->positions;
+  p.cos_table = a->cos_table;
+  p.sin_table = a->sin_table;
+  p.table_rows = a->table_rows;
+  p.type = a->type;
+  p.cache = kv8_cache(a->cache);
+  const char* detail = nullptr;
+  const cudaError_t st = disc_b200::kv8_append_launch(p, static_cast<cudaStream_t>(stream), &detail);
+  return finish(st, "kv8_append", detail);
+}
+
+int32_t disc_b200_kv8_read(const disc_b200_kv8_read_args* a, void* stream) {
+  if (!a) {
+    g_last_error = "kv8_read: null args";
+    return 1;
+  }
+  disc_b200::Kv8ReadParams p;
+  p.cache = kv8_cache(a->cache);
+  p.blocks = a->blocks;
+  p.count = a->count;
+  p.k_out = a->k_out;
+  p.v_out = a->v_out;
+  p.type = a->type;
+  const char* detail = nullptr;
+  const cudaError_t st = disc_b200::kv8_read_launch(p, static_cast<cudaStream_t>(stream), &detail);
+  return finish(st, "kv8_read", detail);
+}
+
+int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* a, void* stream) {
+  if (!a) {
+    g_last_error = "kv8_attention: null args";
+    return 1;
+  }
+  disc_b200::Kv8AttentionParams p;
+  p.q = a->q;
+  p.out = a->out;
+  p.tokens = a->tokens;
+  p.ld_q = a->ld_q;
+  p.ld_out = a->ld_out;
+  p.q_heads = a->q_heads;
+  p.cache = kv8_cache(a->cache);
+  p.table = a->table;
+  p.q_start = a->q_start;
+  p.q_lens = a->q_lens;
+  p.kv_lens = a->kv_lens;
+  p.requests = a->requests;
+  p.table_width = a->table_width;
+  p.max_q = a->max_q;
+  p.max_kv = a->max_kv;
+  p.scale = a->scale;
+  p.type = a->type;
+  const char* detail = nullptr;
+  const cudaError_t st = disc_b200::kv8_attention_launch(p, static_cast<cudaStream_t>(stream), &detail);
+  return finish(st, "kv8_attention", detail);
 }
 
 int32_t disc_b200_gated_quantize(const disc_b200_gated_quantize_args* a, void* stream) {

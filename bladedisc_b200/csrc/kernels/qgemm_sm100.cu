@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "kv8.h"
 #include "device_info.h"
 #include "qgemm.h"
 #include "rowops.h"
@@ -1692,7 +1693,8 @@ int kernel_status_fetch_and_clear() {
   const int r = rowops_status_fetch_and_clear();
   const int a = attention_status_fetch_and_clear();
   const int w = woq_tc_status_fetch_and_clear();
-  return h != 0 ? h : (r != 0 ? r : (a != 0 ? a : w));
+  const int k = kv8_status_fetch_and_clear();
+  return h != 0 ? h : (r != 0 ? r : (a != 0 ? a : (w != 0 ? w : k)));
 }
 
 }  // namespace disc_b200

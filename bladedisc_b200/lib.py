@@ -20,7 +20,7 @@ ACT_NONE, ACT_GELU, ACT_SILU = 0, 1, 2
 BIAS_NONE, BIAS_F32, BIAS_I8 = 0, 1, 2
 SCALE_NONE, SCALE_SCALAR, SCALE_PER_COL, SCALE_PER_ROW = 0, 1, 2, 3
 PATH_AUTO, PATH_TILED, PATH_SMALL_M, PATH_SIMT, PATH_PAIR, PATH_GEMV, PATH_SKINNY = 0, 1, 2, 3, 4, 5, 6
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2  # BF16: the kv8 calls only
 
 
 class ContextOptions(Structure):
@@ -80,6 +80,47 @@ class AttentionArgs(Structure):
     ]
 
 
+class KvBlocksArgs(Structure):
+    _fields_ = [
+        ("tokens", c_void_p), ("lens", c_void_p), ("table", c_void_p), ("free_list", c_void_p),
+        ("free_count", c_void_p),
+        ("requests", c_int32), ("table_width", c_int32), ("num_blocks", c_int32), ("block_size", c_int32),
+        ("max_tokens", c_int32), ("slots", c_void_p), ("positions", c_void_p), ("q_start", c_void_p),
+        ("q_lens", c_void_p), ("kv_lens", c_void_p),
+    ]
+
+
+class Kv8Cache(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("num_blocks", c_int32), ("kv_heads", c_int32), ("block_size", c_int32), ("dim", c_int32),
+    ]
+
+
+class Kv8AppendArgs(Structure):
+    _fields_ = [
+        ("qkv", c_void_p), ("tokens", c_int64), ("ld_qkv", c_int64), ("q_heads", c_int32), ("type", c_int32),
+        ("q_out", c_void_p), ("slots", c_void_p), ("positions", c_void_p), ("cos_table", c_void_p),
+        ("sin_table", c_void_p), ("table_rows", c_int32), ("cache", Kv8Cache),
+    ]
+
+
+class Kv8ReadArgs(Structure):
+    _fields_ = [
+        ("cache", Kv8Cache), ("blocks", c_void_p), ("count", c_int32), ("type", c_int32), ("k_out", c_void_p),
+        ("v_out", c_void_p),
+    ]
+
+
+class Kv8AttentionArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("out", c_void_p), ("tokens", c_int64), ("ld_q", c_int64), ("ld_out", c_int64),
+        ("q_heads", c_int32), ("type", c_int32), ("cache", Kv8Cache), ("table", c_void_p), ("q_start", c_void_p),
+        ("q_lens", c_void_p), ("kv_lens", c_void_p), ("requests", c_int32), ("table_width", c_int32),
+        ("max_q", c_int32), ("max_kv", c_int32), ("scale", c_float),
+    ]
+
+
 class WeightOnlyQGemmArgs(Structure):
     _fields_ = [
         ("x", c_void_p), ("w", c_void_p), ("scale", c_void_p), ("zero_point", c_void_p), ("bias", c_void_p),
@@ -136,6 +177,11 @@ SIGNATURES = {
     "disc_b200_softmax": (c_int32, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p,
                                     c_void_p, c_float, c_int32, c_void_p]),
     "disc_b200_attention": (c_int32, [POINTER(AttentionArgs), c_void_p]),
+    "disc_b200_kv_blocks_extend": (c_int32, [POINTER(KvBlocksArgs), c_void_p]),
+    "disc_b200_kv_blocks_trim": (c_int32, [POINTER(KvBlocksArgs), c_void_p]),
+    "disc_b200_kv8_append": (c_int32, [POINTER(Kv8AppendArgs), c_void_p]),
+    "disc_b200_kv8_read": (c_int32, [POINTER(Kv8ReadArgs), c_void_p]),
+    "disc_b200_kv8_attention": (c_int32, [POINTER(Kv8AttentionArgs), c_void_p]),
     "disc_b200_nccl_available": (c_int32, []),
     "disc_b200_nccl_unique_id": (c_int32, [c_void_p]),
     "disc_b200_nccl_comm_create": (c_int32, [c_void_p, c_int32, c_int32, POINTER(c_void_p)]),

@@ -7,7 +7,7 @@ back to torch operators.
 """
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -557,6 +557,217 @@ def rope_kv_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _lib.check(_lib.load().disc_b200_rope_kv_append(qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                                     cos.data_ptr(), sin.data_ptr(), batch, seq, heads, dim, pos0,
                                                     cache_len, _stream()))
+
+
+# ---------------------------------------------------------------- paged key / value cache in 8 bits
+class KvPlan(NamedTuple):
+    """What `kv_blocks_extend` says about one batch of new tokens (int32 CUDA tensors)."""
+    slots: torch.Tensor      # [max_tokens] slot of each token row, -1 = none
+    positions: torch.Tensor  # [max_tokens] position in its request, -1 = none
+    q_start: torch.Tensor    # [requests + 1] first token row of each request
+    q_lens: torch.Tensor     # [requests] tokens that found room (all that were asked for, or 0)
+    kv_lens: torch.Tensor    # [requests] cached tokens with the new ones
+
+
+def _one_device(first: torch.Tensor, **tensors) -> torch.device:
+    """The CUDA device that all of them are on."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("the paged cache lives on CUDA tensors: there is no CPU implementation")
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, not on {dev} like the others")
+    return dev
+
+
+def _call(dev: torch.device, fn, args) -> None:
+    """Launches on the current stream of `dev`, whichever device is current."""
+    if torch.cuda.current_device() == dev.index:
+        _lib.check(fn(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int) -> torch.Tensor:
+    if t.dtype != dtype or t.dim() != dims or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor with {dims} dimension(s), got {t.dtype} "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return t
+
+
+def _kv_blocks_args(tokens, lens, table, free_list, free_count, block_size):
+    dev = _one_device(lens, tokens=tokens, table=table, free_list=free_list, free_count=free_count)
+    _dense("tokens", tokens, torch.int32, 1)
+    _dense("lens", lens, torch.int32, 1)
+    _dense("table", table, torch.int32, 2)
+    _dense("free_list", free_list, torch.int32, 1)
+    if free_count.dtype != torch.int32 or free_count.numel() != 1:
+        raise ValueError("free_count must be one int32 value")
+    if tokens.shape != lens.shape or table.shape[0] != lens.numel():
+        raise ValueError("tokens, lens and table must have one entry (row) per request")
+    a = _lib.KvBlocksArgs(tokens.data_ptr(), lens.data_ptr(), table.data_ptr(), free_list.data_ptr(),
+                          free_count.data_ptr(), lens.numel(), table.shape[1], free_list.numel(), int(block_size))
+    return dev, a
+
+
+def kv_blocks_extend(tokens: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, free_list: torch.Tensor,
+                     free_count: torch.Tensor, block_size: int, max_tokens: int) -> KvPlan:
+    """Makes room for ``tokens[r]`` new tokens of each request: pops blocks off the stack
+    ``free_list[:free_count]``, enters them into ``table [requests, width]`` and grows ``lens`` (all int32, updated
+    in place), and returns where every token of the batch goes.  The batch holds the tokens of the requests one
+    after the other; ``max_tokens`` is the number of rows it has room for.
+
+    A request is refused as a whole (``q_lens`` 0, slots -1, nothing else changed) when the blocks for it and for
+    all requests before it are not there, its table row is too short, or its rows end behind ``max_tokens``."""
+    dev, a = _kv_blocks_args(tokens, lens, table, free_list, free_count, block_size)
+    n, cap = lens.numel(), int(max_tokens)
+    if cap < 0:
+        raise ValueError("max_tokens must not be negative")
+    out = KvPlan(*torch.empty(2 * cap + 3 * n + 1, dtype=torch.int32, device=dev).split([cap, cap, n + 1, n, n]))
+    a.max_tokens = cap
+    a.slots, a.positions, a.q_start, a.q_lens, a.kv_lens = (t.data_ptr() for t in out)
+    _call(dev, _lib.load().disc_b200_kv_blocks_extend, a)
+    return out
+
+
+def kv_blocks_trim(keep: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, free_list: torch.Tensor,
+                   free_count: torch.Tensor, block_size: int) -> None:
+    """Keeps the first ``keep[r]`` cached tokens of each request (0 releases it) and gives the blocks behind them
+    back to the stack, in place.  Trimming to the lengths before a `kv_blocks_extend` undoes it exactly."""
+    dev, a = _kv_blocks_args(keep, lens, table, free_list, free_count, block_size)
+    _call(dev, _lib.load().disc_b200_kv_blocks_trim, a)
+
+
+_KV_TYPE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+def _kv8_cache(k, v, k_scale, v_scale) -> "_lib.Kv8Cache":
+    _dense("k", k, torch.int8, 4)
+    _dense("v", v, torch.int8, 4)
+    _dense("k_scale", k_scale, torch.float32, 2)
+    _dense("v_scale", v_scale, torch.float32, 2)
+    blocks, heads, size, dim = k.shape
+    if v.shape != k.shape or tuple(k_scale.shape) != (blocks, heads) or v_scale.shape != k_scale.shape:
+        raise ValueError("k and v must be [blocks, kv heads, block size, head size], their scales [blocks, kv heads]")
+    return _lib.Kv8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, size, dim)
+
+
+def _kv_type(name: str, dtype: torch.dtype) -> int:
+    if dtype not in _KV_TYPE:
+        raise TypeError(f"{name} must be float16 or bfloat16, got {dtype}")
+    return _KV_TYPE[dtype]
+
+
+def kv8_append(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               slots: torch.Tensor, positions: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None,
+               sin: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Quantizes the new keys and values of ``qkv [tokens, (q heads + 2 kv heads) * head size]`` (float16 or
+    bfloat16, rows may be strided) into one layer of the cache, in place, after rotating q and k by ``cos`` / ``sin``
+    (float32 ``[positions, head size / 2]``) when those are given.  Returns q ``[tokens, q heads, head size]``,
+    rotated (a view of ``qkv`` without ``cos``), or None if there are no query heads.
+
+    The cache is ``k``, ``v`` int8 ``[blocks, kv heads, block size, head size]`` with ``k_scale``, ``v_scale`` float32
+    ``[blocks, kv heads]``: a block and a head share the scale ``max|x| / 127`` of the tokens stored so far; tokens
+    that the block held before are moved to the new scale when it grows.  ``slots`` and ``positions`` are those of
+    `kv_blocks_extend` (the first ``tokens`` entries are read; slot -1 = not stored)."""
+    dev = _one_device(k, qkv=qkv, v=v, k_scale=k_scale, v_scale=v_scale, slots=slots, positions=positions, cos=cos,
+                      sin=sin)
+    cache = _kv8_cache(k, v, k_scale, v_scale)
+    kind = _kv_type("qkv", qkv.dtype)
+    if qkv.dim() != 2 or (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]) or (qkv.numel() and qkv.stride(1) != 1):
+        raise ValueError("qkv must be [tokens, columns] with unit column stride and rows that do not overlap")
+    tokens, cols = qkv.shape
+    dim, kv_heads = cache.dim, cache.kv_heads
+    if cols % dim or cols < 2 * kv_heads * dim:
+        raise ValueError(f"qkv rows of {cols} values do not hold whole heads of {dim} beside {kv_heads} + {kv_heads}")
+    q_heads = cols // dim - 2 * kv_heads
+    _dense("slots", slots, torch.int32, 1)
+    if slots.numel() < tokens:
+        raise ValueError("one slot per token expected")
+    ld = qkv.stride(0) if tokens > 1 else cols
+    a = _lib.Kv8AppendArgs(qkv.data_ptr(), tokens, ld, q_heads, kind, None, slots.data_ptr())
+    a.cache = cache
+    q = None
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or positions is None:
+            raise ValueError("a rotation needs cos, sin and positions")
+        _dense("cos", cos, torch.float32, 2)
+        _dense("sin", sin, torch.float32, 2)
+        _dense("positions", positions, torch.int32, 1)
+        if cos.shape[1] != dim // 2 or cos.shape != sin.shape or cos.shape[0] < 1 or positions.numel() < tokens:
+            raise ValueError("cos / sin must be [positions, head size / 2], positions one per token")
+        a.positions, a.cos_table, a.sin_table = positions.data_ptr(), cos.data_ptr(), sin.data_ptr()
+        a.table_rows = cos.shape[0]
+        if q_heads:
+            q = torch.empty((tokens, q_heads, dim), dtype=qkv.dtype, device=dev)
+            a.q_out = q.data_ptr()
+    elif q_heads:
+        q = qkv[:, :q_heads * dim].unflatten(1, (q_heads, dim))
+    _call(dev, _lib.load().disc_b200_kv8_append, a)
+    return q
+
+
+def kv8_read(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, blocks: torch.Tensor,
+             dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The given blocks (int32 ids) of one layer as the values they stand for: keys and values of ``dtype``
+    ``[len(blocks), kv heads, block size, head size]``; zeros for an id outside the cache."""
+    dev = _one_device(k, v=v, k_scale=k_scale, v_scale=v_scale, blocks=blocks)
+    a = _lib.Kv8ReadArgs(_kv8_cache(k, v, k_scale, v_scale))
+    _dense("blocks", blocks, torch.int32, 1)
+    a.type = _kv_type("dtype", dtype)
+    a.blocks, a.count = blocks.data_ptr(), blocks.numel()
+    out = torch.empty((2, blocks.numel()) + tuple(k.shape[1:]), dtype=dtype, device=dev)
+    ko, vo = out.unbind(0)
+    a.k_out, a.v_out = ko.data_ptr(), vo.data_ptr()
+    _call(dev, _lib.load().disc_b200_kv8_read, a)
+    return ko, vo
+
+
+def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  table: torch.Tensor, q_start: torch.Tensor, q_lens: torch.Tensor, kv_lens: torch.Tensor, *,
+                  max_q: int, scale: Optional[float] = None, max_kv: Optional[int] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of ``q [tokens, q heads, head size]`` over one layer of the 8-bit cache.
+
+    Request ``r`` has the rows ``q_start[r] ... q_start[r] + q_lens[r] - 1`` of ``q``, its last tokens; they see its
+    ``kv_lens[r]`` cached tokens (their own included: append first) up to their own position.  The index tensors
+    are int32 and stay on the device; ``max_q`` bounds ``q_lens`` and shapes the launch (rows behind it are not
+    computed), ``max_kv`` bounds ``kv_lens`` and only steers how the work is split (default: the table's width).
+    Query heads are a multiple of the kv heads.  ``scale`` defaults to ``head size ** -0.5``.  Rows that belong to
+    no request are left as ``out`` had them; a row that sees no key gives zeros."""
+    dev = _one_device(q, k=k, v=v, k_scale=k_scale, v_scale=v_scale, table=table, q_start=q_start, q_lens=q_lens,
+                      kv_lens=kv_lens, out=out)
+    cache = _kv8_cache(k, v, k_scale, v_scale)
+    kind = _kv_type("q", q.dtype)
+    if q.dim() != 3 or q.shape[2] != cache.dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"q must be [tokens, heads, {cache.dim}] with a multiple of {cache.kv_heads} heads, got "
+                         f"{tuple(q.shape)}")
+    tokens, heads, dim = q.shape
+    if q.numel() and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or
+                      (tokens > 1 and q.stride(0) < heads * dim)):
+        raise ValueError("the heads of a row of q must lie one after the other, and rows may not overlap")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of q's shape and dtype")
+    _dense("table", table, torch.int32, 2)
+    _dense("q_lens", q_lens, torch.int32, 1)
+    _dense("kv_lens", kv_lens, torch.int32, 1)
+    _dense("q_start", q_start, torch.int32, 1)
+    n = q_lens.numel()
+    if kv_lens.numel() != n or table.shape[0] != n or q_start.numel() < n:
+        raise ValueError("q_start, q_lens, kv_lens and table must have one entry (row) per request")
+    if max_q < 0 or (max_kv is not None and max_kv < 0):
+        raise ValueError("max_q and max_kv must not be negative")
+    room = table.shape[1] * cache.block_size
+    a = _lib.Kv8AttentionArgs(q.data_ptr(), out.data_ptr(), tokens, q.stride(0) if tokens > 1 else heads * dim,
+                              heads * dim, heads, kind, cache, table.data_ptr(), q_start.data_ptr(),
+                              q_lens.data_ptr(), kv_lens.data_ptr(), n, table.shape[1], int(max_q),
+                              room if max_kv is None else min(int(max_kv), room),
+                              dim ** -0.5 if scale is None else float(scale))
+    _call(dev, _lib.load().disc_b200_kv8_attention, a)
+    return out
 
 
 def kernel_status() -> int:

@@ -138,7 +138,8 @@ enum { DISC_B200_SCALE_NONE = 0, DISC_B200_SCALE_SCALAR = 1, DISC_B200_SCALE_PER
 enum { DISC_B200_PATH_AUTO = 0, DISC_B200_PATH_TILED = 1, DISC_B200_PATH_SMALL_M = 2,
        DISC_B200_PATH_SIMT = 3, DISC_B200_PATH_PAIR = 4, DISC_B200_PATH_GEMV = 5,
        DISC_B200_PATH_SKINNY = 6 };
-enum { DISC_B200_F32 = 0, DISC_B200_F16 = 1 };
+enum { DISC_B200_F32 = 0, DISC_B200_F16 = 1,
+       DISC_B200_BF16 = 2 /* the disc_b200_kv8_* calls only */ };
 
 /* out[m, n] = epilogue(sum_k a[m, k] * w[n, k]); a int8 [M, K], w int8 [N, K],
  * both row-major.  All scale / bias pointers are DEVICE pointers: nothing is
@@ -470,6 +471,111 @@ typedef struct disc_b200_attention_args {
   const float* out_scale;
 } disc_b200_attention_args;
 int32_t disc_b200_attention(const disc_b200_attention_args* args, void* stream);
+
+/* ---- Paged key / value cache in 8 bits.  No counterpart in the reference, whose compiled decoders carry
+ * fp16 caches as ordinary tensors.  Token p of request r lives in block table[r * table_width + p / block_size]
+ * at offset p % block_size; its slot is block * block_size + offset.  Everything below works on lengths and
+ * tables that lie on the device, allocates nothing and does not synchronise: a decode step made of these calls
+ * can be captured into a CUDA graph and replayed.
+ *
+ * extend: makes room for tokens[r] (< 0 reads as 0) new tokens of every request.  Blocks are popped off the
+ * stack free_list[0 .. *free_count) in the order (request, place) and entered into the table; lens grows.  A
+ * request is refused as a whole when the stack does not hold its blocks and those of all requests before it, when
+ * its table row is too short, or when its tokens would end behind max_tokens; one that needs no new block is not
+ * refused for want of blocks.  The batch holds the tokens of all requests one after the other, the refused ones' too:
+ *   q_start[r]  first token row of request r, q_start[requests] the number of rows (exclusive sums of tokens)
+ *   q_lens[r]   tokens[r], 0 if refused          kv_lens[r]  lens[r] after the call
+ *   slots[t], positions[t]  of token row t; -1 for rows of refused requests and behind the last row.
+ * trim: keeps the first tokens[r] (at most lens[r]; 0 releases the request) tokens of every request, pushes the
+ * blocks behind them back and sets their table entries to -1.  trim to the lengths before an extend undoes it
+ * bit for bit.  A block belongs to one request at a time.  requests <= 8192.  Calls that share state must be
+ * ordered by the caller. */
+typedef struct disc_b200_kv_blocks_args {
+  const int32_t* tokens; /* [requests] */
+  int32_t* lens;         /* [requests] */
+  int32_t* table;        /* [requests, table_width] */
+  int32_t* free_list;    /* [num_blocks] */
+  int32_t* free_count;   /* [1] */
+  int32_t requests, table_width, num_blocks, block_size;
+  /* extend only */
+  int32_t max_tokens;
+  int32_t* slots;        /* [max_tokens] */
+  int32_t* positions;    /* [max_tokens] */
+  int32_t* q_start;      /* [requests + 1] */
+  int32_t* q_lens;       /* [requests] */
+  int32_t* kv_lens;      /* [requests] */
+} disc_b200_kv_blocks_args;
+int32_t disc_b200_kv_blocks_extend(const disc_b200_kv_blocks_args* args, void* stream);
+int32_t disc_b200_kv_blocks_trim(const disc_b200_kv_blocks_args* args, void* stream);
+
+/* One layer of the cache: levels int8 [num_blocks, kv_heads, block_size, dim], scales f32 [num_blocks, kv_heads],
+ * value = level * scale.  dim 64 or 128, block_size 16, 32, 64 or 128. */
+typedef struct disc_b200_kv8_cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int32_t num_blocks, kv_heads, block_size, dim;
+} disc_b200_kv8_cache;
+
+/* Rotary embedding of q and k (pairs (i, i + dim / 2), as disc_b200_rope_kv_append) and the append of k and v:
+ *   scale  s = max(s_old, max|x| / 127) over the new tokens of the block and head; s_old counts only if the block
+ *          holds tokens before the first new one (offset > 0)
+ *   levels clamp(rne(x / s), -127, 127), 0 when s = 0; tokens that the block held before move to the new scale,
+ *          rne(level * (s_old / s)).  A value that is not finite makes the scale NaN until the block is reused.
+ * qkv: f16 / bf16 [tokens, (q_heads + 2 * kv_heads) * dim] with row stride ld_qkv, not modified; rotated q goes to
+ * q_out [tokens, q_heads, dim].  cos_table NULL: no rotation, q_out and positions are not used.  slots: as extend
+ * writes them (-1 = skip); the slots of one block must follow one another without a gap, and no slot may occur twice.
+ * positions outside [0, table_rows) read the nearest row of the tables. */
+typedef struct disc_b200_kv8_append_args {
+  const void* qkv;
+  int64_t tokens, ld_qkv;
+  int32_t q_heads; /* may be 0 */
+  int32_t type;    /* DISC_B200_F16 / DISC_B200_BF16 */
+  void* q_out;
+  const int32_t* slots;
+  const int32_t* positions;
+  const float* cos_table; /* f32 [table_rows, dim / 2] */
+  const float* sin_table;
+  int32_t table_rows;
+  disc_b200_kv8_cache cache;
+} disc_b200_kv8_append_args;
+int32_t disc_b200_kv8_append(const disc_b200_kv8_append_args* args, void* stream);
+
+/* Blocks of the cache as the values they stand for: k_out, v_out f16 / bf16 [count, kv_heads, block_size, dim];
+ * a block id outside the cache reads as zeros. */
+typedef struct disc_b200_kv8_read_args {
+  disc_b200_kv8_cache cache;
+  const int32_t* blocks;
+  int32_t count;
+  int32_t type;
+  void* k_out;
+  void* v_out;
+} disc_b200_kv8_read_args;
+int32_t disc_b200_kv8_read(const disc_b200_kv8_read_args* args, void* stream);
+
+/* Causal attention of q over the cache: token i of the q_lens[r] tokens of request r, row q_start[r] + i of q,
+ * sees the keys 0 .. kv_lens[r] - q_lens[r] + i.  Query head h reads kv head h / (q_heads / kv_heads).  Scores,
+ * softmax and sums are fp32.  A row without keys gives 0; keys whose table entry is not a block of the cache are
+ * left out; rows that belong to no request are left as they were.  max_q and max_kv: bounds on q_lens and
+ * kv_lens known to the host (the launch is shaped by them: tokens of a request behind its first max_q are not
+ * computed, keys behind max_kv do count).  One kernel serves any mix of single tokens and prompts. */
+typedef struct disc_b200_kv8_attention_args {
+  const void* q;   /* f16 / bf16, row stride ld_q */
+  void* out;       /* same type, row stride ld_out; may not overlap q */
+  int64_t tokens, ld_q, ld_out;
+  int32_t q_heads;
+  int32_t type;
+  disc_b200_kv8_cache cache;
+  const int32_t* table; /* [requests, table_width] */
+  const int32_t* q_start;
+  const int32_t* q_lens;
+  const int32_t* kv_lens;
+  int32_t requests, table_width;
+  int32_t max_q, max_kv;
+  float scale;
+} disc_b200_kv8_attention_args;
+int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* args, void* stream);
 
 /* ---- Collectives of the column-parallel (N-split) configuration.
  * One process per GPU.  NCCL is reached through dlopen (the copy already
