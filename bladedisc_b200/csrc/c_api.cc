@@ -537,6 +537,10 @@ int32_t disc_b200_kv8_read(const disc_b200_kv8_read_args* a, void* stream) {
   return finish(st, "kv8_read", detail);
 }
 
+int64_t disc_b200_kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv) {
+  return disc_b200::kv8_attention_workspace_bytes(dim, max_kv);
+}
+
 int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* a, void* stream) {
   if (!a) {
     g_last_error = "kv8_attention: null args";
@@ -559,6 +563,8 @@ int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* a, void* str
   p.max_q = a->max_q;
   p.max_kv = a->max_kv;
   p.scale = a->scale;
+  p.workspace = a->workspace;
+  p.workspace_bytes = a->workspace_bytes;
   p.type = a->type;
   const char* detail = nullptr;
   const cudaError_t st = disc_b200::kv8_attention_launch(p, static_cast<cudaStream_t>(stream), &detail);

@@ -81,7 +81,11 @@ struct Kv8AttentionParams {
   int32_t max_q, max_kv;   // the host's bounds on q_lens and kv_lens
   float scale;
   int32_t type;
+  void* workspace;         // kv8_attention_workspace_bytes, 16-byte aligned
+  int64_t workspace_bytes;
 };
+// Device memory a call on the current device needs: fixed per device and head size, none for short caches.
+int64_t kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv);
 cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t stream, const char** err);
 int kv8_status_fetch_and_clear();
 

@@ -204,7 +204,9 @@ const char* kv8_cache_problem(const Kv8Cache& c) {
   if (c.dim != 64 && c.dim != 128) return "head size must be 64 or 128";
   if (c.block_size != 16 && c.block_size != 32 && c.block_size != 64 && c.block_size != 128)
     return "block size must be 16, 32, 64 or 128";
-  if (static_cast<int64_t>(c.num_blocks) * c.block_size > INT32_MAX) return "slots are 32-bit: too many blocks";
+  if (static_cast<int64_t>(c.num_blocks) * c.block_size > INT32_MAX ||
+      static_cast<int64_t>(c.num_blocks) * c.kv_heads > INT32_MAX)
+    return "slots are 32-bit: too many blocks";
   if (c.num_blocks > 0 && (!c.k || !c.v || !c.k_scale || !c.v_scale)) return "null operand";
   if (misaligned(c.k, 16) || misaligned(c.v, 16)) return "levels must be 16-byte aligned";
   return nullptr;

@@ -36,6 +36,8 @@ __device__ __forceinline__ void store8(T* p, const float* f) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()),
                                             pack2(f[6], f[7], T()));
 }
+__device__ __forceinline__ __half pack_one(float a, __half) { return __float2half_rn(a); }
+__device__ __forceinline__ __nv_bfloat16 pack_one(float a, __nv_bfloat16) { return __float2bfloat16_rn(a); }
 __device__ __forceinline__ float level_of(uint32_t w, int byte) {
   return static_cast<float>(static_cast<int8_t>(w >> (8 * byte)));
 }

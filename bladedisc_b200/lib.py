@@ -117,7 +117,8 @@ class Kv8AttentionArgs(Structure):
         ("q", c_void_p), ("out", c_void_p), ("tokens", c_int64), ("ld_q", c_int64), ("ld_out", c_int64),
         ("q_heads", c_int32), ("type", c_int32), ("cache", Kv8Cache), ("table", c_void_p), ("q_start", c_void_p),
         ("q_lens", c_void_p), ("kv_lens", c_void_p), ("requests", c_int32), ("table_width", c_int32),
-        ("max_q", c_int32), ("max_kv", c_int32), ("scale", c_float),
+        ("max_q", c_int32), ("max_kv", c_int32), ("scale", c_float), ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
     ]
 
 
@@ -181,6 +182,7 @@ SIGNATURES = {
     "disc_b200_kv_blocks_trim": (c_int32, [POINTER(KvBlocksArgs), c_void_p]),
     "disc_b200_kv8_append": (c_int32, [POINTER(Kv8AppendArgs), c_void_p]),
     "disc_b200_kv8_read": (c_int32, [POINTER(Kv8ReadArgs), c_void_p]),
+    "disc_b200_kv8_attention_workspace_bytes": (c_int64, [c_int32, c_int64]),
     "disc_b200_kv8_attention": (c_int32, [POINTER(Kv8AttentionArgs), c_void_p]),
     "disc_b200_nccl_available": (c_int32, []),
     "disc_b200_nccl_unique_id": (c_int32, [c_void_p]),

@@ -724,6 +724,17 @@ def kv8_read(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: t
     return ko, vo
 
 
+_kv8_workspace = {}
+
+
+def _kv8_workspace_bytes(dev: torch.device, dim: int, max_kv: int) -> int:
+    key = (dev.index, dim, max_kv > 512)
+    if key not in _kv8_workspace:
+        with torch.cuda.device(dev):
+            _kv8_workspace[key] = _lib.load().disc_b200_kv8_attention_workspace_bytes(dim, max_kv)
+    return _kv8_workspace[key]
+
+
 def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                   table: torch.Tensor, q_start: torch.Tensor, q_lens: torch.Tensor, kv_lens: torch.Tensor, *,
                   max_q: int, scale: Optional[float] = None, max_kv: Optional[int] = None,
@@ -766,6 +777,10 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
                               q_lens.data_ptr(), kv_lens.data_ptr(), n, table.shape[1], int(max_q),
                               room if max_kv is None else min(int(max_kv), room),
                               dim ** -0.5 if scale is None else float(scale))
+    need = _kv8_workspace_bytes(dev, dim, a.max_kv)
+    if need:  # from torch's allocator: ordered with this stream, a captured graph keeps its own
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
     _call(dev, _lib.load().disc_b200_kv8_attention, a)
     return out
 

@@ -574,7 +574,12 @@ typedef struct disc_b200_kv8_attention_args {
   int32_t requests, table_width;
   int32_t max_q, max_kv;
   float scale;
+  void* workspace; /* device, 16-byte aligned; may be NULL when the size below is 0 */
+  int64_t workspace_bytes;
 } disc_b200_kv8_attention_args;
+/* Workspace of a call with this head size and max_kv on the current device (the same for every batch; 0 for short
+ * caches).  Calls that overlap on the GPU need one each; its contents mean nothing between calls. */
+int64_t disc_b200_kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv);
 int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* args, void* stream);
 
 /* ---- Collectives of the column-parallel (N-split) configuration.
