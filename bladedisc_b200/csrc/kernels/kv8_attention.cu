@@ -20,7 +20,7 @@ namespace {
 // Up to a few dozen query rows per request and kv head: the cache is read once and its bytes are what bounds the
 // kernel, closely followed by the instructions that turn levels into f16.
 //
-// An item is a request, a kv head and 16 query rows (query heads of that kv head, tokens of that request); its work
+// An item is a request, a kv head and 8 or 16 query rows (query heads of that kv head, tokens of that request); its work
 // is steps of 32 keys.  All steps of all items are laid end to end and cut into equal shares, one per CTA, three CTAs
 // per SM: ragged lengths balance to one step.  A share that ends inside an item leaves its partial maximum, sum and
 // output in the workspace, and a second small kernel joins them.  Short caches (max_kv <= kDirectKeys) take one CTA
@@ -29,11 +29,13 @@ namespace {
 // Inside a CTA a warp runs by itself: it fetches its steps with TMA into its own ring, multiplies with mma.sync
 // m16n8k16, keeps running maximum, sum and output in registers and meets the others at the end of the item.
 //
-//   S = Q K^T  the head dimension is permuted alike in Q and K so that a lane's B fragments are the bytes of 16-byte
-//              loads; levels become f16 exactly (byte b as 0x6400 | b + 128 is 1152 + b, one subtraction).
-//   O += P V   a lane's B fragments pair bytes of two keys: two byte permutes, again exact in f16.
+//   S' = K Q'    keys are the wide operand, so that eight query rows fill the instruction (a decode step has one to
+//                eight); the head dimension is permuted alike in K and Q so that a lane's fragments are the bytes of
+//                16-byte loads; levels become f16 exactly (byte b as 0x6400 | b + 128 is 1152 + b, one subtraction).
+//   O' += V' P'  a lane's fragments pair bytes of two keys: two byte permutes, again exact in f16; P changes its
+//                fragment layout with one 8 x 8 transpose.
 // Query rows in bf16 are scaled by a power of two per row to f16 (exact but for values 2^-24 of the row's largest).
-// P goes to f16 with 2^13 of head room so that a probability keeps its 11 bits down to 2^-27 of the largest; the
+// P goes to f16 times 2^11 so that a probability keeps its 11 bits down to 2^-25 of the largest; the
 // value scale is multiplied in relative to a running reference that O is kept in units of.
 // The 128-byte (64-byte for dim 64) swizzle of the TMA boxes and the key order perm(n) = n ^ ((n & 1) << 2) make the
 // 16-byte shared-memory reads free of bank conflicts.
@@ -41,8 +43,9 @@ constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kDirectKeys = 512;  // caches up to this long are not cut
-constexpr float kPScaleLog2 = 13.f;
-constexpr float kRefSlack = 4.f;  // a value scale may exceed the reference by this much before O is rescaled
+constexpr float kPScaleLog2 = 11.f;
+constexpr float kMaxSlack = 2.f;  // a score may exceed the running maximum by this much (in log2) and
+constexpr float kRefSlack = 4.f;  // a value scale the reference by this factor before O is rescaled: P < 2^15
 constexpr float kRef0 = 1e-30f;
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -51,6 +54,12 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t w) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
 }
 
 // Bytes b (as b + 128) `sel` picks two of them -> two f16 with the values b.
@@ -106,8 +115,8 @@ __device__ __forceinline__ float row_power(uint32_t top) {
 
 // What is left of a share that ends inside an item: a maximum, a sum and an output per row.
 struct SplitWs {
-  float* o;      // [2 * ctas][16][dim]: slot 2 c for a piece that does not start its item, 2 c + 1 for one that does
-  float2* ml;    // [2 * ctas][16]
+  float* o;      // [2 * ctas][16 rows][dim]: slot 2 c for a piece that does not start its item, 2 c + 1 for one that does
+  float2* ml;    // [2 * ctas][16 rows]
   int4* desc;    // [ctas] {request, kv head, row tile, pieces} of the item that CTA c starts and does not finish
 };
 
@@ -130,29 +139,29 @@ struct SplitSmem {
 struct Request {
   int q_asked, q_len, kv_len, tiles, steps;
 };
-__device__ __forceinline__ Request request_of(const Kv8AttentionParams& p, int r, int max_rows) {
+__device__ __forceinline__ Request request_of(const Kv8AttentionParams& p, int r, int max_rows, int tile_rows) {
   Request q;
   const int G = p.q_heads / p.cache.kv_heads;
   q.q_asked = max(p.q_lens[r], 0);
   q.q_len = min(q.q_asked, p.max_q);
   q.kv_len = min(max(p.kv_lens[r], 0), p.table_width * p.cache.block_size);
-  const int64_t rows = static_cast<int64_t>(q.q_asked) * G <= max_rows ? static_cast<int64_t>(q.q_len) * G : 0;
-  q.tiles = static_cast<int>((rows + 15) / 16);
+  const int rows = static_cast<int64_t>(q.q_asked) * G <= max_rows ? q.q_len * G : 0;  // q_len <= max_q: fits
+  q.tiles = static_cast<int>(static_cast<uint32_t>(rows + tile_rows - 1) / static_cast<uint32_t>(tile_rows));
   q.steps = max(1, (q.kv_len + kStep - 1) / kStep);
   return q;
 }
 
-template <typename T, int D, bool HI>
+template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(kSplitThreads, 3)
 split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
              const __grid_constant__ Kv8AttentionParams p, SplitShape shape, SplitWs ws) {
   using L = SplitSmem<D>;
   constexpr int W = kSplitWarps, S = L::kStages;
   constexpr int KQ = D / 16;  // k steps of the first product
-  constexpr int NV = D / 8;   // n tiles of the second
-  constexpr int E = HI ? 2 : 1;  // rows per lane: g, and g + 8 when there may be more than eight
+  constexpr int NV = D / 16;  // m tiles of the second
+  constexpr int ROWS = 8 * NQ;
   extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   __shared__ uint64_t bars[W * S];
   __shared__ float part_m[W][16], part_l[W][16];
   __shared__ long long sums[W];
@@ -177,14 +186,14 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
   grid_dep_launch();
 
   // ---- which steps are this CTA's: `left` steps from step `s0` of item `item` of request r on
-  int r;
-  int64_t left, item, s0, total = 0;
+  int r, item, s0;
+  int64_t left, total = 0;
   if (!shape.stream) {
     r = blockIdx.y;
-    const Request q = request_of(p, r, shape.max_rows);
+    const Request q = request_of(p, r, shape.max_rows, ROWS);
     const int tile = blockIdx.x % shape.row_tiles;
     if (tile >= q.tiles) return;
-    item = static_cast<int64_t>(blockIdx.x / shape.row_tiles) * q.tiles + tile;
+    item = static_cast<int>(blockIdx.x / shape.row_tiles) * q.tiles + tile;
     s0 = 0;
     left = q.steps;
   } else {
@@ -192,7 +201,7 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     const int r0 = min(p.requests, static_cast<int>(threadIdx.x) * per), r1 = min(p.requests, r0 + per);
     int64_t mine = 0;
     for (int i = r0; i < r1; ++i) {
-      const Request q = request_of(p, i, shape.max_rows);
+      const Request q = request_of(p, i, shape.max_rows, ROWS);
       mine += static_cast<int64_t>(q.tiles) * KH * q.steps;
     }
     int64_t incl = mine;
@@ -212,7 +221,7 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
     if (left > 0 && begin >= incl - mine && begin < incl) {  // one thread's requests hold the first step
       int64_t at = incl - mine;
       for (int i = r0; i < r1; ++i) {
-        const Request q = request_of(p, i, shape.max_rows);
+        const Request q = request_of(p, i, shape.max_rows, ROWS);
         const int64_t work = static_cast<int64_t>(q.tiles) * KH * q.steps;
         if (begin < at + work) {
           found[0] = i;
@@ -229,11 +238,11 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
       return;
     }
     r = found[0];
-    const Request q = request_of(p, r, shape.max_rows);
-    item = found_at / q.steps;
-    s0 = found_at % q.steps;
+    const Request q = request_of(p, r, shape.max_rows, ROWS);
+    item = static_cast<int>(found_at / q.steps);
+    s0 = static_cast<int>(found_at % q.steps);
   }
-  Request rq = request_of(p, r, shape.max_rows);
+  Request rq = request_of(p, r, shape.max_rows, ROWS);
 
   const uint32_t ring = smem_u32(smem) + warp * (S * 2 * L::kHalf);
   const uint8_t* ring_ptr = smem + warp * (S * 2 * L::kHalf);
@@ -244,37 +253,31 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
   bool ok = true;
 
   while (left > 0) {
-    while (item >= static_cast<int64_t>(rq.tiles) * KH) {  // on to the next request with rows
+    while (item >= rq.tiles * KH) {  // on to the next request with rows
       if (++r >= p.requests) return;  // not with lengths that stay as they are during the call
       item = 0;
-      rq = request_of(p, r, shape.max_rows);
+      rq = request_of(p, r, shape.max_rows, ROWS);
     }
-    const int head = static_cast<int>(item / rq.tiles), tile = static_cast<int>(item % rq.tiles);
+    const int head = item / rq.tiles, tile = item % rq.tiles;
     const int s1 = static_cast<int>(min(static_cast<int64_t>(rq.steps), s0 + left));
-    const int64_t row0 = static_cast<int64_t>(tile) * 16;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(16), static_cast<int64_t>(rq.q_len) * G - row0));
+    const int row0 = tile * ROWS;
+    const int rows = min(ROWS, rq.q_len * G - row0);
     const int64_t tok0 = p.q_start[r];
     const int64_t behind = static_cast<int64_t>(rq.kv_len) - rq.q_asked + 1;
     // keys that the first row of the tile sees, and the last one
     const int lim_first = static_cast<int>(max(static_cast<int64_t>(0), behind + row0 / G));
     const int keys = static_cast<int>(max(static_cast<int64_t>(0), behind + (row0 + rows - 1) / G));
 
-    // Q fragments of rows g and g + 8
-    uint32_t qa[KQ][4];
-    float qmul[E];
-    int lim[E];
+    // Q fragments: this lane loads row 8 j + g; its scores belong to the rows 8 j + 2 t + e
+    uint32_t qb[NQ][KQ][2];
+    float qmul[NQ][2], m[NQ][2], l[NQ][2];
+    int lim[NQ][2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      if (e >= E) {
-#pragma unroll
-        for (int j = 0; j < KQ; ++j) qa[j][1] = qa[j][3] = 0;
-        continue;
-      }
-      const int row = g + 8 * e;
-      const int64_t i = (row0 + row) / G, h = (row0 + row) % G;
+    for (int j = 0; j < NQ; ++j) {
+      const int row = j * 8 + g;
+      const int i = (row0 + row) / G, h = (row0 + row) % G;
       const int64_t at = tok0 + i;
       const bool there = row < rows && at >= 0 && at < p.tokens;
-      lim[e] = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i)) : 0;
       const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q : 0) + (head * G + (there ? h : 0)) * D + 16 * t;
       float mul = 1.f;
       if constexpr (!std::is_same<T, __half>::value) {
@@ -291,22 +294,27 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
         uint32_t w[8];
         load_q16(x + 64 * i2, there, mul, w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          qa[i2 * 4 + j][e] = w[2 * j];
-          qa[i2 * 4 + j][2 + e] = w[2 * j + 1];
+        for (int k = 0; k < 4; ++k) {
+          qb[j][i2 * 4 + k][0] = w[2 * k];
+          qb[j][i2 * 4 + k][1] = w[2 * k + 1];
         }
       }
-      qmul[e] = p.scale * 1.4426950408889634f / mul;
+      const float f = p.scale * 1.4426950408889634f / mul;
+      const int see = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i)) : 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qmul[j][e] = __shfl_sync(~0u, f, (2 * t + e) * 4);
+        lim[j][e] = __shfl_sync(~0u, see, (2 * t + e) * 4);
+        m[j][e] = -INFINITY;
+        l[j][e] = 0.f;
+      }
     }
 
-    float o[NV][4];
+    float o[NQ][NV][4];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[E], l[E];
+    for (int j = 0; j < NQ; ++j) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      m[e] = -INFINITY;
-      l[e] = 0.f;
+      for (int i = 0; i < NV; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
     }
     float ref = kRef0, inv_ref = 1.f / kRef0;
 
@@ -390,44 +398,67 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
       const uint8_t* kt = ring_ptr + stage * 2 * L::kHalf;
       const uint8_t* vt = kt + L::kHalf;
 
-      float s[4][4];
+      float s[2][NQ][4];  // [16 keys][rows]: key g rows 2 t, 2 t + 1, key g + 8 rows 2 t, 2 t + 1
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt) {
-        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-        const int row = nt * 8 + prow;
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 64; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(
-              D == 128 ? kt + row * 128 + (((i * 4 + t) ^ (row & 7)) << 4) : kt + row * 64 + ((t ^ ((row >> 1) & 3)) << 4));
-          const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+          uint4 w[2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            mma_f16(s[nt], qa[i * 4 + j], bytes_to_f16(x[j], 0x4140), bytes_to_f16(x[j], 0x4342));
+          for (int u = 0; u < 2; ++u) {
+            const int row = mt * 16 + u * 8 + prow;
+            w[u] = *reinterpret_cast<const uint4*>(D == 128 ? kt + row * 128 + (((i * 4 + t) ^ (row & 7)) << 4)
+                                                            : kt + row * 64 + ((t ^ ((row >> 1) & 3)) << 4));
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t x = (k == 0 ? w[0].x : k == 1 ? w[0].y : k == 2 ? w[0].z : w[0].w) ^ 0x80808080u;
+            const uint32_t y = (k == 0 ? w[1].x : k == 1 ? w[1].y : k == 2 ? w[1].z : w[1].w) ^ 0x80808080u;
+            const uint32_t a[4] = {bytes_to_f16(x, 0x4140), bytes_to_f16(y, 0x4140), bytes_to_f16(x, 0x4342),
+                                   bytes_to_f16(y, 0x4342)};
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) mma_f16(s[mt][j], a, qb[j][i * 4 + k][0], qb[j][i * 4 + k][1]);
+          }
         }
       }
 
       const int key0 = (first + n * W) * kStep;
       const bool edge = key0 + kStep > lim_first || id0 < 0 || id1 < 0;
-      float mn[E];
-      bool up = false;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float mx = -INFINITY;
+      for (int j = 0; j < NQ; ++j) {
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const float f = qmul[e] * ks[nt >> 1];
+        for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float& x = s[nt][2 * e + j];
-            x *= f;
-            if (edge && (key0 + nt * 8 + (j ? v1 : v0) >= lim[e] || (nt < 2 ? id0 : id1) < 0)) x = -INFINITY;
-            mx = fmaxf(mx, x);
+          for (int e = 0; e < 4; ++e) s[mt][j][e] *= qmul[j][e & 1] * ks[mt];
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + mt * 16 + (e >> 1) * 8 + prow >= lim[j][e & 1] || (mt == 0 ? id0 : id1) < 0)
+                s[mt][j][e] = -INFINITY;
           }
         }
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-        mn[e] = fmaxf(m[e], mx);
-        up = up || mn[e] > m[e];
+      }
+      float mn[NQ][2];
+      bool up = false;
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(s[0][j][e], s[0][j][2 + e]), fmaxf(s[1][j][e], s[1][j][2 + e]));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
+          mn[j][e] = fmaxf(m[j][e], mx);
+          up = up || mn[j][e] > m[j][e] + kMaxSlack;
+        }
       }
       float vtop = vs[0] < INFINITY ? vs[0] : 0.f;
       vtop = vs[1] < INFINITY ? fmaxf(vtop, vs[1]) : vtop;
@@ -440,47 +471,52 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
           inv_ref = 1.f / vtop;
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float a = mn[e] == -INFINITY ? 1.f : exp2_approx(m[e] - mn[e]);
-          m[e] = mn[e];
-          l[e] *= a;
-          a *= down;
+        for (int j = 0; j < NQ; ++j) {
+          float a[2];
 #pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            o[j][2 * e] *= a;
-            o[j][2 * e + 1] *= a;
+          for (int e = 0; e < 2; ++e) {
+            a[e] = mn[j][e] == -INFINITY ? 1.f : exp2_approx(m[j][e] - mn[j][e]);
+            m[j][e] = mn[j][e];
+            l[j][e] *= a[e];
+            a[e] *= down;
+          }
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][i][e] *= a[e & 1];
           }
         }
       }
-      uint32_t pa[2][4];
+      uint32_t pb[2][NQ][2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if (e >= E) {
-          pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0;
-          continue;
-        }
-        const float base = (m[e] == -INFINITY ? 0.f : m[e]) - kPScaleLog2;
+      for (int j = 0; j < NQ; ++j) {
+        const float base[2] = {(m[j][0] == -INFINITY ? 0.f : m[j][0]) - kPScaleLog2,
+                               (m[j][1] == -INFINITY ? 0.f : m[j][1]) - kPScaleLog2};
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt) {
-          const float w = vs[nt >> 1] * inv_ref;
-          float pv[2];
+        for (int mt = 0; mt < 2; ++mt) {
+          const float w = vs[mt] * inv_ref;
+          float pv[4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float x = exp2_approx(s[nt][2 * e + j] - base);
-            l[e] += x;
-            pv[j] = x * w;
-            // whatever the scale is
-            if (edge && (key0 + nt * 8 + (j ? v1 : v0) >= lim[e] || (nt < 2 ? id0 : id1) < 0)) pv[j] = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const float x = exp2_approx(s[mt][j][e] - base[e & 1]);
+            l[j][e & 1] += x;
+            pv[e] = x * w;
           }
-          pa[nt >> 1][(nt & 1) * 2 + e] = pack2(pv[0], pv[1], __half());
+          if (edge) {  // 0 whatever the scale is
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + mt * 16 + (e >> 1) * 8 + prow >= lim[j][e & 1] || (mt == 0 ? id0 : id1) < 0) pv[e] = 0.f;
+          }
+          pb[mt][j][0] = transpose8x8(pack2(pv[0], pv[1], __half()));
+          pb[mt][j][1] = transpose8x8(pack2(pv[2], pv[3], __half()));
         }
       }
 #pragma unroll
-      for (int h2 = 0; h2 < 2; ++h2) {
+      for (int mt = 0; mt < 2; ++mt) {
         uint4 vw[4];  // D = 64 uses the first two words
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = h2 * 16 + (e >> 1) * 8 + ((e & 1) ? v1 : v0);
+          const int row = mt * 16 + (e >> 1) * 8 + ((e & 1) ? v1 : v0);
           if constexpr (D == 128) {
             vw[e] = *reinterpret_cast<const uint4*>(vt + row * 128 + ((g ^ (row & 7)) << 4));
           } else {
@@ -494,12 +530,15 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             x[e] = (q4 == 0 ? vw[e].x : q4 == 1 ? vw[e].y : q4 == 2 ? vw[e].z : vw[e].w) ^ 0x80808080u;
-          const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[0], x[1], 0x7362);
-          const uint32_t b01 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
-          mma_f16(o[q4 * 4 + 0], pa[h2], bytes_to_f16(a01, 0x4140), bytes_to_f16(b01, 0x4140));
-          mma_f16(o[q4 * 4 + 1], pa[h2], bytes_to_f16(a01, 0x4342), bytes_to_f16(b01, 0x4342));
-          mma_f16(o[q4 * 4 + 2], pa[h2], bytes_to_f16(a23, 0x4140), bytes_to_f16(b23, 0x4140));
-          mma_f16(o[q4 * 4 + 3], pa[h2], bytes_to_f16(a23, 0x4342), bytes_to_f16(b23, 0x4342));
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t lo = __byte_perm(x[0], x[1], u ? 0x7362 : 0x5140);
+            const uint32_t hi = __byte_perm(x[2], x[3], u ? 0x7362 : 0x5140);
+            const uint32_t a[4] = {bytes_to_f16(lo, 0x4140), bytes_to_f16(lo, 0x4342), bytes_to_f16(hi, 0x4140),
+                                   bytes_to_f16(hi, 0x4342)};
+#pragma unroll
+            for (int j = 0; j < NQ; ++j) mma_f16(o[j][q4 * 2 + u], a, pb[mt][j][0], pb[mt][j][1]);
+          }
         }
       }
       __syncwarp();  // every lane has its bytes: the stage may be filled again
@@ -518,28 +557,32 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
 
     // ---- the four warps' results become one
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      l[e] += __shfl_xor_sync(~0u, l[e], 1);
-      l[e] += __shfl_xor_sync(~0u, l[e], 2);
-      if (t == 0) {
-        part_m[warp][g + 8 * e] = m[e];
-        part_l[warp][g + 8 * e] = l[e] * exp2f(-kPScaleLog2);
+    for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[j][e] += __shfl_xor_sync(~0u, l[j][e], 4);
+        l[j][e] += __shfl_xor_sync(~0u, l[j][e], 8);
+        l[j][e] += __shfl_xor_sync(~0u, l[j][e], 16);
+        if (g == 0) {
+          part_m[warp][j * 8 + 2 * t + e] = m[j][e];
+          part_l[warp][j * 8 + 2 * t + e] = l[j][e] * exp2f(-kPScaleLog2);
+        }
       }
     }
     __syncthreads();  // no ring is in use: partial outputs take their place
     float* parts = reinterpret_cast<float*>(smem);
     const float unit = ref * exp2f(-kPScaleLog2);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (g + 8 * e < rows) {
-        float* po = parts + (warp * 16 + g + 8 * e) * D;
+    for (int j = 0; j < NQ; ++j) {
 #pragma unroll
-        for (int j = 0; j < NV; j += 4) {
-          *reinterpret_cast<float4*>(po + 2 * t * NV + j) =
-              make_float4(o[j][2 * e] * unit, o[j + 1][2 * e] * unit, o[j + 2][2 * e] * unit, o[j + 3][2 * e] * unit);
-          *reinterpret_cast<float4*>(po + (2 * t + 1) * NV + j) =
-              make_float4(o[j][2 * e + 1] * unit, o[j + 1][2 * e + 1] * unit, o[j + 2][2 * e + 1] * unit,
-                          o[j + 3][2 * e + 1] * unit);
+      for (int e = 0; e < 2; ++e) {
+        const int row = j * 8 + 2 * t + e;
+        if (row < rows) {
+          float4* po = reinterpret_cast<float4*>(parts + (warp * ROWS + row) * D + g * (D / 8));
+#pragma unroll
+          for (int i = 0; i < NV; i += 2)
+            po[i / 2] = make_float4(o[j][i][e] * unit, o[j][i][2 + e] * unit, o[j][i + 1][e] * unit,
+                                    o[j][i + 1][2 + e] * unit);
         }
       }
     }
@@ -556,7 +599,7 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
       for (int w = 0; w < W; ++w) {
         const float a = top == -INFINITY ? 1.f : exp2_approx(part_m[w][row] - top);
         sum += a * part_l[w][row];
-        acc += a * parts[(w * 16 + row) * D + d];
+        acc += a * parts[(w * ROWS + row) * D + d];
       }
       if (whole) {
         const int64_t at = tok0 + (row0 + row) / G;
@@ -583,35 +626,61 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
   }
 }
 
-// Joins the pieces of the item that CTA blockIdx.x of split_kernel started: one block per row.
-template <typename T, int D>
-__global__ void __launch_bounds__(D) join_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, SplitWs ws) {
+// Joins the pieces of the item that CTA blockIdx.x of split_kernel started: one block per row, its groups of D / 4
+// threads take every kJoinThreads / (D / 4)-th piece each.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kJoinThreads)
+join_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, SplitWs ws) {
+  constexpr int GROUPS = kJoinThreads / (D / 4);
+  __shared__ float part[GROUPS][D], part_m[GROUPS], part_l[GROUPS];
   grid_dep_wait();
   grid_dep_launch();
   const int4 it = ws.desc[blockIdx.x];
   if (it.w <= 1) return;
   const int G = p.q_heads / p.cache.kv_heads;
-  const Request q = request_of(p, it.x, shape.max_rows);
-  const int64_t row = static_cast<int64_t>(it.z) * 16 + blockIdx.y;
-  if (row >= static_cast<int64_t>(q.q_len) * G) return;
+  const Request q = request_of(p, it.x, shape.max_rows, ROWS);
+  const int row = it.z * ROWS + blockIdx.y;
+  if (row >= q.q_len * G) return;
   const int64_t at = p.q_start[it.x] + row / G;
   if (at < 0 || at >= p.tokens) return;
   const int64_t c0 = blockIdx.x;
-  float top = -INFINITY, sum = 0.f, acc = 0.f;
+  const int group = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = 0; i < it.w; ++i) {
+  for (int i = group; i < it.w; i += GROUPS) {
     const int64_t slot = ((i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * 16) + blockIdx.y;
     const float2 ml = ws.ml[slot];
+    const float4 v = *reinterpret_cast<const float4*>(ws.o + slot * D + d);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw no key (its output may not even be written)
-    const float v = ws.o[slot * D + threadIdx.x];
     const float mn = fmaxf(top, ml.x);
     const float a = mn == -INFINITY ? 1.f : exp2_approx(top - mn), b = mn == -INFINITY ? 1.f : exp2_approx(ml.x - mn);
     sum = sum * a + ml.y * b;
-    acc = acc * a + v * b;
+    acc = make_float4(acc.x * a + v.x * b, acc.y * a + v.y * b, acc.z * a + v.z * b, acc.w * a + v.w * b);
     top = mn;
   }
+  *reinterpret_cast<float4*>(&part[group][d]) = acc;
+  if (d == 0) {
+    part_m[group] = top;
+    part_l[group] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, part_m[i]);
+  sum = 0.f;
+  float o = 0.f;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const float a = top == -INFINITY ? 1.f : exp2_approx(part_m[i] - top);
+    sum += a * part_l[i];
+    o += a * part[i][threadIdx.x];
+  }
   static_cast<T*>(p.out)[at * p.ld_out + (it.y * G + row % G) * D + threadIdx.x] =
-      pack_one(sum == 0.f ? 0.f : acc / sum, T());
+      pack_one(sum == 0.f ? 0.f : o / sum, T());
 }
 
 bool misaligned(const void* p, uintptr_t by) { return (reinterpret_cast<uintptr_t>(p) & (by - 1)) != 0; }
@@ -638,7 +707,7 @@ int64_t ws_bytes(int ctas, int dim) {
 
 bool wants_stream(const Kv8AttentionParams& p) { return p.max_kv > kDirectKeys; }
 
-template <typename T, int D, bool HI>
+template <typename T, int D, int NQ>
 cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, dim3 grid, cudaStream_t stream,
                          const char** err) {
   CUtensorMap tk, tv;
@@ -656,13 +725,13 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
     at += static_cast<int64_t>(grid.x) * 2 * 16 * 8;
     ws.desc = reinterpret_cast<int4*>(at);
   }
-  auto kern = split_kernel<T, D, HI>;
+  auto kern = split_kernel<T, D, NQ>;
   constexpr int smem = SplitSmem<D>::kDynamic;
   cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (st != cudaSuccess) return st;
   st = launch_dependent(kern, grid, dim3(kSplitThreads), smem, stream, tk, tv, p, shape, ws);
   if (st != cudaSuccess || !shape.stream) return st;
-  return launch_dependent(join_kernel<T, D>, dim3(grid.x, HI ? 16 : 8), dim3(D), 0, stream, p, shape, ws);
+  return launch_dependent(join_kernel<T, D, 8 * NQ>, dim3(grid.x, 8 * NQ), dim3(kJoinThreads), 0, stream, p, shape, ws);
 }
 
 template <typename T, int D>
@@ -671,16 +740,17 @@ cudaError_t launch_t(const Kv8AttentionParams& p, cudaStream_t stream, const cha
   SplitShape shape;
   shape.max_rows = INT32_MAX;
   shape.stream = wants_stream(p) ? 1 : 0;
-  const int64_t tiles = (rows + 15) / 16;
-  if (tiles * p.cache.kv_heads > INT32_MAX) {
+  const int tile_rows = rows > 8 ? 16 : 8;
+  const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
+  if (rows > INT32_MAX - 16 || tiles * p.cache.kv_heads > INT32_MAX) {
     *err = "too many query rows";
     return cudaErrorInvalidValue;
   }
   shape.row_tiles = static_cast<int>(tiles);
   const dim3 grid = shape.stream ? dim3(static_cast<unsigned>(stream_ctas()))
                                  : dim3(static_cast<unsigned>(tiles * p.cache.kv_heads), static_cast<unsigned>(p.requests));
-  return rows > 8 ? launch_split<T, D, true>(p, shape, grid, stream, err)
-                  : launch_split<T, D, false>(p, shape, grid, stream, err);
+  return rows > 8 ? launch_split<T, D, 2>(p, shape, grid, stream, err)
+                  : launch_split<T, D, 1>(p, shape, grid, stream, err);
 }
 
 }  // namespace
