@@ -35,6 +35,7 @@ SOURCES = [
     "kernels/kv_blocks.cu",
     "kernels/kv8_cache.cu",
     "kernels/kv8_attention.cu",
+    "kernels/kv8_prefill.cu",
     "ral/conv_plan.cc",
     "ral/metadata.cc",
     "ral/cu_driver_dyn.cc",
@@ -44,7 +45,7 @@ SOURCES = [
     "c_api.cc",
 ]
 HEADERS = [
-    "kernels/qgemm.h", "kernels/rowops.h", "kernels/woq_gemm.h", "kernels/qconv.h", "kernels/observer.h", "kernels/attention.h", "kernels/kv8.h", "kernels/kv8_types.cuh", "ral/conv_plan.h", "kernels/sm100_ptx.cuh", "kernels/device_info.h", "kernels/tensor_map.h",
+    "kernels/qgemm.h", "kernels/rowops.h", "kernels/woq_gemm.h", "kernels/qconv.h", "kernels/observer.h", "kernels/attention.h", "kernels/kv8.h", "kernels/kv8_types.cuh", "kernels/kv8_attention.cuh", "ral/conv_plan.h", "kernels/sm100_ptx.cuh", "kernels/device_info.h", "kernels/tensor_map.h",
     "kernels/qgemm_pair.inl", "kernels/qgemm_gemv.inl", "kernels/qgemm_skinny.inl",
     "kernels/rownorm_staged.inl",
     "ral/abi.h", "ral/context.h", "ral/pdl_attr.h", "ral/nccl_dyn.h", "ral/metadata.h", "ral/cu_driver_dyn.h",

@@ -3,12 +3,11 @@
 //   o_i  = sum_j softmax(s_i)_j * v_scale[block(j)] * v_j,   0 where row i sees no key.
 #include "kv8.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #include "device_info.h"
-#include "kv8_types.cuh"
-#include "sm100_ptx.cuh"
-#include "tensor_map.h"
+#include "kv8_attention.cuh"
 
 namespace disc_b200 {
 
@@ -42,6 +41,7 @@ namespace {
 constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
+constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one
 constexpr int kDirectKeys = 512;  // caches up to this long are not cut
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // a score may exceed the running maximum by this much (in log2) and
@@ -60,20 +60,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t w) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
   return r;
-}
-
-// Bytes b (as b + 128) `sel` picks two of them -> two f16 with the values b.
-__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t biased, uint32_t sel) {
-  const uint32_t w = __byte_perm(biased, 0x64646464u, sel);
-  const uint32_t c = 0x64806480u;  // 1152
-  const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(&c));
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Sixteen consecutive 16-bit values of a query row as f16 words; returns nothing for a row that is not there.
@@ -97,22 +83,6 @@ __device__ __forceinline__ void load_q16(const __nv_bfloat16* p, bool there, flo
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = pack2(f[2 * i] * mul, f[2 * i + 1] * mul, __half());
 }
-// Largest magnitude of sixteen values, as its bits.
-__device__ __forceinline__ uint32_t top_q16(const __nv_bfloat16* p) {
-  float f[16];
-  load8(p, f);
-  load8(p + 8, f + 8);
-  uint32_t t = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) t = max(t, __float_as_uint(f[i]) & 0x7fffffffu);
-  return t;
-}
-// 2^n that brings a row with this largest magnitude to [2^13, 2^14); n stays within what a float holds.
-__device__ __forceinline__ float row_power(uint32_t top) {
-  const int n = min(max(13 - (static_cast<int>(top >> 23) - 127), -120), 120);
-  return __uint_as_float(static_cast<uint32_t>(n + 127) << 23);
-}
-
 // What is left of a share that ends inside an item: a maximum, a sum and an output per row.
 struct SplitWs {
   float* o;      // [2 * ctas][16 rows][dim]: slot 2 c for a piece that does not start its item, 2 c + 1 for one that does
@@ -145,7 +115,7 @@ __device__ __forceinline__ Request request_of(const Kv8AttentionParams& p, int r
   q.q_asked = max(p.q_lens[r], 0);
   q.q_len = min(q.q_asked, p.max_q);
   q.kv_len = min(max(p.kv_lens[r], 0), p.table_width * p.cache.block_size);
-  const int rows = static_cast<int64_t>(q.q_asked) * G <= max_rows ? q.q_len * G : 0;  // q_len <= max_q: fits
+  const int rows = q.q_len * G <= max_rows ? q.q_len * G : 0;  // q_len <= max_q: fits
   q.tiles = static_cast<int>(static_cast<uint32_t>(rows + tile_rows - 1) / static_cast<uint32_t>(tile_rows));
   q.steps = max(1, (q.kv_len + kStep - 1) / kStep);
   return q;
@@ -685,27 +655,11 @@ join_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spli
 
 bool misaligned(const void* p, uintptr_t by) { return (reinterpret_cast<uintptr_t>(p) & (by - 1)) != 0; }
 
-// One box is `rows` tokens of one block and head.
-bool make_map(CUtensorMap* tm, const int8_t* base, const Kv8Cache& c, int rows) {
-  EncodeTiledFn fn = tensor_map_encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[3] = {static_cast<cuuint64_t>(c.dim), static_cast<cuuint64_t>(c.block_size),
-                        static_cast<cuuint64_t>(c.num_blocks) * c.kv_heads};
-  cuuint64_t strides[2] = {static_cast<cuuint64_t>(c.dim), static_cast<cuuint64_t>(c.dim) * c.block_size};
-  cuuint32_t box[3] = {static_cast<cuuint32_t>(c.dim), static_cast<cuuint32_t>(rows), 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  return fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, c.dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 int stream_ctas() { return 3 * device_sm_count(); }
 
 int64_t ws_bytes(int ctas, int dim) {
   return static_cast<int64_t>(ctas) * (2 * 16 * (static_cast<int64_t>(dim) * 4 + 8) + 16);
 }
-
-bool wants_stream(const Kv8AttentionParams& p) { return p.max_kv > kDirectKeys; }
 
 template <typename T, int D, int NQ>
 cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, dim3 grid, cudaStream_t stream,
@@ -735,20 +689,16 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
 }
 
 template <typename T, int D>
-cudaError_t launch_t(const Kv8AttentionParams& p, cudaStream_t stream, const char** err) {
-  const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
+cudaError_t launch_t(const Kv8AttentionParams& p, int max_rows, cudaStream_t stream, const char** err) {
+  const int64_t rows = std::min(static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads), static_cast<int64_t>(max_rows));
   SplitShape shape;
-  shape.max_rows = INT32_MAX;
-  shape.stream = wants_stream(p) ? 1 : 0;
+  shape.max_rows = max_rows;
+  shape.stream = p.max_kv > kDirectKeys ? 1 : 0;
   const int tile_rows = rows > 8 ? 16 : 8;
-  const int64_t tiles = (rows + tile_rows - 1) / tile_rows;
-  if (rows > INT32_MAX - 16 || tiles * p.cache.kv_heads > INT32_MAX) {
-    *err = "too many query rows";
-    return cudaErrorInvalidValue;
-  }
-  shape.row_tiles = static_cast<int>(tiles);
+  shape.row_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
   const dim3 grid = shape.stream ? dim3(static_cast<unsigned>(stream_ctas()))
-                                 : dim3(static_cast<unsigned>(tiles * p.cache.kv_heads), static_cast<unsigned>(p.requests));
+                                 : dim3(static_cast<unsigned>(shape.row_tiles * p.cache.kv_heads),
+                                        static_cast<unsigned>(p.requests));
   return rows > 8 ? launch_split<T, D, 2>(p, shape, grid, stream, err)
                   : launch_split<T, D, 1>(p, shape, grid, stream, err);
 }
@@ -781,15 +731,23 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   else if (!(p.scale > 0.f))
     *err = "the score scale must be positive";
   if (*err) return cudaErrorInvalidValue;
-  if (wants_stream(p) && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < ws_bytes(stream_ctas(), p.cache.dim)))
+  // Which requests go where is decided on the device, from q_lens; the host knows the bound.
+  const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
+  const bool many = rows > kSplitRows, few = !many || p.requests > 1;
+  if (few && p.max_kv > kDirectKeys && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < ws_bytes(stream_ctas(), p.cache.dim)))
     *err = "the workspace is too small or not 16-byte aligned";
   if (p.table_width == 0) {  // no keys at all, but the kernel's tensor maps want a cache
     if (p.cache.num_blocks == 0) *err = "a cache without blocks";
   }
   if (*err) return cudaErrorInvalidValue;
+  if (many) {
+    const cudaError_t st = kv8_prefill_launch(p, few ? kSplitRows : 0, stream, err);
+    if (st != cudaSuccess || !few) return st;
+  }
+  const bool f16 = p.type == kKvF16;
   if (p.cache.dim == 128)
-    return p.type == kKvF16 ? launch_t<__half, 128>(p, stream, err) : launch_t<__nv_bfloat16, 128>(p, stream, err);
-  return p.type == kKvF16 ? launch_t<__half, 64>(p, stream, err) : launch_t<__nv_bfloat16, 64>(p, stream, err);
+    return f16 ? launch_t<__half, 128>(p, kSplitRows, stream, err) : launch_t<__nv_bfloat16, 128>(p, kSplitRows, stream, err);
+  return f16 ? launch_t<__half, 64>(p, kSplitRows, stream, err) : launch_t<__nv_bfloat16, 64>(p, kSplitRows, stream, err);
 }
 
 int kv8_status_fetch_and_clear() {
@@ -799,7 +757,8 @@ int kv8_status_fetch_and_clear() {
     int z = 0;
     cudaMemcpyToSymbol(g_kv8_status, &z, sizeof(int));
   }
-  return h;
+  const int f = kv8_prefill_status_fetch_and_clear();
+  return h != 0 ? h : f;
 }
 
 }  // namespace disc_b200

@@ -1,0 +1,580 @@
+// Attention over the 8-bit cache for many query rows per request and kv head: prompts and chunks of them.
+//
+// A CTA owns 256 query rows (tokens x heads of one kv head) as two tiles of 128 and walks the keys in tiles of 128.
+// Its warps:
+//   loader       looks up blocks and scales of the next key tile and fetches its levels with TMA
+//   converters   levels -> f16 (exact) in the 128-byte swizzled layout of the tensor core's operands; the rows of a
+//                tile are keys, 64 values wide, which reads as K-major for Q K^T and as MN-major for P V alike
+//   two issuers  one thread per query tile: S = Q K^T and O += P V with tcgen05.mma kind::f16, O in TMEM, P as the
+//                TMEM operand in the columns that S had.  Each waits for its own chain only, so that one tile's
+//                products run while the other tile is in its softmax.
+//   softmax      a warpgroup per query tile, a thread per row: running maximum in the scale of log2, exp2, sums in
+//                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
+// Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
+// loader keeps (O is in its units), so that P stays in the range of f16; see kPScaleLog2.
+// Bound by the tensor core and, as closely, by exp2: at dim 128 a tile of 128 x 128 costs 1024 cycles of products
+// and 1024 cycles of the SM's 16 exp2 per cycle.
+#include "kv8.h"
+
+#include <type_traits>
+
+#include "device_info.h"
+#include "kv8_attention.cuh"
+
+namespace disc_b200 {
+
+__device__ int g_kv8_prefill_status = 0;
+
+namespace {
+
+constexpr int kTile = 128;               // query rows of a tile and keys of a tile
+constexpr int kGroups = kTile / 16;      // scale groups of a key tile
+constexpr int kSoftmaxWarps = 4;         // per query tile
+constexpr int kConvWarps = 4;
+constexpr int kLoaderWarp = 2 * kSoftmaxWarps + kConvWarps;
+constexpr int kIssueWarp = kLoaderWarp + 1;
+constexpr int kThreads = (kIssueWarp + 2) * 32;
+constexpr int kInfo = 4;                 // key tiles whose scales are held
+constexpr float kPScaleLog2 = 8.f;       // P = 2^8 p: 11 bits down to 2^-22 of the row's (stale) maximum
+constexpr float kSlack = 5.f;            // a maximum may be stale by 2^5 and
+constexpr float kRefSlack = 4.f;         // a value scale above the reference by 4: P < 2^15
+constexpr float kRef0 = 1e-30f;
+constexpr int kSubTile = kTile * 128;    // 128 rows of 64 f16
+
+struct TileInfo {
+  float f[kGroups];   // key scale * softmax scale * log2 e
+  float w[kGroups];   // value scale / reference
+  float down;         // old reference / new one
+  float ref;
+  uint32_t there;     // bit per group: the block exists and has keys that some row sees
+  uint32_t pad;
+};
+
+template <int D>
+struct Smem {
+  static constexpr int kSub = D / 64;
+  static constexpr int kOp = kSub * kSubTile;       // a [128 x D] f16 operand
+  static constexpr int kRaw = kTile * D;            // a tile of levels
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQ + 2 * kOp;           // two buffers
+  static constexpr int kV = kK + 2 * kOp;           // two buffers
+  static constexpr int kRawK = kV + 2 * kOp;
+  static constexpr int kRawV = kRawK + kRaw;
+  static constexpr int kInfoAt = kRawV + kRaw;
+  static constexpr int kBars = kInfoAt + kInfo * static_cast<int>(sizeof(TileInfo));
+  // q_full[2], raw_full[2], raw_free[2], k_full[2], v_full[2], k_free[2], v_free[2], s_full[2], p_full[2], pv_done[2],
+  // info_full[4]
+  static constexpr int kNumBars = 20 + kInfo;
+  static constexpr int kMisc = kBars + kNumBars * 8;
+  static constexpr int kTotal = kMisc + 16;
+  static constexpr int kDynamic = kTotal + 1024;
+};
+static_assert(Smem<128>::kDynamic <= 227 * 1024, "shared memory of one SM");
+
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// A from TMEM: lane = row, a 32-bit column holds two consecutive k.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// D f32, A and B f16, B MN-major with bit 16; N >> 3 at [17, 23), M >> 4 at [24, 29).
+__host__ __device__ constexpr uint32_t f16_idesc(int n, bool b_mn_major) {
+  return (1u << 4) | (b_mn_major ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+// MN-major operand, 128-byte swizzle: rows are k indices of 64 n, groups of 8 rows 1024 bytes apart, the next 64 n
+// one sub-tile further.
+__device__ __forceinline__ uint64_t mn_major_desc(uint32_t addr) {
+  uint64_t d = (addr & 0x3FFFF) >> 4;
+  d |= static_cast<uint64_t>(kSubTile >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+               const __grid_constant__ Kv8AttentionParams p, int min_rows, int box_rows) {
+  using L = Smem<D>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  const uint32_t base = smem_u32(smem);
+  const uint32_t bars = base + L::kBars;
+  auto bar = [&](int i, int j) { return bars + 8u * (2 * i + j); };
+  auto q_full = [&](int q) { return bar(0, q); };
+  auto raw_full = [&](int v) { return bar(1, v); };
+  auto raw_free = [&](int v) { return bar(2, v); };
+  auto op_full = [&](int v, int b) { return bar(3 + v, b); };
+  auto op_free = [&](int v, int b) { return bar(5 + v, b); };
+  auto s_full = [&](int q) { return bar(7, q); };
+  auto p_full = [&](int q) { return bar(8, q); };
+  auto pv_done = [&](int q) { return bar(9, q); };
+  auto info_full = [&](int i) { return bars + 8u * (20 + i); };
+  TileInfo* info = reinterpret_cast<TileInfo*>(smem + L::kInfoAt);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Kv8Cache& c = p.cache;
+  const int bs = c.block_size, G = p.q_heads / c.kv_heads;
+
+  // ---- the item: heads vary fastest, the rows with the most keys come first
+  grid_dep_wait();
+  grid_dep_launch();
+  const int head = blockIdx.x, r = blockIdx.z;
+  const int q_asked = max(p.q_lens[r], 0);
+  const int q_len = min(q_asked, p.max_q);
+  const int rows_all = q_len * G;  // max_q * G fits
+  const int row0 = (gridDim.y - 1 - blockIdx.y) * 2 * kTile;
+  if (rows_all <= min_rows || row0 >= rows_all) return;
+  const int rows = min(2 * kTile, rows_all - row0);
+  const int kv_len = min(max(p.kv_lens[r], 0), p.table_width * bs);
+  const int64_t behind = static_cast<int64_t>(kv_len) - q_asked + 1;  // token i sees behind + i keys
+  const int keys = static_cast<int>(max(static_cast<int64_t>(0), behind + (row0 + rows - 1) / G));
+  const int nt = (keys + kTile - 1) / kTile;
+  const int64_t tok0 = p.q_start[r];
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tk);
+    tma_prefetch_desc(&tv);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full(i), kSoftmaxWarps);
+      mbar_init(raw_full(i), 1);
+      mbar_init(raw_free(i), kConvWarps);
+      mbar_init(s_full(i), 1);
+      mbar_init(p_full(i), kSoftmaxWarps);
+      mbar_init(pv_done(i), 1);
+      for (int v = 0; v < 2; ++v) {
+        mbar_init(op_full(v, i), kConvWarps);
+        mbar_init(op_free(v, i), 2);
+      }
+    }
+    for (int i = 0; i < kInfo; ++i) mbar_init(info_full(i), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == kIssueWarp) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint32_t b, uint32_t parity, int code) {
+    return mbar_wait(b, parity, abort_flag, &g_kv8_prefill_status, code);
+  };
+
+  if (warp < 2 * kSoftmaxWarps) {
+    // ------------------------------------------------------------------ softmax: a thread per row
+    const int q = warp / kSoftmaxWarps;
+    const int row = (warp % kSoftmaxWarps) * 32 + lane;
+    const int my_row = row0 + q * kTile + row;
+    const bool valid = q * kTile + row < rows;
+    const int i_tok = my_row / G, h = my_row % G;
+    const int64_t at = tok0 + i_tok;
+    const bool there = valid && at >= 0 && at < p.tokens;
+    // a row that is not there computes along and is not stored
+    const int lim = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i_tok)) : INT32_MAX;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp % kSoftmaxWarps) * 32) << 16);
+    const uint32_t t_s = t_lane + q * kTile, t_p = t_s, t_o = t_lane + 256 + q * D;
+    const bool active = q * kTile < rows;
+    float mul = 1.f;
+    if (active && nt > 0) {
+      const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q + (head * G + h) * D : 0);
+      if constexpr (!std::is_same<T, __half>::value) {
+        uint32_t top = 0;
+        if (there)
+#pragma unroll
+          for (int d = 0; d < D; d += 16) top = max(top, top_q16(x + d));
+        mul = row_power(top);
+      }
+      uint8_t* dst = smem + L::kQ + q * L::kOp + row * 128;
+#pragma unroll
+      for (int d = 0; d < D; d += 8) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (there) {
+          w = *reinterpret_cast<const uint4*>(x + d);
+          if constexpr (!std::is_same<T, __half>::value) {
+            float f[8];
+            load8(x + d, f);
+            w = make_uint4(pack2(f[0] * mul, f[1] * mul, __half()), pack2(f[2] * mul, f[3] * mul, __half()),
+                           pack2(f[4] * mul, f[5] * mul, __half()), pack2(f[6] * mul, f[7] * mul, __half()));
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + (d / 64) * kSubTile + (((d % 64 / 8) ^ (row & 7)) << 4)) = w;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full(q));
+    }
+    const float rmul = p.scale * 1.4426950408889634f / mul;
+    // the first key tile in which some row of this warp does not see every key
+    const int first_masked = __reduce_min_sync(~0u, lim) / kTile;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int t = 0; t < nt && active; ++t) {
+      ok = wait(info_full(t % kInfo), (t / kInfo) & 1, 51) && wait(s_full(q), t & 1, 52);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const TileInfo& in = info[t % kInfo];
+      const uint32_t present = in.there;
+      const bool edge = t >= first_masked || present != (1u << kGroups) - 1;
+      const int key0 = t * kTile;
+
+      float mx = -INFINITY;
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        uint32_t s[32];
+        tmem_ld_x32(t_s + cc * 32, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          float top = -INFINITY;
+          if (!edge) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, __uint_as_float(s[g * 16 + e]));
+          } else if (present >> (cc * 2 + g) & 1) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (key0 + cc * 32 + g * 16 + e < lim) top = fmaxf(top, __uint_as_float(s[g * 16 + e]));
+          }
+          const float v = top * in.f[cc * 2 + g];
+          mx = fmaxf(mx, top == -INFINITY ? -INFINITY : v);
+        }
+      }
+      mx *= rmul;
+      const float mn = fmaxf(m, mx);
+      const bool up = mn > m + kSlack;
+      const float down = in.down;
+      if (__any_sync(~0u, up) || down != 1.f) {
+        // a row that stays keeps its maximum: its factor is the reference's alone
+        float a = down;
+        if (up) {
+          const float k = exp2_approx(m - mn);
+          l *= k;
+          a *= k;
+          m = mn;
+        }
+        if (t > 0) {
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o[32];
+            tmem_ld_x32(t_o + cc * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+            tmem_st_x16(t_o + cc * 32, o);
+            tmem_st_x16(t_o + cc * 32 + 16, o + 16);
+          }
+        }
+      }
+      const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        uint32_t s[32], w[16];
+        tmem_ld_x32(t_s + cc * 32, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float f = in.f[cc * 2 + g] * rmul, vw = in.w[cc * 2 + g];
+          if (!edge) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float a = exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e]), f, off));
+              const float b = exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e + 1]), f, off));
+              l += a + b;
+              w[g * 8 + e] = pack2(a * vw, b * vw, __half());
+            }
+          } else {
+            const bool in_cache = present >> (cc * 2 + g) & 1;
+            const int left = in_cache ? lim - (key0 + cc * 32 + g * 16) : 0;  // keys of the group that this row sees
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float a = 2 * e < left ? exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e]), f, off)) : 0.f;
+              const float b = 2 * e + 1 < left ? exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e + 1]), f, off)) : 0.f;
+              l += a + b;
+              w[g * 8 + e] = pack2(2 * e < left ? a * vw : 0.f, 2 * e + 1 < left ? b * vw : 0.f, __half());
+            }
+          }
+        }
+        tmem_st_x16(t_p + cc * 16, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(q));
+    }
+    // ---- epilogue
+    if (active) {
+      T* dst = static_cast<T*>(p.out) + (there ? at * p.ld_out + (head * G + h) * D : 0);
+      if (nt == 0) {
+        if (there)
+#pragma unroll
+          for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+      } else {
+        if (ok) ok = wait(pv_done(q), (nt - 1) & 1, 53);
+        ok = __all_sync(~0u, ok);
+        if (ok) {
+          tc_fence_after();
+          const float k = l == 0.f ? 0.f : info[(nt - 1) % kInfo].ref / l;
+#pragma unroll
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t o[32];
+            tmem_ld_x32(t_o + cc * 32, o);
+            tmem_ld_wait();
+            if (there) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = l == 0.f ? 0.f : __uint_as_float(o[e + j]) * k;
+                store8(dst + cc * 32 + e, f);
+              }
+            }
+          }
+        }
+      }
+    }
+  } else if (warp < kLoaderWarp) {
+    // ------------------------------------------------------------------ converters: 32 keys of a tile per warp
+    const int w = warp - 2 * kSoftmaxWarps;
+    const int piece = lane & 3;
+    bool ok = true;
+    for (int t = 0; t < nt && ok; ++t) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int b = t & 1;
+        ok = wait(raw_full(v), t & 1, 54);
+        if (ok && t >= 2) ok = wait(op_free(v, b), ((t >> 1) - 1) & 1, 55);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        const uint8_t* src = smem + (v ? L::kRawV : L::kRawK);
+        uint8_t* dst = smem + (v ? L::kV : L::kK) + b * L::kOp;
+        // a quarter warp reads four 16-byte pieces of two keys and writes them as 32 bytes each; which half of a
+        // 128-value row it takes alternates with the key, so that neither side meets in a bank
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = D == 128 ? w * 32 + j * 8 + (lane >> 3) * 2 + ((lane >> 2) & 1) : w * 32 + j * 8 + (lane >> 2);
+#pragma unroll
+          for (int i = 0; i < L::kSub; ++i) {
+            const int sub = D == 128 ? i ^ (key & 1) : 0;
+            const uint4 x = *reinterpret_cast<const uint4*>(
+                D == 128 ? src + key * 128 + (((sub * 4 + piece) ^ (key & 7)) << 4)
+                         : src + key * 64 + ((piece ^ ((key >> 1) & 3)) << 4));
+            uint32_t y[8];
+            const uint32_t in4[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              y[2 * e] = bytes_to_f16(in4[e], 0x4140);
+              y[2 * e + 1] = bytes_to_f16(in4[e], 0x4342);
+            }
+            uint8_t* o = dst + sub * kSubTile + key * 128;
+            *reinterpret_cast<uint4*>(o + (((2 * piece) ^ (key & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(o + (((2 * piece + 1) ^ (key & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(op_full(v, b));
+          mbar_arrive(raw_free(v));
+        }
+      }
+    }
+  } else if (warp == kLoaderWarp) {
+    // ------------------------------------------------------------------ loader: lane g < 8 knows group g of the tile
+    float ref = kRef0;
+    bool ok = true;
+    int id = -1;
+    float ks = 0.f, vs = 0.f;
+    auto lookup = [&](int t) {
+      const int key = t * kTile + lane * 16;
+      id = -1;
+      ks = vs = 0.f;
+      if (lane < kGroups && key < keys) {
+        const int b = p.table[static_cast<int64_t>(r) * p.table_width + key / bs];
+        if (b >= 0 && b < c.num_blocks) {
+          id = b;
+          ks = c.k_scale[static_cast<int64_t>(b) * c.kv_heads + head];
+          vs = c.v_scale[static_cast<int64_t>(b) * c.kv_heads + head];
+        }
+      }
+    };
+    const int boxes = kTile / box_rows, per_box = box_rows / 16;
+    if (nt > 0) lookup(0);
+    for (int t = 0; t < nt; ++t) {
+      const int id_now = id;
+      const float ks_now = ks, vs_now = vs;
+      if (t + 1 < nt) lookup(t + 1);
+      if (t > 0) ok = wait(raw_free(0), (t - 1) & 1, 56);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      // Tile t - 4, whose entry this overwrites, is done with: the keys of tile t - 1 are converted, so the scores
+      // of tile t - 3 are complete for both query tiles, and they were begun after P of tile t - 4 was there.
+      float top = vs_now < INFINITY ? vs_now : 0.f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+      top = __shfl_sync(~0u, top, 0);
+      float down = 1.f;
+      if (top > kRefSlack * ref) {
+        down = ref / top;
+        ref = top;
+      }
+      const uint32_t there = __ballot_sync(~0u, id_now >= 0);
+      TileInfo& in = info[t % kInfo];
+      if (lane < kGroups) {
+        in.f[lane] = ks_now;
+        in.w[lane] = vs_now / ref;
+      }
+      if (lane == 0) {
+        in.down = down;
+        in.ref = ref;
+        in.there = there;
+      }
+      __syncwarp();
+      const int box_id = __shfl_sync(~0u, id_now, (lane * per_box) & 31);
+      const bool mine = lane < boxes && box_id >= 0;
+      const uint32_t bytes = __popc(__ballot_sync(~0u, mine)) * box_rows * D;
+      const int off = bs > kTile ? 0 : (t * kTile + lane * box_rows) & (bs - 1);
+      if (lane == 0) {
+        mbar_arrive(info_full(t % kInfo));
+        mbar_arrive_expect_tx(raw_full(0), bytes);
+      }
+      __syncwarp();
+      if (mine) tma_load_3d(base + L::kRawK + lane * box_rows * D, &tk, raw_full(0), 0, off, box_id * c.kv_heads + head);
+      if (t > 0) ok = wait(raw_free(1), (t - 1) & 1, 57);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(raw_full(1), bytes);
+      __syncwarp();
+      if (mine) tma_load_3d(base + L::kRawV + lane * box_rows * D, &tv, raw_full(1), 0, off, box_id * c.kv_heads + head);
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------------ issuers: one thread per query tile
+    const int q = warp - kIssueWarp;
+    const bool active = q * kTile < rows;
+    constexpr uint32_t idesc_s = f16_idesc(kTile, false);
+    constexpr uint32_t idesc_o = f16_idesc(D, true);
+    const uint32_t t_s = tmem + q * kTile, t_p = t_s, t_o = tmem + 256 + q * D;
+    const uint32_t q_at = base + L::kQ + q * L::kOp;
+    bool ok = true;
+    if (active && nt > 0) ok = wait(q_full(q), 0, 58);
+    for (int t = 0; t < nt && ok; ++t) {
+      const int b = t & 1;
+      const uint32_t round = (t >> 1) & 1;
+      ok = wait(op_full(0, b), round, 59);
+      if (!ok) break;
+      if (!active) {  // the other tile alone decides when the operands are free
+        mbar_arrive(op_free(0, b));
+        ok = wait(op_full(1, b), round, 60);
+        if (ok) mbar_arrive(op_free(1, b));
+        continue;
+      }
+      // the columns of S hold P of the tile before until its product with V is done
+      if (t > 0) ok = wait(pv_done(q), (t - 1) & 1, 61);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t k_at = base + L::kK + b * L::kOp;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t step = (kk >> 2) * kSubTile;
+        umma_f16_ss(t_s, make_kmajor_sw128_desc(q_at + step) + 2 * (kk & 3), make_kmajor_sw128_desc(k_at + step) + 2 * (kk & 3),
+                    idesc_s, kk != 0 ? 1u : 0u);
+      }
+      umma_commit(s_full(q));
+      umma_commit(op_free(0, b));
+      ok = wait(op_full(1, b), round, 62);
+      if (ok) ok = wait(p_full(q), t & 1, 63);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t v_at = base + L::kV + b * L::kOp;
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; ++kk)
+        umma_f16_ts(t_o, t_p + kk * 8, mn_major_desc(v_at + kk * 16 * 128), idesc_o, (t | kk) != 0 ? 1u : 0u);
+      umma_commit(pv_done(q));
+      umma_commit(op_free(1, b));
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) {  // let copies and products in flight end before shared memory and TMEM are given back
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssueWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
+  const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
+  const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile);
+  if (rows > INT32_MAX - 2 * kTile || blocks > 65535) {
+    *err = "too many query rows";
+    return cudaErrorInvalidValue;
+  }
+  CUtensorMap tk, tv;
+  const int box = p.cache.block_size < kTile ? p.cache.block_size : kTile;
+  if (!make_map(&tk, p.cache.k, p.cache, box) || !make_map(&tv, p.cache.v, p.cache, box)) {
+    *err = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  auto kern = prefill_kernel<T, D>;
+  constexpr int smem = Smem<D>::kDynamic;
+  cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (st != cudaSuccess) return st;
+  const dim3 grid(static_cast<unsigned>(p.cache.kv_heads), static_cast<unsigned>(blocks),
+                  static_cast<unsigned>(p.requests));
+  return launch_dependent(kern, grid, dim3(kThreads), smem, stream, tk, tv, p, min_rows, box);
+}
+
+}  // namespace
+
+cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
+  if (p.cache.dim == 128)
+    return p.type == kKvF16 ? launch_t<__half, 128>(p, min_rows, stream, err)
+                            : launch_t<__nv_bfloat16, 128>(p, min_rows, stream, err);
+  return p.type == kKvF16 ? launch_t<__half, 64>(p, min_rows, stream, err)
+                          : launch_t<__nv_bfloat16, 64>(p, min_rows, stream, err);
+}
+
+int kv8_prefill_status_fetch_and_clear() {
+  int h = 0;
+  if (cudaMemcpyFromSymbol(&h, g_kv8_prefill_status, sizeof(int)) != cudaSuccess) return -1;
+  if (h != 0) {
+    int z = 0;
+    cudaMemcpyToSymbol(g_kv8_prefill_status, &z, sizeof(int));
+  }
+  return h;
+}
+
+}  // namespace disc_b200
