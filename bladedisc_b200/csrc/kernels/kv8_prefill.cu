@@ -5,9 +5,9 @@
 //   loader       looks up blocks and scales of the next key tile and fetches its levels with TMA
 //   converters   levels -> f16 (exact) in the 128-byte swizzled layout of the tensor core's operands; the rows of a
 //                tile are keys, 64 values wide, which reads as K-major for Q K^T and as MN-major for P V alike
-//   two issuers  one thread per query tile: S = Q K^T and O += P V with tcgen05.mma kind::f16, O in TMEM, P as the
-//                TMEM operand in the columns that S had.  Each waits for its own chain only, so that one tile's
-//                products run while the other tile is in its softmax.
+//   issuer       one thread: S = Q K^T and O += P V with tcgen05.mma kind::f16, O in TMEM, P as the TMEM operand in
+//                the columns that S had.  O += P V and the next S of a query tile follow one another, so that one
+//                tile is in its products while the other is in its softmax.
 //   softmax      a warpgroup per query tile, a thread per row: running maximum in the scale of log2, exp2, sums in
 //                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
 // Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
@@ -33,7 +33,10 @@ constexpr int kSoftmaxWarps = 4;         // per query tile
 constexpr int kConvWarps = 4;
 constexpr int kLoaderWarp = 2 * kSoftmaxWarps + kConvWarps;
 constexpr int kIssueWarp = kLoaderWarp + 1;
-constexpr int kThreads = (kIssueWarp + 2) * 32;
+constexpr int kThreads = 16 * 32;         // four warpgroups; the last warp only keeps its group whole
+// Registers per thread: the launch gives 128 to each; the softmax groups hold a whole row of scores.
+constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * (65536 / kThreads), "what setmaxnreg hands out was launched");
 constexpr int kInfo = 4;                 // key tiles whose scales are held
 constexpr float kPScaleLog2 = 8.f;       // P = 2^8 p: 11 bits down to 2^-22 of the row's (stale) maximum
 constexpr float kSlack = 5.f;            // a maximum may be stale by 2^5 and
@@ -113,6 +116,88 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// The wait for loads in flight, tied to the registers of one of them: nothing that reads them moves before it.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max16(const uint32_t* s) {
+  auto f = [&](int i) { return __uint_as_float(s[i]); };
+  const float a = max3(f(0), f(1), f(2)), b = max3(f(3), f(4), f(5)), c = max3(f(6), f(7), f(8));
+  const float d = max3(f(9), f(10), f(11)), e = max3(f(12), f(13), f(14));
+  return max3(max3(a, b, c), max3(d, e, f(15)), -INFINITY);
+}
+// Scores of one row and key tile -> P in TMEM and the row's sum.  EDGE: some keys are hidden from some rows.
+// `left` keys are visible from the tile's first on; groups that are not `present` are not.
+template <bool EDGE>
+__device__ __forceinline__ void softmax_tile(uint32_t* s, const TileInfo& in, float rmul, float off, uint32_t t_p,
+                                             int left, uint32_t present, uint64_t* sum) {
+  const uint64_t off2 = pair(off, off);
+#pragma unroll
+  for (int cc = 0; cc < 4; ++cc) {
+    uint32_t w[16];
+#pragma unroll
+    for (int g = cc * 2; g < cc * 2 + 2; ++g) {
+      const float f = in.f[g] * rmul, vw = in.w[g];
+      const uint64_t f2 = pair(f, f), w2 = pair(vw, vw);
+      const int see = EDGE ? ((present >> g & 1) ? left - g * 16 : 0) : 16;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float a, b;
+        unpair(fma2(pair(__uint_as_float(s[g * 16 + 2 * e]), __uint_as_float(s[g * 16 + 2 * e + 1])), f2, off2), a, b);
+        a = exp2_approx(a);
+        b = exp2_approx(b);
+        if (EDGE) {
+          if (2 * e >= see) a = 0.f;
+          if (2 * e + 1 >= see) b = 0.f;
+        }
+        const uint64_t ab = pair(a, b);
+        sum[e & 1] = add2(sum[e & 1], ab);
+        unpair(mul2(ab, w2), a, b);
+        if (EDGE) {  // 0 whatever the scale is
+          if (2 * e >= see) a = 0.f;
+          if (2 * e + 1 >= see) b = 0.f;
+        }
+        w[(g & 1) * 8 + e] = pack2(a, b, __half());
+      }
+    }
+    tmem_st_x16(t_p + cc * 16, w);
+  }
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <typename T, int D>
@@ -169,7 +254,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       mbar_init(pv_done(i), 1);
       for (int v = 0; v < 2; ++v) {
         mbar_init(op_full(v, i), kConvWarps);
-        mbar_init(op_free(v, i), 2);
+        mbar_init(op_free(v, i), 1);
       }
     }
     for (int i = 0; i < kInfo; ++i) mbar_init(info_full(i), 1);
@@ -189,6 +274,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   };
 
   if (warp < 2 * kSoftmaxWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------------ softmax: a thread per row
     const int q = warp / kSoftmaxWarps;
     const int row = (warp % kSoftmaxWarps) * 32 + lane;
@@ -234,7 +320,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const float rmul = p.scale * 1.4426950408889634f / mul;
     // the first key tile in which some row of this warp does not see every key
     const int first_masked = __reduce_min_sync(~0u, lim) / kTile;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;
+    uint64_t sum[2] = {0, 0};  // four partial sums
     bool ok = true;
     for (int t = 0; t < nt && active; ++t) {
       ok = wait(info_full(t % kInfo), (t / kInfo) & 1, 51) && wait(s_full(q), t & 1, 52);
@@ -246,25 +333,23 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       const bool edge = t >= first_masked || present != (1u << kGroups) - 1;
       const int key0 = t * kTile;
 
+      uint32_t s[kTile];
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) tmem_ld_x32(t_s + cc * 32, s + cc * 32);
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) tmem_ld_wait32(s + cc * 32);
       float mx = -INFINITY;
+      if (!edge) {
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        uint32_t s[32];
-        tmem_ld_x32(t_s + cc * 32, s);
-        tmem_ld_wait();
+        for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, max16(s + g * 16) * in.f[g]);
+      } else {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < kGroups; ++g) {
+          const int see = (present >> g & 1) ? lim - key0 - g * 16 : 0;
           float top = -INFINITY;
-          if (!edge) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, __uint_as_float(s[g * 16 + e]));
-          } else if (present >> (cc * 2 + g) & 1) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (key0 + cc * 32 + g * 16 + e < lim) top = fmaxf(top, __uint_as_float(s[g * 16 + e]));
-          }
-          const float v = top * in.f[cc * 2 + g];
-          mx = fmaxf(mx, top == -INFINITY ? -INFINITY : v);
+          for (int e = 0; e < 16; ++e) top = e < see ? fmaxf(top, __uint_as_float(s[g * 16 + e])) : top;
+          mx = see > 0 ? fmaxf(mx, top * in.f[g]) : mx;
         }
       }
       mx *= rmul;
@@ -276,54 +361,26 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         float a = down;
         if (up) {
           const float k = exp2_approx(m - mn);
-          l *= k;
+          sum[0] = mul2(sum[0], pair(k, k));
+          sum[1] = mul2(sum[1], pair(k, k));
           a *= k;
           m = mn;
         }
         if (t > 0) {
 #pragma unroll
-          for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o[32];
-            tmem_ld_x32(t_o + cc * 32, o);
-            tmem_ld_wait();
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t o[16];
+            tmem_ld_x16(t_o + cc * 16, o);
+            tmem_ld_wait_regs(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
-            tmem_st_x16(t_o + cc * 32, o);
-            tmem_st_x16(t_o + cc * 32 + 16, o + 16);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+            tmem_st_x16(t_o + cc * 16, o);
           }
         }
       }
       const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        uint32_t s[32], w[16];
-        tmem_ld_x32(t_s + cc * 32, s);
-        tmem_ld_wait();
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float f = in.f[cc * 2 + g] * rmul, vw = in.w[cc * 2 + g];
-          if (!edge) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e]), f, off));
-              const float b = exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e + 1]), f, off));
-              l += a + b;
-              w[g * 8 + e] = pack2(a * vw, b * vw, __half());
-            }
-          } else {
-            const bool in_cache = present >> (cc * 2 + g) & 1;
-            const int left = in_cache ? lim - (key0 + cc * 32 + g * 16) : 0;  // keys of the group that this row sees
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = 2 * e < left ? exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e]), f, off)) : 0.f;
-              const float b = 2 * e + 1 < left ? exp2_approx(fmaf(__uint_as_float(s[g * 16 + 2 * e + 1]), f, off)) : 0.f;
-              l += a + b;
-              w[g * 8 + e] = pack2(2 * e < left ? a * vw : 0.f, 2 * e + 1 < left ? b * vw : 0.f, __half());
-            }
-          }
-        }
-        tmem_st_x16(t_p + cc * 16, w);
-      }
+      if (!edge) softmax_tile<false>(s, in, rmul, off, t_p, 0, 0, sum);
+      else softmax_tile<true>(s, in, rmul, off, t_p, lim - key0, present, sum);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -341,12 +398,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         ok = __all_sync(~0u, ok);
         if (ok) {
           tc_fence_after();
+          float a, b;
+          unpair(add2(sum[0], sum[1]), a, b);
+          const float l = a + b;
           const float k = l == 0.f ? 0.f : info[(nt - 1) % kInfo].ref / l;
 #pragma unroll
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t o[32];
             tmem_ld_x32(t_o + cc * 32, o);
-            tmem_ld_wait();
+            tmem_ld_wait32(o);
             if (there) {
 #pragma unroll
               for (int e = 0; e < 32; e += 8) {
@@ -360,7 +420,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
       }
     }
-  } else if (warp < kLoaderWarp) {
+  } else {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp < kLoaderWarp) {
     // ------------------------------------------------------------------ converters: 32 keys of a tile per warp
     const int w = warp - 2 * kSoftmaxWarps;
     const int piece = lane & 3;
@@ -474,51 +536,52 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       __syncwarp();
       if (mine) tma_load_3d(base + L::kRawV + lane * box_rows * D, &tv, raw_full(1), 0, off, box_id * c.kv_heads + head);
     }
-  } else if (lane == 0) {
-    // ------------------------------------------------------------------ issuers: one thread per query tile
-    const int q = warp - kIssueWarp;
-    const bool active = q * kTile < rows;
+  } else if (warp == kIssueWarp && lane == 0) {
+    // ------------------------------------------------------------------ issuer: one thread for both query tiles
+    const int tiles = rows > kTile ? 2 : 1;
     constexpr uint32_t idesc_s = f16_idesc(kTile, false);
     constexpr uint32_t idesc_o = f16_idesc(D, true);
-    const uint32_t t_s = tmem + q * kTile, t_p = t_s, t_o = tmem + 256 + q * D;
-    const uint32_t q_at = base + L::kQ + q * L::kOp;
     bool ok = true;
-    if (active && nt > 0) ok = wait(q_full(q), 0, 58);
-    for (int t = 0; t < nt && ok; ++t) {
+    // S of key tile t for query tile q; its columns hold P of the tile before until its product with V is done
+    auto scores = [&](int q, int t) {
       const int b = t & 1;
-      const uint32_t round = (t >> 1) & 1;
-      ok = wait(op_full(0, b), round, 59);
-      if (!ok) break;
-      if (!active) {  // the other tile alone decides when the operands are free
-        mbar_arrive(op_free(0, b));
-        ok = wait(op_full(1, b), round, 60);
-        if (ok) mbar_arrive(op_free(1, b));
-        continue;
-      }
-      // the columns of S hold P of the tile before until its product with V is done
-      if (t > 0) ok = wait(pv_done(q), (t - 1) & 1, 61);
-      if (!ok) break;
+      if (q == 0) ok = ok && wait(op_full(0, b), (t >> 1) & 1, 59);
+      if (t > 0) ok = ok && wait(pv_done(q), (t - 1) & 1, 61);
+      if (!ok) return;
       tc_fence_after();
-      const uint32_t k_at = base + L::kK + b * L::kOp;
+      const uint32_t q_at = base + L::kQ + q * L::kOp, k_at = base + L::kK + b * L::kOp;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint32_t step = (kk >> 2) * kSubTile;
-        umma_f16_ss(t_s, make_kmajor_sw128_desc(q_at + step) + 2 * (kk & 3), make_kmajor_sw128_desc(k_at + step) + 2 * (kk & 3),
-                    idesc_s, kk != 0 ? 1u : 0u);
+        umma_f16_ss(tmem + q * kTile, make_kmajor_sw128_desc(q_at + step) + 2 * (kk & 3),
+                    make_kmajor_sw128_desc(k_at + step) + 2 * (kk & 3), idesc_s, kk != 0 ? 1u : 0u);
       }
       umma_commit(s_full(q));
-      umma_commit(op_free(0, b));
-      ok = wait(op_full(1, b), round, 62);
-      if (ok) ok = wait(p_full(q), t & 1, 63);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t v_at = base + L::kV + b * L::kOp;
-#pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk)
-        umma_f16_ts(t_o, t_p + kk * 8, mn_major_desc(v_at + kk * 16 * 128), idesc_o, (t | kk) != 0 ? 1u : 0u);
-      umma_commit(pv_done(q));
-      umma_commit(op_free(1, b));
+      if (q == tiles - 1) umma_commit(op_free(0, b));
+    };
+    for (int q = 0; q < tiles && ok && nt > 0; ++q) {
+      ok = wait(q_full(q), 0, 58);
+      scores(q, 0);
     }
+    for (int t = 0; t < nt && ok; ++t) {
+      const int b = t & 1;
+      for (int q = 0; q < tiles && ok; ++q) {
+        if (q == 0) ok = wait(op_full(1, b), (t >> 1) & 1, 62);
+        if (ok) ok = wait(p_full(q), t & 1, 63 + q);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v_at = base + L::kV + b * L::kOp, t_p = tmem + q * kTile, t_o = tmem + 256 + q * D;
+#pragma unroll
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          umma_f16_ts(t_o, t_p + kk * 8, mn_major_desc(v_at + kk * 16 * 128), idesc_o, (t | kk) != 0 ? 1u : 0u);
+        umma_commit(pv_done(q));
+        if (q == tiles - 1) umma_commit(op_free(1, b));
+        // the next scores of this tile at once, before the other tile's P is looked at: its softmax then runs while
+        // the other tile is in its products
+        if (t + 1 < nt) scores(q, t + 1);
+      }
+    }
+  }
   }
 
   __syncwarp();
