@@ -1,13 +1,14 @@
 // Attention over the 8-bit cache for many query rows per request and kv head: prompts and chunks of them.
 //
-// A CTA owns 256 query rows (tokens x heads of one kv head) as two tiles of 128 and walks the keys in tiles of 128.
-// Its warps:
+// A CTA owns 256 query rows (tokens x heads of one kv head) as two tiles of 128 and walks the keys in tiles of 128,
+// in two steps of 64 each.  Its warps:
 //   loader       looks up blocks and scales of the next key tile and fetches its levels with TMA
 //   converters   levels -> f16 (exact) in the 128-byte swizzled layout of the tensor core's operands; the rows of a
 //                tile are keys, 64 values wide, which reads as K-major for Q K^T and as MN-major for P V alike
-//   issuer       one thread: S = Q K^T and O += P V with tcgen05.mma kind::f16, O in TMEM, P as the TMEM operand in
-//                the columns that S had.  O += P V and the next S of a query tile follow one another, so that one
-//                tile is in its products while the other is in its softmax.
+//   two issuers  one thread per query tile: S = Q K^T and O += P V with tcgen05.mma kind::f16; O in TMEM, S in two
+//                buffers of 64 columns per query tile, P as the TMEM operand in the columns that its S had.  The
+//                scores of step u + 1 are there before the softmax of step u ends; while one tile's thread waits the
+//                other tile's products run.
 //   softmax      a warpgroup per query tile, a thread per row: running maximum in the scale of log2, exp2, sums in
 //                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
 // Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
@@ -28,14 +29,16 @@ __device__ int g_kv8_prefill_status = 0;
 namespace {
 
 constexpr int kTile = 128;               // query rows of a tile and keys of a tile
+constexpr int kKeys = 64;                // keys of a step
 constexpr int kGroups = kTile / 16;      // scale groups of a key tile
+constexpr int kStepGroups = kKeys / 16;
 constexpr int kSoftmaxWarps = 4;         // per query tile
 constexpr int kConvWarps = 4;
 constexpr int kLoaderWarp = 2 * kSoftmaxWarps + kConvWarps;
 constexpr int kIssueWarp = kLoaderWarp + 1;
-constexpr int kThreads = 16 * 32;         // four warpgroups; the last warp only keeps its group whole
-// Registers per thread: the launch gives 128 to each; the softmax groups hold a whole row of scores.
-constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
+constexpr int kThreads = 16 * 32;         // four warpgroups; the last two warps only keep theirs whole
+// Registers per thread: the launch gives 128 to each; the softmax groups hold a step's scores and P.
+constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * (65536 / kThreads), "what setmaxnreg hands out was launched");
 constexpr int kInfo = 4;                 // key tiles whose scales are held
 constexpr float kPScaleLog2 = 8.f;       // P = 2^8 p: 11 bits down to 2^-22 of the row's (stale) maximum
@@ -65,15 +68,39 @@ struct Smem {
   static constexpr int kRawV = kRawK + kRaw;
   static constexpr int kInfoAt = kRawV + kRaw;
   static constexpr int kBars = kInfoAt + kInfo * static_cast<int>(sizeof(TileInfo));
-  // q_full[2], raw_full[2], raw_free[2], k_full[2], v_full[2], k_free[2], v_free[2], s_full[2], p_full[2], pv_done[2],
-  // info_full[4]
-  static constexpr int kNumBars = 20 + kInfo;
+  // q_full[2], raw_full[2], raw_free[2], op_full[2][2], op_free[2][2], s_full[2][2], p_full[2][2], pv_done[2][2],
+  // info_full[4], turn[2][4]
+  static constexpr int kNumBars = 26 + kInfo + 2 * kSoftmaxWarps;
   static constexpr int kMisc = kBars + kNumBars * 8;
   static constexpr int kTotal = kMisc + 16;
   static constexpr int kDynamic = kTotal + 1024;
 };
 static_assert(Smem<128>::kDynamic <= 227 * 1024, "shared memory of one SM");
 
+// 32 bytes at once: a whole sector per lane.
+__device__ __forceinline__ void ldg256(const void* p, uint32_t* r) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void stg256(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// One lane of a converged warp, the same each time.  Products and commits behind it, in code that the whole warp runs
+// with uniform values, issue back to back; behind `lane == 0` each commit cost 180 cycles of the tensor core.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(r));
+  return r != 0;
+}
 __device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t"
@@ -161,26 +188,55 @@ __device__ __forceinline__ float max16(const uint32_t* s) {
   const float d = max3(f(9), f(10), f(11)), e = max3(f(12), f(13), f(14));
   return max3(max3(a, b, c), max3(d, e, f(15)), -INFINITY);
 }
-// Scores of one row and key tile -> P in TMEM and the row's sum.  EDGE: some keys are hidden from some rows.
-// `left` keys are visible from the tile's first on; groups that are not `present` are not.
+// 2^x for a pair on the FMA pipe: x = n + f with |f| <= 1/2 by adding 1.5 2^23, a polynomial of degree 5 in f (the
+// minimax one, relative error 2^-22.6), n into the exponent.  Below 2^-125 the result stays there.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f), minus = pair(-12582912.f, -12582912.f);
+  const uint64_t r = add2(x, magic);
+  const uint64_t f = fma2(add2(r, minus), pair(-1.f, -1.f), x);
+  uint64_t y = pair(1.327647129073739e-3f, 1.327647129073739e-3f);
+  y = fma2(y, f, pair(9.675540961325169e-3f, 9.675540961325169e-3f));
+  y = fma2(y, f, pair(5.550713092088699e-2f, 5.550713092088699e-2f));
+  y = fma2(y, f, pair(2.4022120237350464e-1f, 2.4022120237350464e-1f));
+  y = fma2(y, f, pair(6.931469440460205e-1f, 6.931469440460205e-1f));
+  y = fma2(y, f, pair(1.0000001192092896f, 1.0000001192092896f));
+  float n0, n1;
+  unpair(r, n0, n1);
+  unpair(y, a, b);
+  return pair(__uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23)),
+              __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23)));
+}
+// Scores of one row and step -> P in TMEM and the row's sum.  EDGE: some keys are hidden from some rows.
+// `left` keys are visible from the step's first on; groups that are not `present` are not.
+#ifndef POLY
+#define POLY 0x20
+#endif
 template <bool EDGE>
-__device__ __forceinline__ void softmax_tile(uint32_t* s, const TileInfo& in, float rmul, float off, uint32_t t_p,
+__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, float rmul, float off, uint32_t t_p,
                                              int left, uint32_t present, uint64_t* sum) {
   const uint64_t off2 = pair(off, off);
 #pragma unroll
-  for (int cc = 0; cc < 4; ++cc) {
+  for (int cc = 0; cc < kKeys / 32; ++cc) {
     uint32_t w[16];
 #pragma unroll
     for (int g = cc * 2; g < cc * 2 + 2; ++g) {
-      const float f = in.f[g] * rmul, vw = in.w[g];
+      const float f = fs[g] * rmul, vw = ws[g];
       const uint64_t f2 = pair(f, f), w2 = pair(vw, vw);
       const int see = EDGE ? ((present >> g & 1) ? left - g * 16 : 0) : 16;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float a, b;
-        unpair(fma2(pair(__uint_as_float(s[g * 16 + 2 * e]), __uint_as_float(s[g * 16 + 2 * e + 1])), f2, off2), a, b);
-        a = exp2_approx(a);
-        b = exp2_approx(b);
+        const uint64_t x = fma2(pair(__uint_as_float(s[g * 16 + 2 * e]), __uint_as_float(s[g * 16 + 2 * e + 1])), f2, off2);
+        if (!EDGE && (POLY >> e & 1)) {
+          unpair(exp2_pair(x), a, b);
+        } else {
+          unpair(x, a, b);
+          a = exp2_approx(a);
+          b = exp2_approx(b);
+        }
         if (EDGE) {
           if (2 * e >= see) a = 0.f;
           if (2 * e + 1 >= see) b = 0.f;
@@ -203,7 +259,7 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-               const __grid_constant__ Kv8AttentionParams p, int min_rows, int box_rows) {
+               const __grid_constant__ Kv8AttentionParams p, int min_rows, int box_rows, int wide) {
   using L = Smem<D>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -215,14 +271,16 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   auto raw_free = [&](int v) { return bar(2, v); };
   auto op_full = [&](int v, int b) { return bar(3 + v, b); };
   auto op_free = [&](int v, int b) { return bar(5 + v, b); };
-  auto s_full = [&](int q) { return bar(7, q); };
-  auto p_full = [&](int q) { return bar(8, q); };
-  auto pv_done = [&](int q) { return bar(9, q); };
-  auto info_full = [&](int i) { return bars + 8u * (20 + i); };
+  // of query tile q and step u (two buffers)
+  auto s_full = [&](int q, int u) { return bar(7 + q, u & 1); };
+  auto p_full = [&](int q, int u) { return bar(9 + q, u & 1); };
+  auto pv_done = [&](int q, int u) { return bar(11 + q, u & 1); };
+  auto info_full = [&](int i) { return bars + 8u * (26 + i); };
+  auto turn = [&](int q, int w) { return bars + 8u * (26 + kInfo + q * kSoftmaxWarps + w); };
   TileInfo* info = reinterpret_cast<TileInfo*>(smem + L::kInfoAt);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const Kv8Cache& c = p.cache;
   const int bs = c.block_size, G = p.q_heads / c.kv_heads;
 
@@ -239,7 +297,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   const int kv_len = min(max(p.kv_lens[r], 0), p.table_width * bs);
   const int64_t behind = static_cast<int64_t>(kv_len) - q_asked + 1;  // token i sees behind + i keys
   const int keys = static_cast<int>(max(static_cast<int64_t>(0), behind + (row0 + rows - 1) / G));
-  const int nt = (keys + kTile - 1) / kTile;
+  const int nt = (keys + kTile - 1) / kTile, nu = (keys + kKeys - 1) / kKeys;
   const int64_t tok0 = p.q_start[r];
 
   if (threadIdx.x == 0) {
@@ -249,15 +307,16 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       mbar_init(q_full(i), kSoftmaxWarps);
       mbar_init(raw_full(i), 1);
       mbar_init(raw_free(i), kConvWarps);
-      mbar_init(s_full(i), 1);
-      mbar_init(p_full(i), kSoftmaxWarps);
-      mbar_init(pv_done(i), 1);
       for (int v = 0; v < 2; ++v) {
+        mbar_init(s_full(v, i), 1);
+        mbar_init(p_full(v, i), kSoftmaxWarps);
+        mbar_init(pv_done(v, i), 1);
         mbar_init(op_full(v, i), kConvWarps);
-        mbar_init(op_free(v, i), 1);
+        mbar_init(op_free(v, i), 2);
       }
     }
     for (int i = 0; i < kInfo; ++i) mbar_init(info_full(i), 1);
+    for (int i = 0; i < 2 * kSoftmaxWarps; ++i) mbar_init(turn(0, i), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -268,7 +327,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(~0u, *tmem_slot, 0);
   auto wait = [&](uint32_t b, uint32_t parity, int code) {
     return mbar_wait(b, parity, abort_flag, &g_kv8_prefill_status, code);
   };
@@ -286,76 +345,92 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     // a row that is not there computes along and is not stored
     const int lim = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i_tok)) : INT32_MAX;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp % kSoftmaxWarps) * 32) << 16);
-    const uint32_t t_s = t_lane + q * kTile, t_p = t_s, t_o = t_lane + 256 + q * D;
-    const bool active = q * kTile < rows;
+    const uint32_t t_o = t_lane + 256 + q * D;
+    const bool active = q * kTile < rows, both = false;
     float mul = 1.f;
     if (active && nt > 0) {
       const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q + (head * G + h) * D : 0);
+      uint32_t w[D / 2];
+      if (there) {
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) ldg256(x + 16 * i, w + 8 * i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = *reinterpret_cast<const uint4*>(x + 8 * i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) w[i] = 0;
+      }
       if constexpr (!std::is_same<T, __half>::value) {
         uint32_t top = 0;
-        if (there)
 #pragma unroll
-          for (int d = 0; d < D; d += 16) top = max(top, top_q16(x + d));
-        mul = row_power(top);
+        for (int i = 0; i < D / 2; ++i) top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
+        mul = row_power(top << 16);
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) {
+          float a, b;
+          unpack2(w[i], a, b, T());
+          w[i] = pack2(a * mul, b * mul, __half());
+        }
       }
       uint8_t* dst = smem + L::kQ + q * L::kOp + row * 128;
 #pragma unroll
-      for (int d = 0; d < D; d += 8) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (there) {
-          w = *reinterpret_cast<const uint4*>(x + d);
-          if constexpr (!std::is_same<T, __half>::value) {
-            float f[8];
-            load8(x + d, f);
-            w = make_uint4(pack2(f[0] * mul, f[1] * mul, __half()), pack2(f[2] * mul, f[3] * mul, __half()),
-                           pack2(f[4] * mul, f[5] * mul, __half()), pack2(f[6] * mul, f[7] * mul, __half()));
-          }
-        }
-        *reinterpret_cast<uint4*>(dst + (d / 64) * kSubTile + (((d % 64 / 8) ^ (row & 7)) << 4)) = w;
-      }
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<uint4*>(dst + (i / 8) * kSubTile + (((i % 8) ^ (row & 7)) << 4)) =
+            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full(q));
     }
     const float rmul = p.scale * 1.4426950408889634f / mul;
-    // the first key tile in which some row of this warp does not see every key
-    const int first_masked = __reduce_min_sync(~0u, lim) / kTile;
+    // the first step in which some row of this warp does not see every key
+    const int first_masked = __reduce_min_sync(~0u, lim) / kKeys;
     float m = -INFINITY;
     uint64_t sum[2] = {0, 0};  // four partial sums
     bool ok = true;
-    for (int t = 0; t < nt && active; ++t) {
-      ok = wait(info_full(t % kInfo), (t / kInfo) & 1, 51) && wait(s_full(q), t & 1, 52);
+    for (int u = 0; u < nu && active; ++u) {
+      const int t = u >> 1, first_group = (u & 1) * kStepGroups;
+      if ((u & 1) == 0) ok = wait(info_full(t % kInfo), (t / kInfo) & 1, 51);
+      ok = ok && wait(s_full(q, u), (u >> 1) & 1, 52);
       ok = __all_sync(~0u, ok);
       if (!ok) break;
       tc_fence_after();
       const TileInfo& in = info[t % kInfo];
-      const uint32_t present = in.there;
-      const bool edge = t >= first_masked || present != (1u << kGroups) - 1;
-      const int key0 = t * kTile;
-
-      uint32_t s[kTile];
+      const uint32_t t_s = t_lane + q * kTile + (u & 1) * kKeys;
+      uint32_t s[kKeys];
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) tmem_ld_x32(t_s + cc * 32, s + cc * 32);
+      for (int cc = 0; cc < kKeys / 32; ++cc) tmem_ld_x32(t_s + cc * 32, s + cc * 32);
+      float fs[kStepGroups], ws[kStepGroups];
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) tmem_ld_wait32(s + cc * 32);
+      for (int g = 0; g < kStepGroups; ++g) {
+        fs[g] = in.f[first_group + g];
+        ws[g] = in.w[first_group + g];
+      }
+      const uint32_t present = in.there >> first_group & ((1u << kStepGroups) - 1);
+      const float down = (u & 1) == 0 ? in.down : 1.f;
+      const bool edge = u >= first_masked || present != (1u << kStepGroups) - 1;
+      const int key0 = u * kKeys;
+#pragma unroll
+      for (int cc = 0; cc < kKeys / 32; ++cc) tmem_ld_wait32(s + cc * 32);
       float mx = -INFINITY;
       if (!edge) {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) mx = fmaxf(mx, max16(s + g * 16) * in.f[g]);
+        for (int g = 0; g < kStepGroups; ++g) mx = fmaxf(mx, max16(s + g * 16) * fs[g]);
       } else {
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
+        for (int g = 0; g < kStepGroups; ++g) {
           const int see = (present >> g & 1) ? lim - key0 - g * 16 : 0;
           float top = -INFINITY;
 #pragma unroll
           for (int e = 0; e < 16; ++e) top = e < see ? fmaxf(top, __uint_as_float(s[g * 16 + e])) : top;
-          mx = see > 0 ? fmaxf(mx, top * in.f[g]) : mx;
+          mx = see > 0 ? fmaxf(mx, top * fs[g]) : mx;
         }
       }
       mx *= rmul;
       const float mn = fmaxf(m, mx);
       const bool up = mn > m + kSlack;
-      const float down = in.down;
       if (__any_sync(~0u, up) || down != 1.f) {
         // a row that stays keeps its maximum: its factor is the reference's alone
         float a = down;
@@ -366,7 +441,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           a *= k;
           m = mn;
         }
-        if (t > 0) {
+        if (u > 0) {
+          ok = wait(pv_done(q, u - 1), ((u - 1) >> 1) & 1, 65);  // nothing is being added to O
+          ok = __all_sync(~0u, ok);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int cc = 0; cc < D / 16; ++cc) {
             uint32_t o[16];
@@ -379,12 +458,20 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
       }
       const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
-      if (!edge) softmax_tile<false>(s, in, rmul, off, t_p, 0, 0, sum);
-      else softmax_tile<true>(s, in, rmul, off, t_p, lim - key0, present, sum);
+      // the exponentials of the two query tiles take turns: while one warp of a scheduler is in them the other loads
+      // its scores and finds its maximum
+      if (both && (q == 1 || u > 0)) {
+        ok = wait(turn(q, warp % kSoftmaxWarps), (q == 1 ? u : u - 1) & 1, 66);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+      }
+      if (!edge) softmax_step<false>(s, fs, ws, rmul, off, t_s, 0, 0, sum);
+      else softmax_step<true>(s, fs, ws, rmul, off, t_s, lim - key0, present, sum);
+      if (both && lane == 0) mbar_arrive(turn(q ^ 1, warp % kSoftmaxWarps));
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(q));
+      if (lane == 0) mbar_arrive(p_full(q, u));
     }
     // ---- epilogue
     if (active) {
@@ -394,7 +481,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 #pragma unroll
           for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
       } else {
-        if (ok) ok = wait(pv_done(q), (nt - 1) & 1, 53);
+        if (ok) ok = wait(pv_done(q, nu - 1), ((nu - 1) >> 1) & 1, 53);
         ok = __all_sync(~0u, ok);
         if (ok) {
           tc_fence_after();
@@ -409,11 +496,19 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
             tmem_ld_wait32(o);
             if (there) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                float f[8];
+              for (int e = 0; e < 32; e += 16) {
+                uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = l == 0.f ? 0.f : __uint_as_float(o[e + j]) * k;
-                store8(dst + cc * 32 + e, f);
+                for (int j = 0; j < 8; ++j) {
+                  const float x = __uint_as_float(o[e + 2 * j]) * k, y = __uint_as_float(o[e + 2 * j + 1]) * k;
+                  w[j] = l == 0.f ? 0u : pack2(x, y, T());
+                }
+                if (wide) {
+                  stg256(dst + cc * 32 + e, w);
+                } else {
+                  *reinterpret_cast<uint4*>(dst + cc * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                  *reinterpret_cast<uint4*>(dst + cc * 32 + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                }
               }
             }
           }
@@ -472,33 +567,45 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     // ------------------------------------------------------------------ loader: lane g < 8 knows group g of the tile
     float ref = kRef0;
     bool ok = true;
-    int id = -1;
-    float ks = 0.f, vs = 0.f;
-    auto lookup = [&](int t) {
+    auto block_of = [&](int t) {  // -1: no such block, or no key of the group is seen
       const int key = t * kTile + lane * 16;
-      id = -1;
-      ks = vs = 0.f;
-      if (lane < kGroups && key < keys) {
+      int id = -1;
+      if (t < nt && lane < kGroups && key < keys) {
         const int b = p.table[static_cast<int64_t>(r) * p.table_width + key / bs];
-        if (b >= 0 && b < c.num_blocks) {
-          id = b;
-          ks = c.k_scale[static_cast<int64_t>(b) * c.kv_heads + head];
-          vs = c.v_scale[static_cast<int64_t>(b) * c.kv_heads + head];
-        }
+        if (b >= 0 && b < c.num_blocks) id = b;
       }
+      return id;
     };
     const int boxes = kTile / box_rows, per_box = box_rows / 16;
-    if (nt > 0) lookup(0);
+    int id = block_of(0);
     for (int t = 0; t < nt; ++t) {
-      const int id_now = id;
-      const float ks_now = ks, vs_now = vs;
-      if (t + 1 < nt) lookup(t + 1);
+      const int box_id = __shfl_sync(~0u, id, (lane * per_box) & 31);
+      const bool mine = lane < boxes && box_id >= 0;
+      const uint32_t bytes = __popc(__ballot_sync(~0u, mine)) * box_rows * D;
+      const int off = (t * kTile + lane * box_rows) & (bs - 1);
       if (t > 0) ok = wait(raw_free(0), (t - 1) & 1, 56);
       ok = __all_sync(~0u, ok);
       if (!ok) break;
-      // Tile t - 4, whose entry this overwrites, is done with: the keys of tile t - 1 are converted, so the scores
-      // of tile t - 3 are complete for both query tiles, and they were begun after P of tile t - 4 was there.
-      float top = vs_now < INFINITY ? vs_now : 0.f;
+      if (lane == 0) mbar_arrive_expect_tx(raw_full(0), bytes);
+      __syncwarp();
+      if (mine) tma_load_3d(base + L::kRawK + lane * box_rows * D, &tk, raw_full(0), 0, off, box_id * c.kv_heads + head);
+      // while the keys are on their way: the scales, and the blocks of the next tile
+      float ks = 0.f, vs = 0.f;
+      if (id >= 0) {
+        ks = c.k_scale[static_cast<int64_t>(id) * c.kv_heads + head];
+        vs = c.v_scale[static_cast<int64_t>(id) * c.kv_heads + head];
+      }
+      const int id_next = block_of(t + 1);
+      if (t > 0) ok = wait(raw_free(1), (t - 1) & 1, 57);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(raw_full(1), bytes);
+      __syncwarp();
+      if (mine) tma_load_3d(base + L::kRawV + lane * box_rows * D, &tv, raw_full(1), 0, off, box_id * c.kv_heads + head);
+      // Tile t - 4, whose entry this overwrites, is done with: the keys of tile t - 1 are converted, into the buffer
+      // of tile t - 3, so the scores of its second step were complete, and they were begun when P V of the second
+      // step of tile t - 4 was, for which its entry was read.
+      float top = vs < INFINITY ? vs : 0.f;
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
       top = __shfl_sync(~0u, top, 0);
@@ -507,11 +614,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         down = ref / top;
         ref = top;
       }
-      const uint32_t there = __ballot_sync(~0u, id_now >= 0);
+      const uint32_t there = __ballot_sync(~0u, id >= 0);
       TileInfo& in = info[t % kInfo];
       if (lane < kGroups) {
-        in.f[lane] = ks_now;
-        in.w[lane] = vs_now / ref;
+        in.f[lane] = ks;
+        in.w[lane] = vs / ref;
       }
       if (lane == 0) {
         in.down = down;
@@ -519,67 +626,67 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         in.there = there;
       }
       __syncwarp();
-      const int box_id = __shfl_sync(~0u, id_now, (lane * per_box) & 31);
-      const bool mine = lane < boxes && box_id >= 0;
-      const uint32_t bytes = __popc(__ballot_sync(~0u, mine)) * box_rows * D;
-      const int off = bs > kTile ? 0 : (t * kTile + lane * box_rows) & (bs - 1);
-      if (lane == 0) {
-        mbar_arrive(info_full(t % kInfo));
-        mbar_arrive_expect_tx(raw_full(0), bytes);
-      }
-      __syncwarp();
-      if (mine) tma_load_3d(base + L::kRawK + lane * box_rows * D, &tk, raw_full(0), 0, off, box_id * c.kv_heads + head);
-      if (t > 0) ok = wait(raw_free(1), (t - 1) & 1, 57);
-      ok = __all_sync(~0u, ok);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(raw_full(1), bytes);
-      __syncwarp();
-      if (mine) tma_load_3d(base + L::kRawV + lane * box_rows * D, &tv, raw_full(1), 0, off, box_id * c.kv_heads + head);
+      if (lane == 0) mbar_arrive(info_full(t % kInfo));
+      id = id_next;
     }
-  } else if (warp == kIssueWarp && lane == 0) {
-    // ------------------------------------------------------------------ issuer: one thread for both query tiles
-    const int tiles = rows > kTile ? 2 : 1;
-    constexpr uint32_t idesc_s = f16_idesc(kTile, false);
+  } else if (warp < kIssueWarp + 2) {
+    // ------------------------------------------------------------------ issuers: one warp per query tile
+    const int q = warp - kIssueWarp;
+    const bool active = q * kTile < rows;
+    constexpr uint32_t idesc_s = f16_idesc(kKeys, false);
     constexpr uint32_t idesc_o = f16_idesc(D, true);
     bool ok = true;
-    // S of key tile t for query tile q; its columns hold P of the tile before until its product with V is done
-    auto scores = [&](int q, int t) {
-      const int b = t & 1;
-      if (q == 0) ok = ok && wait(op_full(0, b), (t >> 1) & 1, 59);
-      if (t > 0) ok = ok && wait(pv_done(q), (t - 1) & 1, 61);
+    auto await = [&](uint32_t b, uint32_t parity, int code) { ok = __all_sync(~0u, ok && wait(b, parity, code)); };
+    // S of step u, into the buffer that P of step u - 2 was in
+    auto scores = [&](int u) {
+      const int b = (u >> 1) & 1;
+      if ((u & 1) == 0) await(op_full(0, b), (u >> 2) & 1, 59);
+      if (active && u >= 2) await(pv_done(q, u), ((u >> 1) - 1) & 1, 61);
       if (!ok) return;
       tc_fence_after();
-      const uint32_t q_at = base + L::kQ + q * L::kOp, k_at = base + L::kK + b * L::kOp;
+      const uint32_t q_at = base + L::kQ + q * L::kOp, k_at = base + L::kK + b * L::kOp + (u & 1) * kKeys * 128;
+      if (elect_one()) {
+        if (active) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t step = (kk >> 2) * kSubTile;
-        umma_f16_ss(tmem + q * kTile, make_kmajor_sw128_desc(q_at + step) + 2 * (kk & 3),
-                    make_kmajor_sw128_desc(k_at + step) + 2 * (kk & 3), idesc_s, kk != 0 ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t step = (kk >> 2) * kSubTile;
+            umma_f16_ss(tmem + q * kTile + (u & 1) * kKeys, make_kmajor_sw128_desc(q_at + step) + 2 * (kk & 3),
+                        make_kmajor_sw128_desc(k_at + step) + 2 * (kk & 3), idesc_s, kk != 0 ? 1u : 0u);
+          }
+          umma_commit(s_full(q, u));
+          if ((u & 1) == 1) umma_commit(op_free(0, b));
+        } else if ((u & 1) == 1) {  // the other tile alone decides when the operands are free
+          mbar_arrive(op_free(0, b));
+        }
       }
-      umma_commit(s_full(q));
-      if (q == tiles - 1) umma_commit(op_free(0, b));
+      __syncwarp();
     };
-    for (int q = 0; q < tiles && ok && nt > 0; ++q) {
-      ok = wait(q_full(q), 0, 58);
-      scores(q, 0);
-    }
-    for (int t = 0; t < nt && ok; ++t) {
-      const int b = t & 1;
-      for (int q = 0; q < tiles && ok; ++q) {
-        if (q == 0) ok = wait(op_full(1, b), (t >> 1) & 1, 62);
-        if (ok) ok = wait(p_full(q), t & 1, 63 + q);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t v_at = base + L::kV + b * L::kOp, t_p = tmem + q * kTile, t_o = tmem + 256 + q * D;
+    auto products = [&](int u) {
+      const int b = (u >> 1) & 1;
+      if ((u & 1) == 0) await(op_full(1, b), (u >> 2) & 1, 62);
+      if (active) await(p_full(q, u), (u >> 1) & 1, 63);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t v_at = base + L::kV + b * L::kOp + (u & 1) * kKeys * 128;
+      const uint32_t t_p = tmem + q * kTile + (u & 1) * kKeys, t_o = tmem + 256 + q * D;
+      if (elect_one()) {
+        if (active) {
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)
-          umma_f16_ts(t_o, t_p + kk * 8, mn_major_desc(v_at + kk * 16 * 128), idesc_o, (t | kk) != 0 ? 1u : 0u);
-        umma_commit(pv_done(q));
-        if (q == tiles - 1) umma_commit(op_free(1, b));
-        // the next scores of this tile at once, before the other tile's P is looked at: its softmax then runs while
-        // the other tile is in its products
-        if (t + 1 < nt) scores(q, t + 1);
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_f16_ts(t_o, t_p + kk * 8, mn_major_desc(v_at + kk * 16 * 128), idesc_o, (u | kk) != 0 ? 1u : 0u);
+          umma_commit(pv_done(q, u));
+          if ((u & 1) == 1) umma_commit(op_free(1, b));
+        } else if ((u & 1) == 1) {
+          mbar_arrive(op_free(1, b));
+        }
       }
+      __syncwarp();
+    };
+    if (active && nu > 0) await(q_full(q), 0, 58);
+    for (int u = 0; u < 2 && u < nu && ok; ++u) scores(u);
+    for (int u = 0; u < nu && ok; ++u) {
+      products(u);
+      if (ok && u + 2 < nu) scores(u + 2);
     }
   }
   }
@@ -617,7 +724,10 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
   if (st != cudaSuccess) return st;
   const dim3 grid(static_cast<unsigned>(p.cache.kv_heads), static_cast<unsigned>(blocks),
                   static_cast<unsigned>(p.requests));
-  return launch_dependent(kern, grid, dim3(kThreads), smem, stream, tk, tv, p, min_rows, box);
+  // rows of q and out on 32-byte boundaries take whole sectors per lane
+  const int wide = ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0 &&
+                   p.ld_q % 16 == 0 && p.ld_out % 16 == 0;
+  return launch_dependent(kern, grid, dim3(kThreads), smem, stream, tk, tv, p, min_rows, box, wide);
 }
 
 }  // namespace
