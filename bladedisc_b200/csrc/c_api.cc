@@ -538,6 +538,7 @@ int32_t disc_b200_kv8_read(const disc_b200_kv8_read_args* a, void* stream) {
 }
 
 int64_t disc_b200_kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv) {
+  static_assert(DISC_B200_KV8_DIRECT_KEYS == disc_b200::kKv8DirectKeys, "the header's threshold is the kernel's");
   return disc_b200::kv8_attention_workspace_bytes(dim, max_kv);
 }
 

@@ -14,6 +14,7 @@ namespace disc_b200 {
 
 enum KvElemType : int { kKvF16 = 1, kKvBF16 = 2 };  // DISC_B200_F16 / DISC_B200_BF16
 
+constexpr int kKv8DirectKeys = 512;   // caches up to this long take one CTA per item and no workspace
 constexpr int kKvMaxRequests = 8192;  // per-request bookkeeping of the table kernels lives in shared memory
 
 struct KvBlocksParams {

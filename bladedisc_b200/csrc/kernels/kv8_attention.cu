@@ -22,7 +22,7 @@ namespace {
 // An item is a request, a kv head and 8 or 16 query rows (query heads of that kv head, tokens of that request); its work
 // is steps of 32 keys.  All steps of all items are laid end to end and cut into equal shares, one per CTA, three CTAs
 // per SM: ragged lengths balance to one step.  A share that ends inside an item leaves its partial maximum, sum and
-// output in the workspace, and a second small kernel joins them.  Short caches (max_kv <= kDirectKeys) take one CTA
+// output in the workspace, and a second small kernel joins them.  Short caches (max_kv <= kKv8DirectKeys) take one CTA
 // per item and need neither.
 //
 // Inside a CTA a warp runs by itself: it fetches its steps with TMA into its own ring, multiplies with mma.sync
@@ -42,7 +42,6 @@ constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one
-constexpr int kDirectKeys = 512;  // caches up to this long are not cut
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // a score may exceed the running maximum by this much (in log2) and
 constexpr float kRefSlack = 4.f;  // a value scale the reference by this factor before O is rescaled: P < 2^15
@@ -681,7 +680,8 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
   }
   auto kern = split_kernel<T, D, NQ>;
   constexpr int smem = SplitSmem<D>::kDynamic;
-  cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t st = allow_smem(kern, smem, ready);
   if (st != cudaSuccess) return st;
   st = launch_dependent(kern, grid, dim3(kSplitThreads), smem, stream, tk, tv, p, shape, ws);
   if (st != cudaSuccess || !shape.stream) return st;
@@ -693,7 +693,7 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int max_rows, cudaStream_t str
   const int64_t rows = std::min(static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads), static_cast<int64_t>(max_rows));
   SplitShape shape;
   shape.max_rows = max_rows;
-  shape.stream = p.max_kv > kDirectKeys ? 1 : 0;
+  shape.stream = p.max_kv > kKv8DirectKeys ? 1 : 0;
   const int tile_rows = rows > 8 ? 16 : 8;
   shape.row_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
   const dim3 grid = shape.stream ? dim3(static_cast<unsigned>(stream_ctas()))
@@ -706,7 +706,7 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int max_rows, cudaStream_t str
 }  // namespace
 
 int64_t kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv) {
-  return max_kv > kDirectKeys ? ws_bytes(stream_ctas(), dim) : 0;
+  return max_kv > kKv8DirectKeys ? ws_bytes(stream_ctas(), dim) : 0;
 }
 
 cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t stream, const char** err) {
@@ -734,7 +734,7 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   // Which requests go where is decided on the device, from q_lens; the host knows the bound.
   const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
   const bool many = rows > kSplitRows, few = !many || p.requests > 1;
-  if (few && p.max_kv > kDirectKeys && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < ws_bytes(stream_ctas(), p.cache.dim)))
+  if (few && p.max_kv > kKv8DirectKeys && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < ws_bytes(stream_ctas(), p.cache.dim)))
     *err = "the workspace is too small or not 16-byte aligned";
   if (p.table_width == 0) {  // no keys at all, but the kernel's tensor maps want a cache
     if (p.cache.num_blocks == 0) *err = "a cache without blocks";

@@ -720,7 +720,8 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
   }
   auto kern = prefill_kernel<T, D>;
   constexpr int smem = Smem<D>::kDynamic;
-  cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> ready{0};
+  cudaError_t st = allow_smem(kern, smem, ready);
   if (st != cudaSuccess) return st;
   const dim3 grid(static_cast<unsigned>(p.cache.kv_heads), static_cast<unsigned>(blocks),
                   static_cast<unsigned>(p.requests));

@@ -241,8 +241,11 @@ const char* problem(const KvBlocksParams& p) {
 }
 
 cudaError_t launch(void (*kern)(KvBlocksParams), const KvBlocksParams& p, int ctas, size_t smem, cudaStream_t stream) {
-  cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (st != cudaSuccess) return st;
+  if (smem > 48 * 1024) {
+    const cudaError_t st =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (st != cudaSuccess) return st;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kThreads);

@@ -21,6 +21,7 @@ BIAS_NONE, BIAS_F32, BIAS_I8 = 0, 1, 2
 SCALE_NONE, SCALE_SCALAR, SCALE_PER_COL, SCALE_PER_ROW = 0, 1, 2, 3
 PATH_AUTO, PATH_TILED, PATH_SMALL_M, PATH_SIMT, PATH_PAIR, PATH_GEMV, PATH_SKINNY = 0, 1, 2, 3, 4, 5, 6
 F32, F16, BF16 = 0, 1, 2  # BF16: the kv8 calls only
+KV8_DIRECT_KEYS = 512  # DISC_B200_KV8_DIRECT_KEYS
 
 
 class ContextOptions(Structure):

@@ -569,24 +569,27 @@ class KvPlan(NamedTuple):
     kv_lens: torch.Tensor    # [requests] cached tokens with the new ones
 
 
-def _one_device(first: torch.Tensor, **tensors) -> torch.device:
-    """The CUDA device that all of them are on."""
-    dev = first.device
-    if dev.type != "cuda":
+def _one_device(*tensors) -> int:
+    """Ordinal of the CUDA device that all of them (None aside) are on."""
+    dev = tensors[0].get_device()
+    if dev < 0:
         raise ValueError("the paged cache lives on CUDA tensors: there is no CPU implementation")
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not on {dev} like the others")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor is on {t.device}, not on cuda:{dev} like the others")
     return dev
 
 
-def _call(dev: torch.device, fn, args) -> None:
-    """Launches on the current stream of `dev`, whichever device is current."""
-    if torch.cuda.current_device() == dev.index:
-        _lib.check(fn(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+def _call(dev: int, fn, args) -> None:
+    """Launches on the current stream of device `dev`, whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if torch._C._cuda_getDevice() == dev:
+        code = fn(args, stream)
     else:
         with torch.cuda.device(dev):
-            _lib.check(fn(ctypes.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+            code = fn(args, stream)
+    if code:
+        _lib.check(code)
 
 
 def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int) -> torch.Tensor:
@@ -597,7 +600,7 @@ def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int) -> torch.T
 
 
 def _kv_blocks_args(tokens, lens, table, free_list, free_count, block_size):
-    dev = _one_device(lens, tokens=tokens, table=table, free_list=free_list, free_count=free_count)
+    dev = _one_device(lens, tokens, table, free_list, free_count)
     _dense("tokens", tokens, torch.int32, 1)
     _dense("lens", lens, torch.int32, 1)
     _dense("table", table, torch.int32, 2)
@@ -624,9 +627,12 @@ def kv_blocks_extend(tokens: torch.Tensor, lens: torch.Tensor, table: torch.Tens
     n, cap = lens.numel(), int(max_tokens)
     if cap < 0:
         raise ValueError("max_tokens must not be negative")
-    out = KvPlan(*torch.empty(2 * cap + 3 * n + 1, dtype=torch.int32, device=dev).split([cap, cap, n + 1, n, n]))
+    buf = torch.empty(2 * cap + 3 * n + 1, dtype=torch.int32, device=lens.device)
+    out = KvPlan(*torch.split_with_sizes(buf, (cap, cap, n + 1, n, n)))
+    at = buf.data_ptr()
     a.max_tokens = cap
-    a.slots, a.positions, a.q_start, a.q_lens, a.kv_lens = (t.data_ptr() for t in out)
+    a.slots, a.positions, a.q_start = at, at + 4 * cap, at + 8 * cap
+    a.q_lens, a.kv_lens = at + 4 * (2 * cap + n + 1), at + 4 * (2 * cap + 2 * n + 1)
     _call(dev, _lib.load().disc_b200_kv_blocks_extend, a)
     return out
 
@@ -671,8 +677,7 @@ def kv8_append(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: tor
     ``[blocks, kv heads]``: a block and a head share the scale ``max|x| / 127`` of the tokens stored so far; tokens
     that the block held before are moved to the new scale when it grows.  ``slots`` and ``positions`` are those of
     `kv_blocks_extend` (the first ``tokens`` entries are read; slot -1 = not stored)."""
-    dev = _one_device(k, qkv=qkv, v=v, k_scale=k_scale, v_scale=v_scale, slots=slots, positions=positions, cos=cos,
-                      sin=sin)
+    dev = _one_device(k, qkv, v, k_scale, v_scale, slots, positions, cos, sin)
     cache = _kv8_cache(k, v, k_scale, v_scale)
     kind = _kv_type("qkv", qkv.dtype)
     if qkv.dim() != 2 or (qkv.shape[0] > 1 and qkv.stride(0) < qkv.shape[1]) or (qkv.numel() and qkv.stride(1) != 1):
@@ -700,7 +705,7 @@ def kv8_append(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: tor
         a.positions, a.cos_table, a.sin_table = positions.data_ptr(), cos.data_ptr(), sin.data_ptr()
         a.table_rows = cos.shape[0]
         if q_heads:
-            q = torch.empty((tokens, q_heads, dim), dtype=qkv.dtype, device=dev)
+            q = torch.empty((tokens, q_heads, dim), dtype=qkv.dtype, device=qkv.device)
             a.q_out = q.data_ptr()
     elif q_heads:
         q = qkv[:, :q_heads * dim].unflatten(1, (q_heads, dim))
@@ -712,12 +717,12 @@ def kv8_read(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: t
              dtype: torch.dtype = torch.float16) -> Tuple[torch.Tensor, torch.Tensor]:
     """The given blocks (int32 ids) of one layer as the values they stand for: keys and values of ``dtype``
     ``[len(blocks), kv heads, block size, head size]``; zeros for an id outside the cache."""
-    dev = _one_device(k, v=v, k_scale=k_scale, v_scale=v_scale, blocks=blocks)
+    dev = _one_device(k, v, k_scale, v_scale, blocks)
     a = _lib.Kv8ReadArgs(_kv8_cache(k, v, k_scale, v_scale))
     _dense("blocks", blocks, torch.int32, 1)
     a.type = _kv_type("dtype", dtype)
     a.blocks, a.count = blocks.data_ptr(), blocks.numel()
-    out = torch.empty((2, blocks.numel()) + tuple(k.shape[1:]), dtype=dtype, device=dev)
+    out = torch.empty((2, blocks.numel()) + tuple(k.shape[1:]), dtype=dtype, device=k.device)
     ko, vo = out.unbind(0)
     a.k_out, a.v_out = ko.data_ptr(), vo.data_ptr()
     _call(dev, _lib.load().disc_b200_kv8_read, a)
@@ -727,8 +732,11 @@ def kv8_read(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: t
 _kv8_workspace = {}
 
 
-def _kv8_workspace_bytes(dev: torch.device, dim: int, max_kv: int) -> int:
-    key = (dev.index, dim, max_kv > 512)
+def _kv8_workspace_bytes(dev: int, dim: int, max_kv: int) -> int:
+    """Bytes of workspace; they depend on the device and the head size, and on max_kv only by a threshold."""
+    if max_kv <= _lib.KV8_DIRECT_KEYS:
+        return 0
+    key = (dev, dim)
     if key not in _kv8_workspace:
         with torch.cuda.device(dev):
             _kv8_workspace[key] = _lib.load().disc_b200_kv8_attention_workspace_bytes(dim, max_kv)
@@ -747,8 +755,7 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     computed), ``max_kv`` bounds ``kv_lens`` and only steers how the work is split (default: the table's width).
     Query heads are a multiple of the kv heads.  ``scale`` defaults to ``head size ** -0.5``.  Rows that belong to
     no request are left as ``out`` had them; a row that sees no key gives zeros."""
-    dev = _one_device(q, k=k, v=v, k_scale=k_scale, v_scale=v_scale, table=table, q_start=q_start, q_lens=q_lens,
-                      kv_lens=kv_lens, out=out)
+    dev = _one_device(q, k, v, k_scale, v_scale, table, q_start, q_lens, kv_lens, out)
     cache = _kv8_cache(k, v, k_scale, v_scale)
     kind = _kv_type("q", q.dtype)
     if q.dim() != 3 or q.shape[2] != cache.dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
@@ -759,7 +766,7 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
                       (tokens > 1 and q.stride(0) < heads * dim)):
         raise ValueError("the heads of a row of q must lie one after the other, and rows may not overlap")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
     _dense("table", table, torch.int32, 2)
@@ -779,7 +786,7 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
                               dim ** -0.5 if scale is None else float(scale))
     need = _kv8_workspace_bytes(dev, dim, a.max_kv)
     if need:  # from torch's allocator: ordered with this stream, a captured graph keeps its own
-        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = work.data_ptr(), need
     _call(dev, _lib.load().disc_b200_kv8_attention, a)
     return out

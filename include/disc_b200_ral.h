@@ -577,6 +577,8 @@ typedef struct disc_b200_kv8_attention_args {
   void* workspace; /* device, 16-byte aligned; may be NULL when the size below is 0 */
   int64_t workspace_bytes;
 } disc_b200_kv8_attention_args;
+/* Caches up to this many keys need no workspace. */
+enum { DISC_B200_KV8_DIRECT_KEYS = 512 };
 /* Workspace of a call with this head size and max_kv on the current device (the same for every batch; 0 for short
  * caches).  Calls that overlap on the GPU need one each; its contents mean nothing between calls. */
 int64_t disc_b200_kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv);

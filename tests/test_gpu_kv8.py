@@ -471,7 +471,7 @@ def test_refusals(ops):
         ops.kv8_attention(q, c[0].float(), *c[1:], table, i, i, i, **good)
     with pytest.raises(ValueError, match="scales"):
         ops.kv8_attention(q, c[0], c[1], c[2][:2].contiguous(), c[3], table, i, i, i, **good)
-    with pytest.raises(ValueError, match="not on"):
+    with pytest.raises(ValueError, match="not on cuda"):
         ops.kv8_attention(q, *c, table, i, i, i.cpu(), **good)
     with pytest.raises(ValueError, match="q's shape"):
         ops.kv8_attention(q, *c, table, i, i, i, out=q[:2].clone(), **good)
