@@ -592,25 +592,33 @@ def _call(dev: int, fn, args) -> None:
         _lib.check(code)
 
 
-def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int) -> torch.Tensor:
-    if t.dtype != dtype or t.dim() != dims or not t.is_contiguous():
+def _is(t: torch.Tensor, dtype: torch.dtype, dims: int) -> bool:
+    return t.dtype is dtype and t.dim() == dims and t.is_contiguous()
+
+
+def _dense(name: str, t: torch.Tensor, dtype: torch.dtype, dims: int) -> None:
+    if not _is(t, dtype, dims):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor with {dims} dimension(s), got {t.dtype} "
                          f"{tuple(t.shape)} with strides {t.stride()}")
-    return t
 
 
 def _kv_blocks_args(tokens, lens, table, free_list, free_count, block_size):
     dev = _one_device(lens, tokens, table, free_list, free_count)
-    _dense("tokens", tokens, torch.int32, 1)
-    _dense("lens", lens, torch.int32, 1)
-    _dense("table", table, torch.int32, 2)
-    _dense("free_list", free_list, torch.int32, 1)
+    i32 = torch.int32
+    if not (_is(tokens, i32, 1) and _is(lens, i32, 1) and _is(table, i32, 2) and _is(free_list, i32, 1)):
+        for name, t, dims in (("tokens", tokens, 1), ("lens", lens, 1), ("table", table, 2),
+                              ("free_list", free_list, 1)):
+            _dense(name, t, i32, dims)
     if free_count.dtype != torch.int32 or free_count.numel() != 1:
         raise ValueError("free_count must be one int32 value")
-    if tokens.shape != lens.shape or table.shape[0] != lens.numel():
+    n = lens.numel()
+    rows, width = table.shape
+    if not 0 < block_size < 1 << 31:
+        raise ValueError("block_size must be positive")
+    if tokens.numel() != n or rows != n:
         raise ValueError("tokens, lens and table must have one entry (row) per request")
     a = _lib.KvBlocksArgs(tokens.data_ptr(), lens.data_ptr(), table.data_ptr(), free_list.data_ptr(),
-                          free_count.data_ptr(), lens.numel(), table.shape[1], free_list.numel(), int(block_size))
+                          free_count.data_ptr(), n, width, free_list.numel(), block_size)
     return dev, a
 
 
@@ -625,10 +633,10 @@ def kv_blocks_extend(tokens: torch.Tensor, lens: torch.Tensor, table: torch.Tens
     all requests before it are not there, its table row is too short, or its rows end behind ``max_tokens``."""
     dev, a = _kv_blocks_args(tokens, lens, table, free_list, free_count, block_size)
     n, cap = lens.numel(), int(max_tokens)
-    if cap < 0:
-        raise ValueError("max_tokens must not be negative")
-    buf = torch.empty(2 * cap + 3 * n + 1, dtype=torch.int32, device=lens.device)
-    out = KvPlan(*torch.split_with_sizes(buf, (cap, cap, n + 1, n, n)))
+    if not 0 <= cap < 1 << 31:
+        raise ValueError("max_tokens must not be negative, nor pass 32 bits")
+    buf = lens.new_empty(2 * cap + 3 * n + 1)
+    out = KvPlan(*torch.unsafe_split_with_sizes(buf, (cap, cap, n + 1, n, n)))
     at = buf.data_ptr()
     a.max_tokens = cap
     a.slots, a.positions, a.q_start = at, at + 4 * cap, at + 8 * cap
@@ -649,12 +657,13 @@ _KV_TYPE = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
 def _kv8_cache(k, v, k_scale, v_scale) -> "_lib.Kv8Cache":
-    _dense("k", k, torch.int8, 4)
-    _dense("v", v, torch.int8, 4)
-    _dense("k_scale", k_scale, torch.float32, 2)
-    _dense("v_scale", v_scale, torch.float32, 2)
-    blocks, heads, size, dim = k.shape
-    if v.shape != k.shape or tuple(k_scale.shape) != (blocks, heads) or v_scale.shape != k_scale.shape:
+    i8, f32 = torch.int8, torch.float32
+    if not (_is(k, i8, 4) and _is(v, i8, 4) and _is(k_scale, f32, 2) and _is(v_scale, f32, 2)):
+        for name, t, dtype, dims in (("k", k, i8, 4), ("v", v, i8, 4), ("k_scale", k_scale, f32, 2),
+                                     ("v_scale", v_scale, f32, 2)):
+            _dense(name, t, dtype, dims)
+    blocks, heads, size, dim = shape = k.shape
+    if v.shape != shape or k_scale.shape != shape[:2] or v_scale.shape != shape[:2]:
         raise ValueError("k and v must be [blocks, kv heads, block size, head size], their scales [blocks, kv heads]")
     return _lib.Kv8Cache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, heads, size, dim)
 
@@ -705,7 +714,7 @@ def kv8_append(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: tor
         a.positions, a.cos_table, a.sin_table = positions.data_ptr(), cos.data_ptr(), sin.data_ptr()
         a.table_rows = cos.shape[0]
         if q_heads:
-            q = torch.empty((tokens, q_heads, dim), dtype=qkv.dtype, device=qkv.device)
+            q = qkv.new_empty(tokens, q_heads, dim)
             a.q_out = q.data_ptr()
     elif q_heads:
         q = qkv[:, :q_heads * dim].unflatten(1, (q_heads, dim))
@@ -722,8 +731,9 @@ def kv8_read(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: t
     _dense("blocks", blocks, torch.int32, 1)
     a.type = _kv_type("dtype", dtype)
     a.blocks, a.count = blocks.data_ptr(), blocks.numel()
-    out = torch.empty((2, blocks.numel()) + tuple(k.shape[1:]), dtype=dtype, device=k.device)
-    ko, vo = out.unbind(0)
+    _, heads, size, dim = k.shape
+    ko = k.new_empty(blocks.numel(), heads, size, dim, dtype=dtype)
+    vo = torch.empty_like(ko)
     a.k_out, a.v_out = ko.data_ptr(), vo.data_ptr()
     _call(dev, _lib.load().disc_b200_kv8_read, a)
     return ko, vo
@@ -758,35 +768,41 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     dev = _one_device(q, k, v, k_scale, v_scale, table, q_start, q_lens, kv_lens, out)
     cache = _kv8_cache(k, v, k_scale, v_scale)
     kind = _kv_type("q", q.dtype)
-    if q.dim() != 3 or q.shape[2] != cache.dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
-        raise ValueError(f"q must be [tokens, heads, {cache.dim}] with a multiple of {cache.kv_heads} heads, got "
+    dim = cache.dim
+    if q.dim() != 3 or q.shape[2] != dim or q.shape[1] < 1 or q.shape[1] % cache.kv_heads:
+        raise ValueError(f"q must be [tokens, heads, {dim}] with a multiple of {cache.kv_heads} heads, got "
                          f"{tuple(q.shape)}")
-    tokens, heads, dim = q.shape
-    if q.numel() and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or
+    tokens, heads, _ = q.shape
+    if not q.is_contiguous() and q.numel() and (q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim) or
                       (tokens > 1 and q.stride(0) < heads * dim)):
         raise ValueError("the heads of a row of q must lie one after the other, and rows may not overlap")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor of q's shape and dtype")
-    _dense("table", table, torch.int32, 2)
-    _dense("q_lens", q_lens, torch.int32, 1)
-    _dense("kv_lens", kv_lens, torch.int32, 1)
-    _dense("q_start", q_start, torch.int32, 1)
+    i32 = torch.int32
+    if not (_is(table, i32, 2) and _is(q_start, i32, 1) and _is(q_lens, i32, 1) and _is(kv_lens, i32, 1)):
+        for name, t, dims in (("table", table, 2), ("q_start", q_start, 1), ("q_lens", q_lens, 1),
+                              ("kv_lens", kv_lens, 1)):
+            _dense(name, t, i32, dims)
     n = q_lens.numel()
-    if kv_lens.numel() != n or table.shape[0] != n or q_start.numel() < n:
+    rows, width = table.shape
+    if kv_lens.numel() != n or rows != n or q_start.numel() < n:
         raise ValueError("q_start, q_lens, kv_lens and table must have one entry (row) per request")
-    if max_q < 0 or (max_kv is not None and max_kv < 0):
+    room = width * cache.block_size
+    if max_kv is None or max_kv > room:
+        max_kv = room
+    if max_q < 0 or max_kv < 0:
         raise ValueError("max_q and max_kv must not be negative")
-    room = table.shape[1] * cache.block_size
+    if max_q > tokens:  # no request has more rows than there are
+        max_q = tokens
     a = _lib.Kv8AttentionArgs(q.data_ptr(), out.data_ptr(), tokens, q.stride(0) if tokens > 1 else heads * dim,
                               heads * dim, heads, kind, cache, table.data_ptr(), q_start.data_ptr(),
-                              q_lens.data_ptr(), kv_lens.data_ptr(), n, table.shape[1], int(max_q),
-                              room if max_kv is None else min(int(max_kv), room),
-                              dim ** -0.5 if scale is None else float(scale))
-    need = _kv8_workspace_bytes(dev, dim, a.max_kv)
+                              q_lens.data_ptr(), kv_lens.data_ptr(), n, width, max_q, max_kv,
+                              dim ** -0.5 if scale is None else scale)
+    need = _kv8_workspace_bytes(dev, dim, max_kv)
     if need:  # from torch's allocator: ordered with this stream, a captured graph keeps its own
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        work = k.new_empty(need)
         a.workspace, a.workspace_bytes = work.data_ptr(), need
     _call(dev, _lib.load().disc_b200_kv8_attention, a)
     return out
