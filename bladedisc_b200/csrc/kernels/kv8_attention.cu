@@ -41,7 +41,8 @@ namespace {
 constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
-constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one
+constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one,
+constexpr int kSplitRowsMixed = 8;  // and with prompts in the batch: what fits one tile of eight rows
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // a score may exceed the running maximum by this much (in log2) and
 constexpr float kRefSlack = 4.f;  // a value scale the reference by this factor before O is rescaled: P < 2^15
@@ -595,8 +596,8 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
   }
 }
 
-// Joins the pieces of the item that CTA blockIdx.x of split_kernel started: one block per row, its groups of D / 4
-// threads take every kJoinThreads / (D / 4)-th piece each.
+// Joins the pieces of the item that CTA blockIdx.x of split_kernel started.  D / 4 threads hold an output row; the
+// groups of them take rows side by side when the pieces are few and the pieces of one row when they are many.
 constexpr int kJoinThreads = 256;
 
 template <typename T, int D, int ROWS>
@@ -607,49 +608,61 @@ join_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spli
   grid_dep_wait();
   grid_dep_launch();
   const int4 it = ws.desc[blockIdx.x];
-  if (it.w <= 1) return;
+  const int pieces = it.w;
+  if (pieces <= 1) return;
   const int G = p.q_heads / p.cache.kv_heads;
   const Request q = request_of(p, it.x, shape.max_rows, ROWS);
-  const int row = it.z * ROWS + blockIdx.y;
-  if (row >= q.q_len * G) return;
-  const int64_t at = p.q_start[it.x] + row / G;
-  if (at < 0 || at >= p.tokens) return;
-  const int64_t c0 = blockIdx.x;
+  const int rows = min(ROWS, q.q_len * G - it.z * ROWS);
+  const int64_t tok0 = p.q_start[it.x], c0 = blockIdx.x;
+  int per_row = 1;  // groups that share a row
+  while (per_row < GROUPS && per_row * 2 < pieces) per_row *= 2;
+  const int at_once = GROUPS / per_row;
   const int group = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  float top = -INFINITY, sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int part_of = group % per_row;
+  for (int row0 = static_cast<int>(blockIdx.y) * at_once; row0 < rows; row0 += at_once * gridDim.y) {
+    const int r = row0 + group / per_row;
+    float top = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < rows) {
 #pragma unroll 4
-  for (int i = group; i < it.w; i += GROUPS) {
-    const int64_t slot = ((i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * 16) + blockIdx.y;
-    const float2 ml = ws.ml[slot];
-    const float4 v = *reinterpret_cast<const float4*>(ws.o + slot * D + d);
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw no key (its output may not even be written)
-    const float mn = fmaxf(top, ml.x);
-    const float a = mn == -INFINITY ? 1.f : exp2_approx(top - mn), b = mn == -INFINITY ? 1.f : exp2_approx(ml.x - mn);
-    sum = sum * a + ml.y * b;
-    acc = make_float4(acc.x * a + v.x * b, acc.y * a + v.y * b, acc.z * a + v.z * b, acc.w * a + v.w * b);
-    top = mn;
+      for (int i = part_of; i < pieces; i += per_row) {
+        const int64_t slot = (i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * 16 + r;
+        const float2 ml = ws.ml[slot];
+        const float4 v = *reinterpret_cast<const float4*>(ws.o + slot * D + d);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw no key (its output may not even be written)
+        const float mn = fmaxf(top, ml.x);
+        const float a = mn == -INFINITY ? 1.f : exp2_approx(top - mn), b = mn == -INFINITY ? 1.f : exp2_approx(ml.x - mn);
+        sum = sum * a + ml.y * b;
+        acc = make_float4(acc.x * a + v.x * b, acc.y * a + v.y * b, acc.z * a + v.z * b, acc.w * a + v.w * b);
+        top = mn;
+      }
+    }
+    __syncthreads();  // the rows before have been read
+    *reinterpret_cast<float4*>(&part[group][d]) = acc;
+    if (d == 0) {
+      part_m[group] = top;
+      part_l[group] = sum;
+    }
+    __syncthreads();
+    if (part_of == 0 && r < rows) {
+      for (int i = 0; i < per_row; ++i) top = fmaxf(top, part_m[group + i]);
+      sum = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < per_row; ++i) {
+        const float a = top == -INFINITY ? 1.f : exp2_approx(part_m[group + i] - top);
+        const float4 v = *reinterpret_cast<const float4*>(&part[group + i][d]);
+        sum += a * part_l[group + i];
+        acc = make_float4(acc.x + a * v.x, acc.y + a * v.y, acc.z + a * v.z, acc.w + a * v.w);
+      }
+      const int row = it.z * ROWS + r;
+      const int64_t at = tok0 + row / G;
+      if (at >= 0 && at < p.tokens) {
+        const bool none = sum == 0.f;
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at * p.ld_out + (it.y * G + row % G) * D + d) =
+            make_uint2(none ? 0u : pack2(acc.x / sum, acc.y / sum, T()), none ? 0u : pack2(acc.z / sum, acc.w / sum, T()));
+      }
+    }
   }
-  *reinterpret_cast<float4*>(&part[group][d]) = acc;
-  if (d == 0) {
-    part_m[group] = top;
-    part_l[group] = sum;
-  }
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, part_m[i]);
-  sum = 0.f;
-  float o = 0.f;
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i) {
-    const float a = top == -INFINITY ? 1.f : exp2_approx(part_m[i] - top);
-    sum += a * part_l[i];
-    o += a * part[i][threadIdx.x];
-  }
-  static_cast<T*>(p.out)[at * p.ld_out + (it.y * G + row % G) * D + threadIdx.x] =
-      pack_one(sum == 0.f ? 0.f : o / sum, T());
 }
 
 bool misaligned(const void* p, uintptr_t by) { return (reinterpret_cast<uintptr_t>(p) & (by - 1)) != 0; }
@@ -685,7 +698,7 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
   if (st != cudaSuccess) return st;
   st = launch_dependent(kern, grid, dim3(kSplitThreads), smem, stream, tk, tv, p, shape, ws);
   if (st != cudaSuccess || !shape.stream) return st;
-  return launch_dependent(join_kernel<T, D, 8 * NQ>, dim3(grid.x, 8 * NQ), dim3(kJoinThreads), 0, stream, p, shape, ws);
+  return launch_dependent(join_kernel<T, D, 8 * NQ>, dim3(grid.x, 2), dim3(kJoinThreads), 0, stream, p, shape, ws);
 }
 
 template <typename T, int D>
@@ -741,13 +754,14 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   }
   if (*err) return cudaErrorInvalidValue;
   if (many) {
-    const cudaError_t st = kv8_prefill_launch(p, few ? kSplitRows : 0, stream, err);
+    const cudaError_t st = kv8_prefill_launch(p, few ? kSplitRowsMixed : 0, stream, err);
     if (st != cudaSuccess || !few) return st;
   }
+  const int most = many ? kSplitRowsMixed : kSplitRows;
   const bool f16 = p.type == kKvF16;
   if (p.cache.dim == 128)
-    return f16 ? launch_t<__half, 128>(p, kSplitRows, stream, err) : launch_t<__nv_bfloat16, 128>(p, kSplitRows, stream, err);
-  return f16 ? launch_t<__half, 64>(p, kSplitRows, stream, err) : launch_t<__nv_bfloat16, 64>(p, kSplitRows, stream, err);
+    return f16 ? launch_t<__half, 128>(p, most, stream, err) : launch_t<__nv_bfloat16, 128>(p, most, stream, err);
+  return f16 ? launch_t<__half, 64>(p, most, stream, err) : launch_t<__nv_bfloat16, 64>(p, most, stream, err);
 }
 
 int kv8_status_fetch_and_clear() {

@@ -31,167 +31,235 @@ __device__ __forceinline__ void load_f8(const float* p, float* f) {
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
 
-__device__ __forceinline__ uint32_t pack_levels(const float* x, float s) {
-  uint32_t w = 0;
+// A level as the low byte of v + 1.5 2^23: rounded half to even, no conversion instruction.
+__device__ __forceinline__ uint32_t level_bits(float v) {
+  return __float_as_uint(fminf(fmaxf(v, -127.f), 127.f) + 12582912.f);
+}
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* b) {
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+// Levels of four values at scale s, inv = rn(1 / s): the quotient corrected by its own remainder (Markstein) is the
+// correctly rounded x / s for normal operands, so that the level is that of the division at a third of its
+// instructions.  inv = 0: 1 / s is not a normal number.
+__device__ __forceinline__ uint32_t pack_levels(const float* x, float s, float inv) {
+  uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float l = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -127.f), 127.f);
-    w |= (static_cast<uint32_t>(static_cast<int>(l)) & 0xffu) << (8 * i);
+    const float q = x[i] * inv;
+    b[i] = level_bits(inv > 0.f ? fmaf(fmaf(-q, s, x[i]), inv, q) : __fdiv_rn(x[i], s));
   }
-  return w;
+  return pack_bytes(b);
 }
 
-// Grid: x = segments of `seg` consecutive tokens; y = kv_heads keys, kv_heads values, then groups of four query
-// heads.  A run is a maximal sequence of consecutive tokens whose slots are consecutive inside one block; the
-// CTA whose segment holds its first token works on all of it, once for the maximum and once for the levels (the
-// second read comes from the caches).
-template <typename T>
-__global__ void __launch_bounds__(kThreads) append_kernel(Kv8AppendParams p, int seg) {
+// Tokens of a run: the consecutive tokens whose slots follow one another inside one block.
+constexpr int kMaxSegment = 128;  // tokens per block of threads, and the longest run
+constexpr int kPasses = 4;        // passes over a run whose loads are in flight together
+constexpr int kQPasses = 4;       // (token, query head) pairs per thread
+
+// The first kv_blocks CTAs take a segment of `seg` consecutive tokens and four key / value heads each, a warp per head:
+// every run whose first token lies in the segment, once for the maximum and once for the levels, eight values of each
+// half of the head per lane; the second read comes from the caches (keeping a run in registers instead took 128 of
+// them and was slower: 79 against 72 us for 9800 tokens).  Nothing is shared between warps but the slots.  The other CTAs rotate q, a thread
+// for eight values of each half of kQPasses heads.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_constant__ Kv8AppendParams p, int seg, int kv_blocks) {
+  constexpr int half = D / 2;
+  constexpr int kLanes = D / 16;          // lanes per token: eight values of each half of the head
+  constexpr int kTokens = 32 / kLanes;    // tokens per pass of a warp
   const Kv8Cache& c = p.cache;
-  const int D = c.dim, bs = c.block_size, half = D / 2;
-  const int chunks = D / 16;               // threads per token: eight values of each half of the head
-  const int per_pass = kThreads / chunks;  // tokens per pass of the CTA
-  const int chunk = threadIdx.x % chunks, sub = threadIdx.x / chunks;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * seg;
-  const int64_t t1 = min(t0 + seg, p.tokens);
+  const int bs = c.block_size;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunk = lane % kLanes;
   const T* qkv = static_cast<const T*>(p.qkv);
+  const int kv_groups = (2 * c.kv_heads + 3) / 4;
   grid_dep_wait();
   grid_dep_launch();
 
-  const int y = blockIdx.y;
-  if (y >= 2 * c.kv_heads) {
-    const int h0 = (y - 2 * c.kv_heads) * 4, h1 = min(h0 + 4, p.q_heads);
+  if (static_cast<int>(blockIdx.x) >= kv_blocks) {
+    constexpr int kPairs = kThreads / kLanes;
     T* out = static_cast<T*>(p.q_out);
-    for (int64_t t = t0 + sub; t < t1; t += per_pass) {
-      const int pos = min(max(p.positions[t], 0), p.table_rows - 1);
-      float cs[8], sn[8], lo[8], hi[8];
-      load_f8(p.cos_table + static_cast<int64_t>(pos) * half + chunk * 8, cs);
-      load_f8(p.sin_table + static_cast<int64_t>(pos) * half + chunk * 8, sn);
-      for (int h = h0; h < h1; ++h) {
+    const uint32_t n = static_cast<uint32_t>(p.tokens * p.q_heads), q_heads = p.q_heads;
+    const uint32_t i0 = (blockIdx.x - kv_blocks) * (kPairs * kQPasses) + threadIdx.x / kLanes;
+    uint4 w[kQPasses][2];
+    int pos[kQPasses];
+#pragma unroll
+    for (int e = 0; e < kQPasses; ++e) {
+      const uint32_t i = i0 + e * kPairs;
+      if (i < n) {
+        const uint32_t t = i / q_heads, h = i - t * q_heads;
         const T* x = qkv + t * p.ld_qkv + h * D + chunk * 8;
-        load8(x, lo);
-        load8(x + half, hi);
+        w[e][0] = *reinterpret_cast<const uint4*>(x);
+        w[e][1] = *reinterpret_cast<const uint4*>(x + half);
+        pos[e] = min(max(p.positions[t], 0), p.table_rows - 1);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kQPasses; ++e) {
+      const uint32_t i = i0 + e * kPairs;
+      if (i < n) {
+        float cs[8], sn[8], lo[8], hi[8];
+        load_f8(p.cos_table + static_cast<int64_t>(pos[e]) * half + chunk * 8, cs);
+        load_f8(p.sin_table + static_cast<int64_t>(pos[e]) * half + chunk * 8, sn);
+        unpack8(w[e][0], lo, T());
+        unpack8(w[e][1], hi, T());
         rotate8(lo, hi, cs, sn);
-        T* o = out + (t * p.q_heads + h) * D + chunk * 8;
+        T* o = out + static_cast<int64_t>(i) * D + chunk * 8;
         store8(o, lo);
         store8(o + half, hi);
       }
     }
     return;
   }
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x / kv_groups) * seg;
+  const int tokens = static_cast<int>(min(static_cast<int64_t>(seg), p.tokens - t0));
 
+  // slots of the segment, the token before it and the block's worth behind it; -2: no such token
+  __shared__ int32_t slot_of[1 + 2 * kMaxSegment], pos_of[1 + 2 * kMaxSegment];
+  for (int i = threadIdx.x; i < 1 + tokens + bs; i += kThreads) {
+    const int64_t t = t0 - 1 + i;
+    const bool there = t >= 0 && t < p.tokens;
+    slot_of[i] = there ? p.slots[t] : -2;
+    if (p.cos_table) pos_of[i] = there ? min(max(p.positions[t], 0), p.table_rows - 1) : 0;
+  }
+  __syncthreads();
+  const int y = blockIdx.x % kv_groups * 4 + warp;
+  if (y >= 2 * c.kv_heads) return;
   const bool is_v = y >= c.kv_heads;
   const int head = is_v ? y - c.kv_heads : y;
   const bool rot = !is_v && p.cos_table != nullptr;
-  const T* x0 = qkv + static_cast<int64_t>(p.q_heads + y) * D + chunk * 8;
   const int64_t slots = static_cast<int64_t>(c.num_blocks) * bs;
-  __shared__ uint32_t red[kThreads / 32];
+  const int sub = lane / kLanes;
 
-  for (int64_t t = t0; t < t1; ++t) {
-    const int64_t slot = p.slots[t];
+  for (int i = 0; i < tokens; ++i) {
+    const int slot = slot_of[1 + i];
     if (slot < 0 || slot >= slots) continue;
-    const int block = static_cast<int>(slot / bs), off = static_cast<int>(slot % bs);
-    if (t > 0 && off > 0 && p.slots[t - 1] == slot - 1) continue;  // inside a run
-    int len = 1;
-    while (off + len < bs && t + len < p.tokens && p.slots[t + len] == slot + len) ++len;
-
-    auto load = [&](int i, float* lo, float* hi) {
-      const T* x = x0 + (t + i) * p.ld_qkv;
-      load8(x, lo);
-      load8(x + half, hi);
-      if (rot) {
-        const int pos = min(max(p.positions[t + i], 0), p.table_rows - 1);
-        float cs[8], sn[8];
-        load_f8(p.cos_table + static_cast<int64_t>(pos) * half + chunk * 8, cs);
-        load_f8(p.sin_table + static_cast<int64_t>(pos) * half + chunk * 8, sn);
-        rotate8(lo, hi, cs, sn);
+    const int block = slot / bs, off = slot % bs;
+    if (off > 0 && slot_of[i] == slot - 1) continue;  // inside a run
+    // the run ends with the block or where a slot does not follow
+    int len = bs - off;
+    for (int b = 1; b < len; b += 32) {
+      const bool stop = b + lane < len && slot_of[1 + i + b + lane] != slot + b + lane;
+      const uint32_t m = __ballot_sync(~0u, stop);
+      if (m) {
+        len = b + __ffs(m) - 1;
+        break;
       }
+    }
+    const int64_t t = t0 + i;
+    const T* x0 = qkv + t * p.ld_qkv + static_cast<int64_t>(p.q_heads + y) * D + chunk * 8;
+    float* scale_at = (is_v ? c.v_scale : c.k_scale) + static_cast<int64_t>(block) * c.kv_heads + head;
+    const float old = off > 0 ? *scale_at : 0.f;
+
+    auto turn = [&](int j, float* lo, float* hi) {
+      if (!rot) return;
+      const int pos = pos_of[1 + i + j];
+      float cs[8], sn[8];
+      load_f8(p.cos_table + static_cast<int64_t>(pos) * half + chunk * 8, cs);
+      load_f8(p.sin_table + static_cast<int64_t>(pos) * half + chunk * 8, sn);
+      rotate8(lo, hi, cs, sn);
     };
     // |x| as bits: ordered like the values, with infinity and NaN on top
     uint32_t top = 0;
-    for (int i = sub; i < len; i += per_pass) {
-      float lo[8], hi[8];
-      load(i, lo, hi);
+    uint4 w[kPasses][2];
+    auto fetch = [&](int j0) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        top = max(top, __float_as_uint(lo[e]) & 0x7fffffffu);
-        top = max(top, __float_as_uint(hi[e]) & 0x7fffffffu);
+      for (int e = 0; e < kPasses; ++e) {
+        const int j = j0 + e * kTokens + sub;
+        if (j < len) {
+          w[e][0] = *reinterpret_cast<const uint4*>(x0 + j * p.ld_qkv);
+          w[e][1] = *reinterpret_cast<const uint4*>(x0 + j * p.ld_qkv + half);
+        }
+      }
+    };
+    for (int j0 = 0; j0 < len; j0 += kTokens * kPasses) {
+      fetch(j0);
+#pragma unroll
+      for (int e = 0; e < kPasses; ++e) {
+        const int j = j0 + e * kTokens + sub;
+        if (j < len) {
+          float lo[8], hi[8];
+          unpack8(w[e][0], lo, T());
+          unpack8(w[e][1], hi, T());
+          turn(j, lo, hi);
+#pragma unroll
+          for (int b = 0; b < 8; ++b)
+            top = max(top, max(__float_as_uint(lo[b]) & 0x7fffffffu, __float_as_uint(hi[b]) & 0x7fffffffu));
+        }
       }
     }
     top = __reduce_max_sync(~0u, top);
-    __syncthreads();  // `red` of the run before has been read
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-    float* scale_at = (is_v ? c.v_scale : c.k_scale) + static_cast<int64_t>(block) * c.kv_heads + head;
-    const float old = off > 0 ? *scale_at : 0.f;
-    __syncthreads();
-    top = max(max(red[0], red[1]), max(red[2], red[3]));
     const float fresh = top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 127.f) : __uint_as_float(0x7fc00000u);
     const float s = isnan(old) || isnan(fresh) ? __uint_as_float(0x7fc00000u) : fmaxf(old, fresh);
-    if (threadIdx.x == 0) *scale_at = s;
+    if (lane == 0) *scale_at = s;
 
     int8_t* base = (is_v ? c.v : c.k) + (static_cast<int64_t>(block) * c.kv_heads + head) * bs * D;
     if (off > 0 && s > old && old > 0.f) {
       const float ratio = __fdiv_rn(old, s);
       uint4* levels = reinterpret_cast<uint4*>(base);
-      for (int i = threadIdx.x; i < off * D / 16; i += kThreads) {
-        uint4 w = levels[i];
+#pragma unroll 4
+      for (int k = lane; k < off * D / 16; k += 32) {
+        uint4 w = levels[k];
         uint32_t* e = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          uint32_t m = 0;
+          uint32_t m[4];
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-            m |= (static_cast<uint32_t>(__float2int_rn(level_of(e[j], b) * ratio)) & 0xffu) << (8 * b);
-          e[j] = m;
+          for (int b = 0; b < 4; ++b) m[b] = level_bits(level_of(e[j], b) * ratio);
+          e[j] = pack_bytes(m);
         }
-        levels[i] = w;
+        levels[k] = w;
       }
     }
-    for (int i = sub; i < len; i += per_pass) {
-      uint2 wl = make_uint2(0, 0), wh = make_uint2(0, 0);
-      if (s > 0.f) {
-        float lo[8], hi[8];
-        load(i, lo, hi);
-        wl = make_uint2(pack_levels(lo, s), pack_levels(lo + 4, s));
-        wh = make_uint2(pack_levels(hi, s), pack_levels(hi + 4, s));
+    const float inv = s > 1.2e-38f && s < 8e37f ? __frcp_rn(s) : 0.f;
+    for (int j0 = 0; j0 < len; j0 += kTokens * kPasses) {
+      fetch(j0);
+#pragma unroll
+      for (int e = 0; e < kPasses; ++e) {
+        const int j = j0 + e * kTokens + sub;
+        if (j < len) {
+          uint2 wl = make_uint2(0, 0), wh = make_uint2(0, 0);
+          if (s > 0.f) {
+            float lo[8], hi[8];
+            unpack8(w[e][0], lo, T());
+            unpack8(w[e][1], hi, T());
+            turn(j, lo, hi);
+            wl = make_uint2(pack_levels(lo, s, inv), pack_levels(lo + 4, s, inv));
+            wh = make_uint2(pack_levels(hi, s, inv), pack_levels(hi + 4, s, inv));
+          }
+          int8_t* o = base + (off + j) * D + chunk * 8;
+          *reinterpret_cast<uint2*>(o) = wl;
+          *reinterpret_cast<uint2*>(o + half) = wh;
+        }
       }
-      int8_t* o = base + (off + i) * D + chunk * 8;
-      *reinterpret_cast<uint2*>(o) = wl;
-      *reinterpret_cast<uint2*>(o + half) = wh;
     }
-    t += len - 1;
+    i += len - 1;
   }
 }
 
-// One thread per 16 levels.
+// A CTA per block and head, of keys (y = 0) or values; a thread per 16 levels.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) read_kernel(Kv8ReadParams p) {
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Kv8ReadParams p) {
   const Kv8Cache& c = p.cache;
-  const int64_t per_head = static_cast<int64_t>(c.block_size) * c.dim;
-  const int64_t n = static_cast<int64_t>(p.count) * c.kv_heads * per_head / 16;
+  const int n = c.block_size * c.dim / 16;
+  const bool is_v = blockIdx.y != 0;
+  const uint32_t heads = c.kv_heads, i = blockIdx.x / heads, head = blockIdx.x - i * heads;
   grid_dep_wait();
   grid_dep_launch();
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < 2 * n;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const bool is_v = i >= n;
-    const int64_t at = (is_v ? i - n : i) * 16;
-    const int64_t bh = at / per_head;
-    const int64_t id = p.blocks[bh / c.kv_heads], head = bh % c.kv_heads;
+  const int id = p.blocks[i];
+  const bool there = id >= 0 && id < c.num_blocks;
+  const int64_t row = there ? static_cast<int64_t>(id) * c.kv_heads + head : 0;
+  const float s = there ? (is_v ? c.v_scale : c.k_scale)[row] : 0.f;
+  const uint4* src = reinterpret_cast<const uint4*>(is_v ? c.v : c.k) + row * n;
+  T* dst = static_cast<T*>(is_v ? p.v_out : p.k_out) + static_cast<int64_t>(blockIdx.x) * n * 16;
+#pragma unroll 4
+  for (int k = threadIdx.x; k < n; k += kThreads) {
+    const uint4 w = there ? src[k] : make_uint4(0, 0, 0, 0);
+    const uint32_t e[4] = {w.x, w.y, w.z, w.w};
     float f[16];
-    if (id >= 0 && id < c.num_blocks) {
-      const int64_t row = id * c.kv_heads + head;
-      const float s = (is_v ? c.v_scale : c.k_scale)[row];
-      const uint4 w = *reinterpret_cast<const uint4*>((is_v ? c.v : c.k) + row * per_head + at % per_head);
-      const uint32_t* e = reinterpret_cast<const uint32_t*>(&w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) f[j] = level_of(e[j >> 2], j & 3) * s;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) f[j] = 0.f;
-    }
-    T* o = static_cast<T*>(is_v ? p.v_out : p.k_out) + at;
-    store8(o, f);
-    store8(o + 8, f + 8);
+    for (int j = 0; j < 16; ++j) f[j] = level_of(e[j >> 2], j & 3) * s;
+    store8(dst + k * 16, f);
+    store8(dst + k * 16 + 8, f + 8);
   }
 }
 
@@ -227,13 +295,18 @@ cudaError_t kv8_append_launch(const Kv8AppendParams& p, cudaStream_t stream, con
   else if (rot && (p.table_rows <= 0 || misaligned(p.cos_table, 16) || misaligned(p.sin_table, 16) ||
                    misaligned(p.q_out, 16)))
     *err = "cos, sin and q_out must be 16-byte aligned and not empty";
-  const int64_t gy = 2 * static_cast<int64_t>(p.cache.kv_heads) + (rot ? (p.q_heads + 3) / 4 : 0);
-  if (!*err && gy > 65535) *err = "too many heads";
   if (*err) return cudaErrorInvalidValue;
-  const int seg = p.tokens >= 2048 ? 16 : p.tokens >= 512 ? 4 : 1;
-  const dim3 grid(static_cast<unsigned>((p.tokens + seg - 1) / seg), static_cast<unsigned>(gy));
-  return p.type == kKvF16 ? launch_dependent(append_kernel<__half>, grid, dim3(kThreads), 0, stream, p, seg)
-                          : launch_dependent(append_kernel<__nv_bfloat16>, grid, dim3(kThreads), 0, stream, p, seg);
+  // decode steps spread over the GPU token by token; prompts take a block's worth of tokens, mostly one run, at a time
+  const int seg = p.tokens >= 2048 ? p.cache.block_size : p.tokens >= 512 ? 4 : 1;
+  const int64_t kv_blocks = (p.tokens + seg - 1) / seg * ((2 * static_cast<int64_t>(p.cache.kv_heads) + 3) / 4);
+  const int64_t per_block = kThreads / (p.cache.dim / 16) * kQPasses;
+  const int64_t q_blocks = rot ? (p.tokens * p.q_heads + per_block - 1) / per_block : 0;
+  if (kv_blocks + q_blocks > INT32_MAX || p.tokens * p.q_heads > INT32_MAX) *err = "too many tokens and heads";
+  if (*err) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(kv_blocks + q_blocks));
+  auto kern = p.cache.dim == 128 ? (p.type == kKvF16 ? append_kernel<__half, 128> : append_kernel<__nv_bfloat16, 128>)
+                                 : (p.type == kKvF16 ? append_kernel<__half, 64> : append_kernel<__nv_bfloat16, 64>);
+  return launch_dependent(kern, grid, dim3(kThreads), 0, stream, p, seg, static_cast<int>(kv_blocks));
 }
 
 cudaError_t kv8_read_launch(const Kv8ReadParams& p, cudaStream_t stream, const char** err) {
@@ -245,14 +318,13 @@ cudaError_t kv8_read_launch(const Kv8ReadParams& p, cudaStream_t stream, const c
   if (!p.blocks || !p.k_out || !p.v_out) *err = "null operand";
   else if (misaligned(p.k_out, 16) || misaligned(p.v_out, 16)) *err = "outputs must be 16-byte aligned";
   if (*err) return cudaErrorInvalidValue;
-  const int64_t items = 2 * static_cast<int64_t>(p.count) * p.cache.kv_heads * p.cache.block_size * p.cache.dim / 16;
-  int64_t grid = (items + kThreads - 1) / kThreads;
-  const int64_t cap = static_cast<int64_t>(device_sm_count()) * 16;
-  if (grid > cap) grid = cap;
-  return p.type == kKvF16
-             ? launch_dependent(read_kernel<__half>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, p)
-             : launch_dependent(read_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
-                                stream, p);
+  const int64_t pairs = static_cast<int64_t>(p.count) * p.cache.kv_heads;
+  if (pairs > INT32_MAX) {
+    *err = "too many blocks";
+    return cudaErrorInvalidValue;
+  }
+  return launch_dependent(p.type == kKvF16 ? read_kernel<__half> : read_kernel<__nv_bfloat16>,
+                          dim3(static_cast<unsigned>(pairs), 2), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace disc_b200

@@ -24,12 +24,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* f) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void unpack8(const uint4& w, float* f, T) {
   unpack2(w.x, f[0], f[1], T());
   unpack2(w.y, f[2], f[3], T());
   unpack2(w.z, f[4], f[5], T());
   unpack2(w.w, f[6], f[7], T());
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* f) {
+  unpack8(*reinterpret_cast<const uint4*>(p), f, T());
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* f) {

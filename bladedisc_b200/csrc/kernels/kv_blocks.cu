@@ -7,10 +7,14 @@
 // in the reverse order, so that trim(old lengths) undoes an extend bit for bit.
 //
 // The work is two prefix sums over at most 8192 requests and one pass over tokens, so latency is what counts:
-// one launch, one cluster.  Every CTA of the cluster computes all the sums (a few hundred ns; cheaper than
-// handing them over), a cluster barrier separates the last read of the state from its first update, and the
-// tokens are dealt over all threads.
+// one launch, one cluster, as few threads as the batch needs (barriers cost with every warp).  Every CTA of the
+// cluster computes all the sums (a few hundred ns; cheaper than handing them over), a cluster barrier separates the
+// last read of the state from its first update, and the tokens are dealt over all threads.  Prompts have more tokens
+// than one cluster writes quickly (115000: 24 us): there it only makes the table, and a second kernel over the whole
+// GPU writes the slots.
 #include "kv8.h"
+
+#include <algorithm>
 
 #include "device_info.h"
 #include "sm100_ptx.cuh"
@@ -18,8 +22,8 @@
 namespace disc_b200 {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kItems = kKvMaxRequests / kThreads;
+constexpr int kMaxThreads = 1024;
+constexpr int kItems = kKvMaxRequests / kMaxThreads;  // requests per thread at most
 
 struct Sums {
   int64_t warp[32];
@@ -27,7 +31,7 @@ struct Sums {
 
 // Inclusive prefix sum over the block of one value per thread.
 __device__ __forceinline__ int64_t block_inclusive(int64_t v, Sums& s) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t u = __shfl_up_sync(~0u, v, o);
@@ -35,18 +39,21 @@ __device__ __forceinline__ int64_t block_inclusive(int64_t v, Sums& s) {
   }
   if (lane == 31) s.warp[warp] = v;
   __syncthreads();
-  if (warp == 0) {
-    int64_t w = s.warp[lane];
+  if (warps <= 8) {
+    for (int w = 0; w < warp; ++w) v += s.warp[w];
+  } else {
+    if (warp == 0) {
+      int64_t w = lane < warps ? s.warp[lane] : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t u = __shfl_up_sync(~0u, w, o);
-      if (lane >= o) w += u;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(~0u, w, o);
+        if (lane >= o) w += u;
+      }
+      s.warp[lane] = w;
     }
-    s.warp[lane] = w;
+    __syncthreads();
+    if (warp > 0) v += s.warp[warp - 1];
   }
-  __syncthreads();
-  if (warp > 0) v += s.warp[warp - 1];
-  __syncthreads();  // the sums may be overwritten by the next call
   return v;
 }
 
@@ -60,23 +67,32 @@ __device__ __forceinline__ int last_not_above(const int32_t* start, int n, int t
   return lo;
 }
 
+// tokens <= 2^31 - 1 and a block of at most as many: no overflow in unsigned arithmetic
+__device__ __forceinline__ int blocks_of(int tokens, int bs) {
+  return static_cast<int>((static_cast<uint32_t>(tokens) + static_cast<uint32_t>(bs) - 1) / static_cast<uint32_t>(bs));
+}
+
 __device__ __forceinline__ int clamp_len(int v, int64_t room) {
   return v < 0 ? 0 : (v > room ? static_cast<int>(room) : v);
 }
 
-__global__ void __launch_bounds__(kThreads, 1) extend_kernel(KvBlocksParams p) {
+template <bool SLOTS>
+__global__ void __launch_bounds__(kMaxThreads, 1) extend_kernel(KvBlocksParams p) {
   extern __shared__ int32_t dyn[];
-  __shared__ Sums sums;
+  __shared__ Sums sums, sums2;
+  __shared__ int given;
   const int R = p.requests, bs = p.block_size;
+  const int threads = blockDim.x;
   int32_t* start = dyn;          // [R + 1] first token row of a request
   int32_t* first = start + R + 1;  // [R] blocks handed out before this request
   int32_t* had = first + R;      // [R] cached tokens before, or -1 - that when the request is not served
-  const int items = (R + kThreads - 1) / kThreads;
+  const int items = (R + threads - 1) / threads;
   const int64_t room = static_cast<int64_t>(p.table_width) * bs;
   grid_dep_wait();
   grid_dep_launch();
 
   const int count = min(max(*p.free_count, 0), p.num_blocks);
+  if (threadIdx.x == 0) given = 0;
   int n[kItems], len[kItems];
   int64_t total = 0;
 #pragma unroll
@@ -101,13 +117,13 @@ __global__ void __launch_bounds__(kThreads, 1) extend_kernel(KvBlocksParams p) {
       start[r] = static_cast<int32_t>(at < INT32_MAX ? at : INT32_MAX);
       at += n[i];
       if (static_cast<int64_t>(len[i]) + n[i] <= room && at <= p.max_tokens)
-        need[i] = static_cast<int>((static_cast<int64_t>(len[i]) + n[i] + bs - 1) / bs - (len[i] + bs - 1) / bs);
+        need[i] = blocks_of(len[i] + n[i], bs) - blocks_of(len[i], bs);
       needs += max(need[i], 0);
       if (r == R - 1) start[R] = static_cast<int32_t>(at < INT32_MAX ? at : INT32_MAX);
     }
   }
-  int64_t upto = block_inclusive(needs, sums) - needs;
-  int64_t given_here = 0;
+  int64_t upto = block_inclusive(needs, sums2) - needs;
+  int last = 0;  // blocks handed out up to the last served request of this thread
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
     const int r = threadIdx.x * items + i;
@@ -119,10 +135,12 @@ __global__ void __launch_bounds__(kThreads, 1) extend_kernel(KvBlocksParams p) {
       const bool served = need[i] == 0 || (need[i] > 0 && upto <= count);
       had[r] = served ? len[i] : -1 - len[i];
       if (!served) n[i] = 0;
-      given_here += served ? need[i] : 0;
+      if (served && need[i] > 0) last = static_cast<int>(upto);
     }
   }
-  const int64_t given = block_inclusive(given_here, sums);  // ends with a barrier: the arrays are complete
+  last = __reduce_max_sync(~0u, last);
+  if ((threadIdx.x & 31) == 0 && last > 0) atomicMax(&given, last);
+  __syncthreads();  // the arrays are complete
   cluster_sync_all();  // every CTA has read the state: it may change now
 
   const uint32_t rank = cluster_ctarank();
@@ -138,29 +156,37 @@ __global__ void __launch_bounds__(kThreads, 1) extend_kernel(KvBlocksParams p) {
         p.q_start[r] = start[r];
       }
     }
-    if (threadIdx.x == kThreads - 1) {
+    if (threadIdx.x == threads - 1) {
       p.q_start[R] = start[R];
-      *p.free_count = static_cast<int32_t>(count - given);
+      *p.free_count = count - given;
     }
   }
 
+  if (!SLOTS) {
+    for (int f = rank * threads + threadIdx.x; f < given; f += gridDim.x * threads) {
+      const int r = last_not_above(first, R, f);  // of requests with the same sum the last one takes blocks
+      p.table[static_cast<int64_t>(r) * p.table_width + blocks_of(had[r], bs) + f - first[r]] =
+          p.free_list[count - 1 - f];
+    }
+    return;
+  }
   const int asked = start[R];
-  for (int64_t t = rank * kThreads + threadIdx.x; t < p.max_tokens; t += gridDim.x * kThreads) {
+  for (int t = rank * threads + threadIdx.x; t < p.max_tokens; t += gridDim.x * threads) {
     int slot = -1, pos = -1;
     if (t < asked) {
-      const int r = last_not_above(start, R, static_cast<int>(t));
+      const int r = last_not_above(start, R, t);
       if (had[r] >= 0) {
-        pos = had[r] + static_cast<int>(t) - start[r];
-        const int b = pos / bs, held = (had[r] + bs - 1) / bs;
+        pos = had[r] + t - start[r];
+        const int b = pos / bs, held = blocks_of(had[r], bs);
         int32_t* entry = p.table + static_cast<int64_t>(r) * p.table_width + b;
         int id;
         if (b >= held) {
           id = p.free_list[count - 1 - (first[r] + b - held)];
-          if (pos % bs == 0) *entry = id;  // the first token of a block enters it into the table
+          if (pos - b * bs == 0) *entry = id;  // the first token of a block enters it into the table
         } else {
           id = *entry;
         }
-        slot = id >= 0 && id < p.num_blocks ? id * bs + pos % bs : -1;
+        slot = id >= 0 && id < p.num_blocks ? id * bs + pos - b * bs : -1;
       }
     }
     p.slots[t] = slot;
@@ -168,13 +194,64 @@ __global__ void __launch_bounds__(kThreads, 1) extend_kernel(KvBlocksParams p) {
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 1) trim_kernel(KvBlocksParams p) {
+// Slots and positions from what extend_kernel wrote, four consecutive tokens per thread.
+constexpr int kSlotThreads = 256;
+__global__ void __launch_bounds__(kSlotThreads) slots_kernel(KvBlocksParams p) {
+  const int R = p.requests, bs = p.block_size;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kSlotThreads + threadIdx.x) * 4;
+  if (t0 >= p.max_tokens) return;
+  const int asked = p.q_start[R];
+  int pos[4], id[4], off[4], slot[4];
+  int r = t0 < asked ? last_not_above(p.q_start, R, static_cast<int>(t0)) : R;
+  int end = r < R ? p.q_start[r + 1] : 0, n = r < R ? p.q_lens[r] : 0;
+  int q = r < R ? p.kv_lens[r] - n + static_cast<int>(t0) - p.q_start[r] : 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t t = t0 + i;
+    pos[i] = -1;
+    off[i] = 0;
+    id[i] = -1;
+    if (t < asked) {
+      if (t >= end) {  // the next request that has tokens
+        while (t >= end) end = p.q_start[++r + 1];
+        n = p.q_lens[r];
+        q = p.kv_lens[r] - n;
+      }
+      if (n > 0) {
+        pos[i] = q;
+        const int b = q / bs;
+        off[i] = q - b * bs;
+        id[i] = p.table[static_cast<int64_t>(r) * p.table_width + b];
+      }
+      ++q;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) slot[i] = id[i] >= 0 && id[i] < p.num_blocks ? id[i] * bs + off[i] : -1;
+  if (t0 + 4 <= p.max_tokens && ((reinterpret_cast<uintptr_t>(p.slots) | reinterpret_cast<uintptr_t>(p.positions)) & 15) == 0) {
+    *reinterpret_cast<int4*>(p.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    *reinterpret_cast<int4*>(p.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t0 + i < p.max_tokens) {
+        p.slots[t0 + i] = slot[i];
+        p.positions[t0 + i] = pos[i];
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kMaxThreads, 1) trim_kernel(KvBlocksParams p) {
   extern __shared__ int32_t dyn[];
   __shared__ Sums sums;
   const int R = p.requests, bs = p.block_size;
+  const int threads = blockDim.x;
   int32_t* base = dyn;       // [R + 1] blocks freed before this request
   int32_t* stay = base + R + 1;  // [R] blocks that the request keeps
-  const int items = (R + kThreads - 1) / kThreads;
+  const int items = (R + threads - 1) / threads;
   const int64_t room = static_cast<int64_t>(p.table_width) * bs;
   grid_dep_wait();
   grid_dep_launch();
@@ -189,8 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1) trim_kernel(KvBlocksParams p) {
     if (i < items && r < R) {
       const int len = clamp_len(p.lens[r], room);
       keep[i] = min(max(p.tokens[r], 0), len);
-      stay[r] = (keep[i] + bs - 1) / bs;
-      freed[i] = (len + bs - 1) / bs - stay[r];
+      stay[r] = blocks_of(keep[i], bs);
+      freed[i] = blocks_of(len, bs) - stay[r];
     }
     total += freed[i];
   }
@@ -218,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) trim_kernel(KvBlocksParams p) {
     }
     if (threadIdx.x == 0) *p.free_count = min(count + gone, p.num_blocks);
   }
-  for (int f = rank * kThreads + threadIdx.x; f < gone; f += gridDim.x * kThreads) {
+  for (int f = rank * threads + threadIdx.x; f < gone; f += gridDim.x * threads) {
     const int r = last_not_above(base, R, f);
     int32_t* entry = p.table + static_cast<int64_t>(r) * p.table_width + stay[r] + (f - base[r]);
     const int place = count + gone - 1 - f;
@@ -240,7 +317,8 @@ const char* problem(const KvBlocksParams& p) {
   return nullptr;
 }
 
-cudaError_t launch(void (*kern)(KvBlocksParams), const KvBlocksParams& p, int ctas, size_t smem, cudaStream_t stream) {
+cudaError_t launch(void (*kern)(KvBlocksParams), const KvBlocksParams& p, int ctas, int threads, size_t smem,
+                   cudaStream_t stream) {
   if (smem > 48 * 1024) {
     const cudaError_t st =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
@@ -248,7 +326,7 @@ cudaError_t launch(void (*kern)(KvBlocksParams), const KvBlocksParams& p, int ct
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -262,8 +340,8 @@ cudaError_t launch(void (*kern)(KvBlocksParams), const KvBlocksParams& p, int ct
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-// One CTA while its threads have one item each; the portable cluster of eight beyond that.
-int ctas_for(int64_t items) { return items <= kThreads ? 1 : 8; }
+// Threads of a CTA for this many requests or tokens; requests beyond go several to a thread.
+int threads_for(int64_t n) { return n <= 256 ? 256 : n <= 512 ? 512 : kMaxThreads; }
 
 }  // namespace
 
@@ -283,15 +361,23 @@ cudaError_t kv_blocks_extend_launch(const KvBlocksParams& p, cudaStream_t stream
     }
     return st;
   }
-  return launch(extend_kernel, p, ctas_for(p.max_tokens), sizeof(int32_t) * (3 * static_cast<size_t>(p.requests) + 1),
-                stream);
+  const size_t smem = sizeof(int32_t) * (3 * static_cast<size_t>(p.requests) + 1);
+  if (p.max_tokens <= 8 * kMaxThreads) {  // a token per thread
+    return launch(extend_kernel<true>, p, p.max_tokens <= kMaxThreads ? 1 : 8,
+                  threads_for(std::max(p.requests, p.max_tokens)), smem, stream);
+  }
+  const cudaError_t st = launch(extend_kernel<false>, p, 8, threads_for(std::max(p.requests, p.num_blocks / 8)), smem, stream);
+  if (st != cudaSuccess) return st;
+  const int64_t blocks = (static_cast<int64_t>(p.max_tokens) + 4 * kSlotThreads - 1) / (4 * kSlotThreads);
+  return launch_dependent(slots_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSlotThreads), 0, stream, p);
 }
 
 cudaError_t kv_blocks_trim_launch(const KvBlocksParams& p, cudaStream_t stream, const char** err) {
   *err = problem(p);
   if (*err) return cudaErrorInvalidValue;
   if (p.requests == 0) return cudaSuccess;
-  return launch(trim_kernel, p, ctas_for(static_cast<int64_t>(p.requests) * p.table_width),
+  const int64_t most = static_cast<int64_t>(p.requests) * p.table_width;  // blocks that can come back
+  return launch(trim_kernel, p, most <= 8 * kMaxThreads ? 1 : 8, threads_for(std::max<int64_t>(p.requests, most / 4)),
                 sizeof(int32_t) * (2 * static_cast<size_t>(p.requests) + 1), stream);
 }
 

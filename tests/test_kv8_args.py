@@ -85,7 +85,7 @@ def test_append(lib):
     _refused(lib, fn, args(qkv=0x1008), "16-byte")
     _refused(lib, fn, args(q_out=0x1008), "16-byte")
     _refused(lib, fn, args(table_rows=0), "not empty")
-    _refused(lib, fn, args(q_heads=1 << 20, ld_qkv=1 << 30), "too many heads")
+    _refused(lib, fn, args(tokens=1 << 30, q_heads=1 << 20, ld_qkv=1 << 30), "too many tokens and heads")
     for name in ("qkv", "slots", "positions", "sin_table", "q_out"):
         _refused(lib, fn, args(**{name: None}), "null operand")
     assert fn(ctypes.byref(args(tokens=0)), None) == 0
