@@ -22,6 +22,10 @@ Per layer and rank (g ranks, M tokens, H hidden, F ffn):
     silu(gate)*up row scales / quantize -> slot r of [g,M,F/g] int8, all-gather
     down linear (gathered int8 in) -> slot r of [g,M,H/g] fp16, all-gather
 
+With :meth:`QuantDecoder.start_paged` the cache is paged and held in 8 bits: every request
+has its own length, RoPE and the append are one kernel, attention is this library's own
+(``ops.kv8_attention``) for prompts and single tokens alike, and nothing is read back.
+
 Weights are random (~N(0, 0.02)), generated from a seed on the device, the full
 matrix on every rank and then cut, so that any number of ranks computes the
 same model.
@@ -34,6 +38,7 @@ import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from . import ops
+from .kv_cache import PagedKVCache8
 from .tp import ColumnParallelQLinear, Communicator, column_share, quantize_rows_gathered
 
 
@@ -117,6 +122,7 @@ class QuantDecoder:
                 lin.weights_static = True
         self.kv: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None
         self.pos = 0
+        self.paged: Optional[PagedKVCache8] = None
         self._cos = self._sin = None
 
     def _linear(self, wq: torch.Tensor, scale: torch.Tensor) -> ColumnParallelQLinear:
@@ -170,10 +176,16 @@ class QuantDecoder:
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         """ids [B, S] (prefill when the cache is empty, else S new tokens per
         sequence) -> final hidden states [B * S, H] fp16."""
-        cfg = self.cfg
         batch, seq = ids.shape
         if self.kv is None:
             raise RuntimeError("call start(batch, max_seq) first")
+        y = self._run_layers(ids, lambda L, idx, qkv: self._attention(L, idx, qkv, batch, seq))
+        self.pos += seq
+        return y
+
+    def _run_layers(self, ids: torch.Tensor, attention) -> torch.Tensor:
+        """Embedding, all layers and the final norm; ``attention(layer, index, qkv)`` is what differs between caches."""
+        cfg = self.cfg
         h = self.embed[ids.reshape(-1)]  # [M, H] residual stream, replicated
         prev = None  # gathered fp16 output of the previous sublayer
         for idx, L in enumerate(self.layers):
@@ -182,7 +194,7 @@ class QuantDecoder:
             else:
                 xq, xs, h = ops.rmsnorm_dynamic_quant(prev, L.g1, cfg.eps, residual=h, x_gathered=True)
             qkv = L.qkv.forward(xq, xs, gather=False)
-            att = self._attention(L, idx, qkv, batch, seq)
+            att = attention(L, idx, qkv)
             aq, a_s = quantize_rows_gathered(self.comm, att)
             o = L.o.forward(aq, a_s, a_gathered=True)
             xq, xs, h = ops.rmsnorm_dynamic_quant(o, L.g2, cfg.eps, residual=h, x_gathered=True)
@@ -190,9 +202,38 @@ class QuantDecoder:
             fl = gu.shape[1] // 2
             hq, h_s = quantize_rows_gathered(self.comm, gu[:, :fl], gu[:, fl:])
             prev = L.down.forward(hq, h_s, a_gathered=True)
-        self.pos += seq
         # final norm straight from the gathered output of the last layer
         return ops.rmsnorm(prev, self.g_final, cfg.eps, residual=h, x_gathered=True)
+
+    def start_paged(self, requests: int, num_blocks: int, max_seq: int, block_size: int = 64) -> PagedKVCache8:
+        """A paged 8-bit cache for ``requests`` requests with lengths of their own (see `forward_paged`)."""
+        cfg = self.cfg
+        self.paged = PagedKVCache8(cfg.layers, requests, num_blocks, cfg.heads // self.world, cfg.head_dim, max_seq,
+                                   block_size, self.device)
+        room = self.paged.table.shape[1] * block_size  # positions that a request can reach
+        self._rope_tables(max(room, 0 if self._cos is None else self._cos.shape[0]))
+        return self.paged
+
+    def forward_paged(self, ids: torch.Tensor, tokens: torch.Tensor, max_q: int,
+                      max_kv: Optional[int] = None) -> torch.Tensor:
+        """One step of the requests of `start_paged`: ``ids [T]`` holds the new tokens of all requests one after the
+        other, ``tokens[r]`` of them (int32 CUDA tensor) for request ``r``, at most ``max_q``; prompts, chunks of
+        prompts and single tokens may be mixed.  Returns the final hidden states ``[T, H]`` fp16; those of a request
+        that found no room (``paged.lens[r]`` did not grow) mean nothing.  Nothing is read back from the GPU: a step
+        may be captured into a CUDA graph and replayed with new contents of ``ids`` and ``tokens``."""
+        if self.paged is None:
+            raise RuntimeError("call start_paged(requests, num_blocks, max_seq) first")
+        cache = self.paged
+        total = ids.numel()
+        plan = cache.extend(tokens, total)
+
+        def attention(L: _Layer, idx: int, qkv: torch.Tensor) -> torch.Tensor:
+            q = cache.append(idx, qkv, plan, self._cos, self._sin)
+            # zeros where no request has rows: the linears behind quantize every row
+            out = cache.attend(idx, q, plan, max_q, max_kv, out=torch.zeros_like(q))
+            return out.view(total, -1)
+
+        return self._run_layers(ids, attention)
 
     def launches_per_layer(self) -> int:
         """Kernels of this library per layer and rank (collectives and torch ops not counted)."""
