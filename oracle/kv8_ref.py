@@ -100,9 +100,8 @@ def attention(q, k, v, ks, vs, table, q_start, q_lens, kv_lens, scale, out, max_
     """q [tokens, heads, d] float64; returns (out float64, allowed difference before the output's own rounding).
 
     The allowance per output: probabilities enter the second product as f16, half a step 2^-11 relative to each;
-    levels may enter the first product as level + 128 <= 255 with 128 times the sum of q taken off again, so a score's
-    sum of d products in fp32 is off by at most (d + 4) 2^-23 times the sum of |q| 255, a probability by twice that
-    relative (its own and the normaliser's); exp2 and the remaining fp32 operations stay
+    a score's sum of d products in fp32 is off by at most (d + 4) 2^-23 times the sum of the magnitudes, a
+    probability by twice that relative (its own and the normaliser's); exp2 and the remaining fp32 operations stay
     within 2^-19 of the magnitudes.  Probabilities under 2^-29 of the row's largest lose bits: 2^-40 of the largest each."""
     out = out.astype(np.float64).copy()
     slack = np.zeros_like(out)
@@ -127,7 +126,7 @@ def attention(q, k, v, ks, vs, table, q_start, q_lens, kv_lens, scale, out, max_
                 kk = k[safe, h // g].reshape(-1, d)[:length].astype(np.float64)
                 vv = v[safe, h // g].reshape(-1, d)[:length].astype(np.float64)
                 s = (q[at, h] @ kk.T) * ksh * scale
-                mag = np.abs(q[at, h]).sum(axis=1, keepdims=True) * 255 * np.abs(ksh) * scale
+                mag = (np.abs(q[at, h]) @ np.abs(kk).T) * np.abs(ksh) * scale
                 s = np.where(seen, s, -np.inf)
                 top = s.max(axis=1, initial=-np.inf, keepdims=True)
                 p = np.where(seen, np.exp(s - np.where(np.isneginf(top), 0, top)), 0)
