@@ -11,8 +11,6 @@
 
 namespace disc_b200 {
 
-__device__ int g_kv8_status = 0;
-
 namespace {
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -25,8 +23,9 @@ namespace {
 // output in the workspace, and a second small kernel joins them.  Short caches (max_kv <= kKv8DirectKeys) take one CTA
 // per item and need neither.
 //
-// Inside a CTA a warp runs by itself: it fetches its steps with TMA into its own ring, multiplies with mma.sync
-// m16n8k16, keeps running maximum, sum and output in registers and meets the others at the end of the item.
+// Inside a CTA a warp runs by itself: it fetches its steps with 16-byte asynchronous copies into its own ring (TMA
+// boxes of 2 to 4 KB cost the warp 170 cycles each, a quarter of a step), multiplies with mma.sync m16n8k16, keeps
+// running maximum, sum and output in registers and meets the others at the end of the item.
 //
 //   S' = K Q'    keys are the wide operand, so that eight query rows fill the instruction (a decode step has one to
 //                eight); the head dimension is permuted alike in K and Q so that a lane's fragments are the bytes of
@@ -36,7 +35,7 @@ namespace {
 // Query rows in bf16 are scaled by a power of two per row to f16 (exact but for values 2^-24 of the row's largest).
 // P goes to f16 times 2^11 so that a probability keeps its 11 bits down to 2^-25 of the largest; the
 // value scale is multiplied in relative to a running reference that O is kept in units of.
-// The 128-byte (64-byte for dim 64) swizzle of the TMA boxes and the key order perm(n) = n ^ ((n & 1) << 2) make the
+// Rows in the ring are swizzled (16-byte chunk c of row r at c ^ (r & 7), for dim 64 c ^ (r / 2 & 3)); that and the key order perm(n) = n ^ ((n & 1) << 2) make the
 // 16-byte shared-memory reads free of bank conflicts.
 constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
@@ -54,6 +53,15 @@ __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t w) {
@@ -102,7 +110,7 @@ struct SplitSmem {
   static constexpr int kHalf = kStep * D;  // bytes of the keys (or values) of one step
   static constexpr int kRing = kSplitWarps * kStages * 2 * kHalf;
   static constexpr int kParts = kSplitWarps * 16 * D * 4;  // O of every warp, in the place of the rings
-  static constexpr int kDynamic = (kRing > kParts ? kRing : kParts) + 1024;
+  static constexpr int kDynamic = kRing > kParts ? kRing : kParts;
 };
 
 // Query rows (tokens x heads of a group) and steps of one request; no rows if the request is not for this kernel.
@@ -123,35 +131,23 @@ __device__ __forceinline__ Request request_of(const Kv8AttentionParams& p, int r
 
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(kSplitThreads, 3)
-split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-             const __grid_constant__ Kv8AttentionParams p, SplitShape shape, SplitWs ws) {
+split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, SplitWs ws) {
   using L = SplitSmem<D>;
   constexpr int W = kSplitWarps, S = L::kStages;
   constexpr int KQ = D / 16;  // k steps of the first product
   constexpr int NV = D / 16;  // m tiles of the second
   constexpr int ROWS = 8 * NQ;
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  __shared__ uint64_t bars[W * S];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float part_m[W][16], part_l[W][16];
   __shared__ long long sums[W];
   __shared__ int found[2];
   __shared__ long long found_at;
-  __shared__ int abort_word;
-  volatile int* abort_flag = &abort_word;
 
   const Kv8Cache& c = p.cache;
   const int bs = c.block_size, G = p.q_heads / c.kv_heads, KH = c.kv_heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int warp = __shfl_sync(~0u, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  if (threadIdx.x == 0) {
-    abort_word = 0;
-    tma_prefetch_desc(&tk);
-    tma_prefetch_desc(&tv);
-  }
-  if (lane < S) mbar_init(smem_u32(&bars[warp * S + lane]), 1);
-  fence_mbar_init();
-  __syncthreads();
   grid_dep_wait();
   grid_dep_launch();
 
@@ -214,13 +210,14 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
   }
   Request rq = request_of(p, r, shape.max_rows, ROWS);
 
-  const uint32_t ring = smem_u32(smem) + warp * (S * 2 * L::kHalf);
   const uint8_t* ring_ptr = smem + warp * (S * 2 * L::kHalf);
-  const uint32_t bar0 = smem_u32(&bars[warp * S]);
+  // where this lane's 16 bytes of every 512 go (dim 128: copies of even and odd index differ in the swizzle)
+  const uint32_t ring = smem_u32(ring_ptr);
+  const uint32_t put_even = D == 128 ? (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4)
+                                     : (lane >> 2) * 64 + (((lane & 3) ^ (lane >> 3 & 3)) << 4);
+  const uint32_t put_odd = D == 128 ? put_even ^ 64 : put_even;
   const int prow = g ^ ((g & 1) << 2);         // key of n = g in a group of eight
   const int v0 = 2 * t, v1 = (2 * t + 1) ^ 4;  // keys of this lane's columns
-  uint32_t waits = 0;                          // steps that this warp's ring has delivered
-  bool ok = true;
 
   while (left > 0) {
     while (item >= rq.tiles * KH) {  // on to the next request with rows
@@ -311,45 +308,37 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
       }
       return f;
     };
-    auto issue = [&](int n, int stage, int id0, int id1) {  // lane 0
-      const uint32_t bar = bar0 + 8 * stage, kt = ring + stage * 2 * L::kHalf;
-      const int off = ((first + n * W) * kStep) & (bs - 1);
-      if (bs >= kStep) {  // both halves lie in one block
-        if (id0 < 0) {
-          mbar_arrive(bar);
-          return;
-        }
-        mbar_arrive_expect_tx(bar, 2 * L::kHalf);
-        tma_load_3d(kt, &tk, bar, 0, off, id0 * KH + head);
-        tma_load_3d(kt + L::kHalf, &tv, bar, 0, off, id0 * KH + head);
-      } else {
-        const int n_there = (id0 >= 0) + (id1 >= 0);
-        if (n_there == 0) {
-          mbar_arrive(bar);
-          return;
-        }
-        mbar_arrive_expect_tx(bar, n_there * L::kHalf);
-        if (id0 >= 0) {
-          tma_load_3d(kt, &tk, bar, 0, 0, id0 * KH + head);
-          tma_load_3d(kt + L::kHalf, &tv, bar, 0, 0, id0 * KH + head);
-        }
-        if (id1 >= 0) {
-          tma_load_3d(kt + L::kHalf / 2, &tk, bar, 0, 0, id1 * KH + head);
-          tma_load_3d(kt + L::kHalf + L::kHalf / 2, &tv, bar, 0, 0, id1 * KH + head);
+    // the whole warp copies step n into its stage: 32 keys and 32 values, 512 bytes per instruction
+    auto issue = [&](int n, int id0, int id1) {
+      const uint32_t kt = ring + (n % S) * (2 * L::kHalf);
+      const int off = ((first + n * W) * kStep) & (bs - 1);  // 0 for blocks of 16, whose halves have a block each
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int id = h == 0 ? id0 : id1;
+        if (id < 0) continue;
+        const int64_t at = ((static_cast<int64_t>(id) * KH + head) * bs + (bs >= kStep ? off + h * 16 : 0)) * D + lane * 16;
+        const int8_t* ks = c.k + at;
+        const int8_t* vs = c.v + at;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint32_t to = kt + h * (L::kHalf / 2) + i * 512 + ((i & 1) ? put_odd : put_even);
+          cp_async16(to, ks + i * 512);
+          cp_async16(to + L::kHalf, vs + i * 512);
         }
       }
+      cp_async_commit();
     };
 
     cur = lookup(0);
 #pragma unroll
     for (int n = 0; n < S; ++n) {
       const int id0 = __shfl_sync(~0u, cur.id, 2 * n), id1 = __shfl_sync(~0u, cur.id, 2 * n + 1);
-      if (ok && n < mine && lane == 0) issue(n, (waits + n) % S, id0, id1);
+      issue(n, n < mine ? id0 : -1, n < mine ? id1 : -1);
     }
     next = lookup(16);
 
-    for (int n = 0; n < mine && ok; ++n, ++waits) {
-      const int stage = waits % S;
+    for (int n = 0; n < mine; ++n) {
+      const int stage = n % S;
       if ((n & 15) == 0 && n > 0) {
         cur = next;
         next = lookup(n + 16);
@@ -362,9 +351,8 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
         ks[i] = __shfl_sync(~0u, cur.ks, src + i);
         vs[i] = __shfl_sync(~0u, cur.vs, src + i);
       }
-      ok = mbar_wait(bar0 + 8 * stage, (waits / S) & 1, abort_flag, &g_kv8_status, 41);
-      ok = __all_sync(~0u, ok);
-      if (!ok) break;
+      cp_async_wait<S - 1>();  // one group per step: this step's copies of this lane have landed,
+      __syncwarp();            // and the other lanes'
       const uint8_t* kt = ring_ptr + stage * 2 * L::kHalf;
       const uint8_t* vt = kt + L::kHalf;
 
@@ -512,18 +500,13 @@ split_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUt
         }
       }
       __syncwarp();  // every lane has its bytes: the stage may be filled again
-      if (n + S < mine) {
-        const int at = 2 * ((n + S) & 15);
-        const int a0 = __shfl_sync(~0u, cur.id, at), a1 = __shfl_sync(~0u, cur.id, at + 1);
-        const int b0 = __shfl_sync(~0u, next.id, at), b1 = __shfl_sync(~0u, next.id, at + 1);
-        const bool same = ((n + S) >> 4) == (n >> 4);
-        if (lane == 0) issue(n + S, stage, same ? a0 : b0, same ? a1 : b1);
-      }
+      const int at = 2 * ((n + S) & 15);
+      const bool same = ((n + S) >> 4) == (n >> 4), more = n + S < mine;
+      const int ahead = same ? cur.id : next.id;
+      const int a0 = __shfl_sync(~0u, ahead, at), a1 = __shfl_sync(~0u, ahead, at + 1);
+      issue(n + S, more ? a0 : -1, more ? a1 : -1);
     }
-    if (!ok) {  // let copies in flight land before the shared memory is used or given back
-      const uint64_t t0 = global_timer_ns();
-      while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
-    }
+    cp_async_wait<0>();
 
     // ---- the four warps' results become one
 #pragma unroll
@@ -676,12 +659,6 @@ int64_t ws_bytes(int ctas, int dim) {
 template <typename T, int D, int NQ>
 cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, dim3 grid, cudaStream_t stream,
                          const char** err) {
-  CUtensorMap tk, tv;
-  const int box = p.cache.block_size < kStep ? p.cache.block_size : kStep;
-  if (!make_map(&tk, p.cache.k, p.cache, box) || !make_map(&tv, p.cache.v, p.cache, box)) {
-    *err = "cuTensorMapEncodeTiled failed";
-    return cudaErrorInvalidValue;
-  }
   SplitWs ws = {};
   if (shape.stream) {
     char* at = static_cast<char*>(p.workspace);
@@ -696,7 +673,7 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
   static std::atomic<uint64_t> ready{0};
   cudaError_t st = allow_smem(kern, smem, ready);
   if (st != cudaSuccess) return st;
-  st = launch_dependent(kern, grid, dim3(kSplitThreads), smem, stream, tk, tv, p, shape, ws);
+  st = launch_dependent(kern, grid, dim3(kSplitThreads), smem, stream, p, shape, ws);
   if (st != cudaSuccess || !shape.stream) return st;
   return launch_dependent(join_kernel<T, D, 8 * NQ>, dim3(grid.x, 2), dim3(kJoinThreads), 0, stream, p, shape, ws);
 }
@@ -762,17 +739,6 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   if (p.cache.dim == 128)
     return f16 ? launch_t<__half, 128>(p, most, stream, err) : launch_t<__nv_bfloat16, 128>(p, most, stream, err);
   return f16 ? launch_t<__half, 64>(p, most, stream, err) : launch_t<__nv_bfloat16, 64>(p, most, stream, err);
-}
-
-int kv8_status_fetch_and_clear() {
-  int h = 0;
-  if (cudaMemcpyFromSymbol(&h, g_kv8_status, sizeof(int)) != cudaSuccess) return -1;
-  if (h != 0) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_kv8_status, &z, sizeof(int));
-  }
-  const int f = kv8_prefill_status_fetch_and_clear();
-  return h != 0 ? h : f;
 }
 
 }  // namespace disc_b200

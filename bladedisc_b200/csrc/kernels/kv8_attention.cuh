@@ -11,6 +11,20 @@
 
 namespace disc_b200 {
 
+// One lane of a converged warp, the same each time.  Copies, products and commits behind it, in code that the whole warp
+// runs with uniform values, issue back to back; behind `lane == 0` a commit cost 180 cycles of the tensor core and a
+// copy 170 of its warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(r));
+  return r != 0;
+}
 // Bytes b (as b + 128) `sel` picks two of them -> two f16 with the values b.
 __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t biased, uint32_t sel) {
   const uint32_t w = __byte_perm(biased, 0x64646464u, sel);
@@ -67,6 +81,5 @@ inline bool make_map(CUtensorMap* tm, const int8_t* base, const Kv8Cache& c, int
 
 // Many rows: requests with more than min_rows query rows per kv head (kv8_prefill.cu).
 cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err);
-int kv8_prefill_status_fetch_and_clear();
 
 }  // namespace disc_b200

@@ -88,19 +88,6 @@ __device__ __forceinline__ void stg256(void* p, const uint32_t* r) {
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-// One lane of a converged warp, the same each time.  Products and commits behind it, in code that the whole warp runs
-// with uniform values, issue back to back; behind `lane == 0` each commit cost 180 cycles of the tensor core.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(r));
-  return r != 0;
-}
 __device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t"
@@ -741,7 +728,7 @@ cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaSt
                           : launch_t<__nv_bfloat16, 64>(p, min_rows, stream, err);
 }
 
-int kv8_prefill_status_fetch_and_clear() {
+int kv8_status_fetch_and_clear() {
   int h = 0;
   if (cudaMemcpyFromSymbol(&h, g_kv8_prefill_status, sizeof(int)) != cudaSuccess) return -1;
   if (h != 0) {
