@@ -41,6 +41,7 @@ constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
 constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one,
+constexpr int kDirectMost = 4096;  // longest cache that is not cut when there are items for two rounds of CTAs
 constexpr int kSplitRowsMixed = 8;  // and with prompts in the batch: what fits one tile of eight rows
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // a score may exceed the running maximum by this much (in log2) and
@@ -91,10 +92,12 @@ __device__ __forceinline__ void load_q16(const __nv_bfloat16* p, bool there, flo
 #pragma unroll
   for (int i = 0; i < 8; ++i) w[i] = pack2(f[2 * i] * mul, f[2 * i + 1] * mul, __half());
 }
+constexpr int kMaxRows = 16;  // of an item
+
 // What is left of a share that ends inside an item: a maximum, a sum and an output per row.
 struct SplitWs {
-  float* o;      // [2 * ctas][16 rows][dim]: slot 2 c for a piece that does not start its item, 2 c + 1 for one that does
-  float2* ml;    // [2 * ctas][16 rows]
+  float* o;      // [2 * ctas][rows][dim]: slot 2 c for a piece that does not start its item, 2 c + 1 for one that does
+  float2* ml;    // [2 * ctas][rows]
   int4* desc;    // [ctas] {request, kv head, row tile, pieces} of the item that CTA c starts and does not finish
 };
 
@@ -109,7 +112,7 @@ struct SplitSmem {
   static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kHalf = kStep * D;  // bytes of the keys (or values) of one step
   static constexpr int kRing = kSplitWarps * kStages * 2 * kHalf;
-  static constexpr int kParts = kSplitWarps * 16 * D * 4;  // O of every warp, in the place of the rings
+  static constexpr int kParts = kSplitWarps * kMaxRows * D * 4;  // O of every warp, in the place of the rings
   static constexpr int kDynamic = kRing > kParts ? kRing : kParts;
 };
 
@@ -138,7 +141,7 @@ split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spl
   constexpr int NV = D / 16;  // m tiles of the second
   constexpr int ROWS = 8 * NQ;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float part_m[W][16], part_l[W][16];
+  __shared__ float part_m[W][ROWS], part_l[W][ROWS];
   __shared__ long long sums[W];
   __shared__ int found[2];
   __shared__ long long found_at;
@@ -200,7 +203,7 @@ split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spl
     if (threadIdx.x == 0) ws.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     __syncthreads();
     if (left <= 0) {  // nothing of an item that may go on around this CTA
-      if (threadIdx.x < 16) ws.ml[static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x] = make_float2(-INFINITY, 0.f);
+      if (threadIdx.x < ROWS) ws.ml[2 * static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x] = make_float2(-INFINITY, 0.f);
       return;
     }
     r = found[0];
@@ -234,56 +237,6 @@ split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spl
     // keys that the first row of the tile sees, and the last one
     const int lim_first = static_cast<int>(max(static_cast<int64_t>(0), behind + row0 / G));
     const int keys = static_cast<int>(max(static_cast<int64_t>(0), behind + (row0 + rows - 1) / G));
-
-    // Q fragments: this lane loads row 8 j + g; its scores belong to the rows 8 j + 2 t + e
-    uint32_t qb[NQ][KQ][2];
-    float qmul[NQ][2], m[NQ][2], l[NQ][2];
-    int lim[NQ][2];
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      const int row = j * 8 + g;
-      const int i = (row0 + row) / G, h = (row0 + row) % G;
-      const int64_t at = tok0 + i;
-      const bool there = row < rows && at >= 0 && at < p.tokens;
-      const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q : 0) + (head * G + (there ? h : 0)) * D + 16 * t;
-      float mul = 1.f;
-      if constexpr (!std::is_same<T, __half>::value) {
-        uint32_t top = 0;
-        if (there)
-#pragma unroll
-          for (int i2 = 0; i2 < D / 64; ++i2) top = max(top, top_q16(x + 64 * i2));
-        top = max(top, __shfl_xor_sync(~0u, top, 1));
-        top = max(top, __shfl_xor_sync(~0u, top, 2));
-        mul = row_power(top);
-      }
-#pragma unroll
-      for (int i2 = 0; i2 < D / 64; ++i2) {
-        uint32_t w[8];
-        load_q16(x + 64 * i2, there, mul, w);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          qb[j][i2 * 4 + k][0] = w[2 * k];
-          qb[j][i2 * 4 + k][1] = w[2 * k + 1];
-        }
-      }
-      const float f = p.scale * 1.4426950408889634f / mul;
-      const int see = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i)) : 0;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        qmul[j][e] = __shfl_sync(~0u, f, (2 * t + e) * 4);
-        lim[j][e] = __shfl_sync(~0u, see, (2 * t + e) * 4);
-        m[j][e] = -INFINITY;
-        l[j][e] = 0.f;
-      }
-    }
-
-    float o[NQ][NV][4];
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
-    }
-    float ref = kRef0, inv_ref = 1.f / kRef0;
 
     // this warp's steps: first, first + W, ...
     const int first = static_cast<int>(s0) + warp;
@@ -336,6 +289,56 @@ split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spl
       issue(n, n < mine ? id0 : -1, n < mine ? id1 : -1);
     }
     next = lookup(16);
+
+    // Q fragments, while the first keys are on their way: this lane loads row 8 j + g; its scores belong to the rows 8 j + 2 t + e
+    uint32_t qb[NQ][KQ][2];
+    float qmul[NQ][2], m[NQ][2], l[NQ][2];
+    int lim[NQ][2];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      const int row = j * 8 + g;
+      const int i = (row0 + row) / G, h = (row0 + row) % G;
+      const int64_t at = tok0 + i;
+      const bool there = row < rows && at >= 0 && at < p.tokens;
+      const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q : 0) + (head * G + (there ? h : 0)) * D + 16 * t;
+      float mul = 1.f;
+      if constexpr (!std::is_same<T, __half>::value) {
+        uint32_t top = 0;
+        if (there)
+#pragma unroll
+          for (int i2 = 0; i2 < D / 64; ++i2) top = max(top, top_q16(x + 64 * i2));
+        top = max(top, __shfl_xor_sync(~0u, top, 1));
+        top = max(top, __shfl_xor_sync(~0u, top, 2));
+        mul = row_power(top);
+      }
+#pragma unroll
+      for (int i2 = 0; i2 < D / 64; ++i2) {
+        uint32_t w[8];
+        load_q16(x + 64 * i2, there, mul, w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          qb[j][i2 * 4 + k][0] = w[2 * k];
+          qb[j][i2 * 4 + k][1] = w[2 * k + 1];
+        }
+      }
+      const float f = p.scale * 1.4426950408889634f / mul;
+      const int see = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i)) : 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qmul[j][e] = __shfl_sync(~0u, f, (2 * t + e) * 4);
+        lim[j][e] = __shfl_sync(~0u, see, (2 * t + e) * 4);
+        m[j][e] = -INFINITY;
+        l[j][e] = 0.f;
+      }
+    }
+
+    float o[NQ][NV][4];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+    }
+    float ref = kRef0, inv_ref = 1.f / kRef0;
 
     for (int n = 0; n < mine; ++n) {
       const int stage = n % S;
@@ -560,8 +563,8 @@ split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spl
           static_cast<T*>(p.out)[at * p.ld_out + (head * G + (row0 + row) % G) * D + d] =
               pack_one(sum == 0.f ? 0.f : acc / sum, T());
       } else {
-        ws.o[(slot * 16 + row) * D + d] = acc;
-        if (d == 0) ws.ml[slot * 16 + row] = make_float2(top, sum);
+        ws.o[(slot * ROWS + row) * D + d] = acc;
+        if (d == 0) ws.ml[slot * ROWS + row] = make_float2(top, sum);
       }
     }
     if (!whole && s0 == 0 && threadIdx.x == 0) {
@@ -609,7 +612,7 @@ join_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, Spli
     if (r < rows) {
 #pragma unroll 4
       for (int i = part_of; i < pieces; i += per_row) {
-        const int64_t slot = (i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * 16 + r;
+        const int64_t slot = (i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * ROWS + r;
         const float2 ml = ws.ml[slot];
         const float4 v = *reinterpret_cast<const float4*>(ws.o + slot * D + d);
         if (ml.x == -INFINITY && ml.y == 0.f) continue;  // saw no key (its output may not even be written)
@@ -653,7 +656,7 @@ bool misaligned(const void* p, uintptr_t by) { return (reinterpret_cast<uintptr_
 int stream_ctas() { return 3 * device_sm_count(); }
 
 int64_t ws_bytes(int ctas, int dim) {
-  return static_cast<int64_t>(ctas) * (2 * 16 * (static_cast<int64_t>(dim) * 4 + 8) + 16);
+  return static_cast<int64_t>(ctas) * (2 * kMaxRows * (dim * 4 + 8) + 16);
 }
 
 template <typename T, int D, int NQ>
@@ -663,9 +666,9 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
   if (shape.stream) {
     char* at = static_cast<char*>(p.workspace);
     ws.o = reinterpret_cast<float*>(at);
-    at += static_cast<int64_t>(grid.x) * 2 * 16 * D * 4;
+    at += static_cast<int64_t>(grid.x) * 2 * 8 * NQ * D * 4;
     ws.ml = reinterpret_cast<float2*>(at);
-    at += static_cast<int64_t>(grid.x) * 2 * 16 * 8;
+    at += static_cast<int64_t>(grid.x) * 2 * 8 * NQ * 8;
     ws.desc = reinterpret_cast<int4*>(at);
   }
   auto kern = split_kernel<T, D, NQ>;
@@ -675,22 +678,24 @@ cudaError_t launch_split(const Kv8AttentionParams& p, const SplitShape& shape, d
   if (st != cudaSuccess) return st;
   st = launch_dependent(kern, grid, dim3(kSplitThreads), smem, stream, p, shape, ws);
   if (st != cudaSuccess || !shape.stream) return st;
-  return launch_dependent(join_kernel<T, D, 8 * NQ>, dim3(grid.x, 2), dim3(kJoinThreads), 0, stream, p, shape, ws);
+  return launch_dependent(join_kernel<T, D, 8 * NQ>, dim3(grid.x, 4), dim3(kJoinThreads), 0, stream, p, shape, ws);
 }
 
 template <typename T, int D>
 cudaError_t launch_t(const Kv8AttentionParams& p, int max_rows, cudaStream_t stream, const char** err) {
   const int64_t rows = std::min(static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads), static_cast<int64_t>(max_rows));
+  const int nq = rows <= 8 ? 1 : 2;
+  const int64_t row_tiles = (rows + 8 * nq - 1) / (8 * nq);
+  const int64_t items = row_tiles * p.cache.kv_heads * p.requests;
   SplitShape shape;
   shape.max_rows = max_rows;
-  shape.stream = p.max_kv > kKv8DirectKeys ? 1 : 0;
-  const int tile_rows = rows > 8 ? 16 : 8;
-  shape.row_tiles = static_cast<int>((rows + tile_rows - 1) / tile_rows);
+  shape.row_tiles = static_cast<int>(row_tiles);
+  // one CTA per item: at most what kDirectMost keys take if the others have nothing to do meanwhile
+  shape.stream = p.max_kv > kKv8DirectKeys && (p.max_kv > kDirectMost || items < 2 * stream_ctas()) ? 1 : 0;
   const dim3 grid = shape.stream ? dim3(static_cast<unsigned>(stream_ctas()))
                                  : dim3(static_cast<unsigned>(shape.row_tiles * p.cache.kv_heads),
                                         static_cast<unsigned>(p.requests));
-  return rows > 8 ? launch_split<T, D, 2>(p, shape, grid, stream, err)
-                  : launch_split<T, D, 1>(p, shape, grid, stream, err);
+  return nq == 1 ? launch_split<T, D, 1>(p, shape, grid, stream, err) : launch_split<T, D, 2>(p, shape, grid, stream, err);
 }
 
 }  // namespace

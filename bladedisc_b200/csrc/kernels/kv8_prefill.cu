@@ -271,14 +271,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   const Kv8Cache& c = p.cache;
   const int bs = c.block_size, G = p.q_heads / c.kv_heads;
 
-  // ---- the item: heads vary fastest, the rows with the most keys come first
+  // ---- the item: heads vary fastest, then requests; the rows with the most keys come first
   grid_dep_wait();
   grid_dep_launch();
-  const int head = blockIdx.x, r = blockIdx.z;
+  const int head = blockIdx.x, r = blockIdx.y;
   const int q_asked = max(p.q_lens[r], 0);
   const int q_len = min(q_asked, p.max_q);
   const int rows_all = q_len * G;  // max_q * G fits
-  const int row0 = (gridDim.y - 1 - blockIdx.y) * 2 * kTile;
+  const int row0 = (gridDim.z - 1 - blockIdx.z) * 2 * kTile;
   if (rows_all <= min_rows || row0 >= rows_all) return;
   const int rows = min(2 * kTile, rows_all - row0);
   const int kv_len = min(max(p.kv_lens[r], 0), p.table_width * bs);
@@ -710,8 +710,8 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
   static std::atomic<uint64_t> ready{0};
   cudaError_t st = allow_smem(kern, smem, ready);
   if (st != cudaSuccess) return st;
-  const dim3 grid(static_cast<unsigned>(p.cache.kv_heads), static_cast<unsigned>(blocks),
-                  static_cast<unsigned>(p.requests));
+  const dim3 grid(static_cast<unsigned>(p.cache.kv_heads), static_cast<unsigned>(p.requests),
+                  static_cast<unsigned>(blocks));
   // rows of q and out on 32-byte boundaries take whole sectors per lane
   const int wide = ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0 &&
                    p.ld_q % 16 == 0 && p.ld_out % 16 == 0;
