@@ -243,10 +243,21 @@ __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs,
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+constexpr int kScan = 1024;  // requests among which a CTA looks for those that this kernel serves
+__device__ __forceinline__ int rows_of(const Kv8AttentionParams& p, int q_len) {
+  return min(max(q_len, 0), p.max_q) * (p.q_heads / p.cache.kv_heads);  // max_q * group fits
+}
+
+// Position of the n-th set bit (from 0), found by a converged warp.
+__device__ __forceinline__ int nth_bit(uint32_t mask, int n, int lane) {
+  const bool it = (mask >> lane & 1) && __popc(mask & ((1u << lane) - 1)) == n;
+  return __ffs(__ballot_sync(~0u, it)) - 1;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-               const __grid_constant__ Kv8AttentionParams p, int min_rows, int box_rows, int wide) {
+               const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, int box_rows, int wide) {
   using L = Smem<D>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -274,18 +285,63 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   // ---- the item: heads vary fastest, then requests; the rows with the most keys come first
   grid_dep_wait();
   grid_dep_launch();
-  const int head = blockIdx.x, r = blockIdx.y;
-  const int q_asked = max(p.q_lens[r], 0);
+  // (the requests that are not for this kernel come last of all, so that their CTAs, which end at once, hold up nobody)
+  const uint32_t KH = c.kv_heads, round = blockIdx.x / KH;
+  const int head = static_cast<int>(blockIdx.x - round * KH);
+  // up to 32 requests: a lane per request has all that is needed of it, one load latency in all
+  int my_len = 0, my_kv = 0, my_start = 0;
+  if (lane < p.requests) {
+    my_len = p.q_lens[lane];
+    my_kv = p.kv_lens[lane];
+    my_start = p.q_start[lane];
+  }
+  uint32_t here = 0, mask = 0;
+  if (p.requests <= 32) {
+    mask = __ballot_sync(~0u, lane < p.requests && rows_of(p, my_len) > min_rows);
+    here = __popc(mask);
+  } else if (p.requests <= kScan) {
+    for (int i = 0; i < p.requests; i += 32)
+      here += __popc(__ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows));
+  } else {
+    here = p.requests;
+  }
+  if (here == 0 || round / here >= blocks) return;
+  const uint32_t from_last = round / here;
+  int r = static_cast<int>(round - from_last * here);
+  int q_asked, kv_have;
+  int64_t tok0;
+  if (p.requests <= 32) {
+    r = nth_bit(mask, r, lane);
+    q_asked = __shfl_sync(~0u, my_len, r);
+    kv_have = __shfl_sync(~0u, my_kv, r);
+    tok0 = __shfl_sync(~0u, my_start, r);
+  } else {
+    if (p.requests <= kScan) {
+      int nth = r;
+      for (int i = 0; i < p.requests; i += 32) {
+        const uint32_t m =
+            __ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows);
+        if (nth < __popc(m)) {
+          r = i + nth_bit(m, nth, lane);
+          break;
+        }
+        nth -= __popc(m);
+      }
+    }
+    q_asked = p.q_lens[r];
+    kv_have = p.kv_lens[r];
+    tok0 = p.q_start[r];
+  }
+  q_asked = max(q_asked, 0);
   const int q_len = min(q_asked, p.max_q);
   const int rows_all = q_len * G;  // max_q * G fits
-  const int row0 = (gridDim.z - 1 - blockIdx.z) * 2 * kTile;
+  const int row0 = static_cast<int>(blocks - 1 - from_last) * 2 * kTile;
   if (rows_all <= min_rows || row0 >= rows_all) return;
   const int rows = min(2 * kTile, rows_all - row0);
-  const int kv_len = min(max(p.kv_lens[r], 0), p.table_width * bs);
+  const int kv_len = min(max(kv_have, 0), p.table_width * bs);
   const int64_t behind = static_cast<int64_t>(kv_len) - q_asked + 1;  // token i sees behind + i keys
   const int keys = static_cast<int>(max(static_cast<int64_t>(0), behind + (row0 + rows - 1) / G));
   const int nt = (keys + kTile - 1) / kTile, nu = (keys + kKeys - 1) / kKeys;
-  const int64_t tok0 = p.q_start[r];
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tk);
@@ -695,7 +751,7 @@ template <typename T, int D>
 cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
   const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
   const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile);
-  if (rows > INT32_MAX - 2 * kTile || blocks > 65535) {
+  if (rows > INT32_MAX - 2 * kTile || blocks * p.cache.kv_heads * p.requests > INT32_MAX) {
     *err = "too many query rows";
     return cudaErrorInvalidValue;
   }
@@ -710,12 +766,11 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
   static std::atomic<uint64_t> ready{0};
   cudaError_t st = allow_smem(kern, smem, ready);
   if (st != cudaSuccess) return st;
-  const dim3 grid(static_cast<unsigned>(p.cache.kv_heads), static_cast<unsigned>(p.requests),
-                  static_cast<unsigned>(blocks));
+  const dim3 grid(static_cast<unsigned>(blocks * p.cache.kv_heads * p.requests));
   // rows of q and out on 32-byte boundaries take whole sectors per lane
   const int wide = ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0 &&
                    p.ld_q % 16 == 0 && p.ld_out % 16 == 0;
-  return launch_dependent(kern, grid, dim3(kThreads), smem, stream, tk, tv, p, min_rows, box, wide);
+  return launch_dependent(kern, grid, dim3(kThreads), smem, stream, tk, tv, p, min_rows, static_cast<uint32_t>(blocks), box, wide);
 }
 
 }  // namespace
