@@ -714,7 +714,7 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   else if (p.tokens < 0 || p.tokens > INT32_MAX || p.requests < 0 || p.requests > 65535 || p.table_width < 0 ||
            p.max_q < 0 || p.max_kv < 0)
     *err = "sizes out of range";
-  else if (static_cast<int64_t>(p.table_width) * p.cache.block_size > INT32_MAX)
+  else if (static_cast<int64_t>(p.table_width) * p.cache.block_size > (1 << 30))
     *err = "positions are 32-bit: the table is too wide";
   if (*err) return cudaErrorInvalidValue;
   if (p.tokens == 0 || p.requests == 0 || p.max_q == 0) return cudaSuccess;
@@ -731,9 +731,7 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   const bool many = rows > kSplitRows, few = !many || p.requests > 1;
   if (few && p.max_kv > kKv8DirectKeys && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < ws_bytes(stream_ctas(), p.cache.dim)))
     *err = "the workspace is too small or not 16-byte aligned";
-  if (p.table_width == 0) {  // no keys at all, but the kernel's tensor maps want a cache
-    if (p.cache.num_blocks == 0) *err = "a cache without blocks";
-  }
+  if (p.cache.num_blocks == 0) *err = "a cache without blocks";
   if (*err) return cudaErrorInvalidValue;
   if (many) {
     const cudaError_t st = kv8_prefill_launch(p, few ? kSplitRowsMixed : 0, stream, err);

@@ -392,6 +392,94 @@ def test_a_request_whose_rows_are_not_in_q(ops):
             _check(o, w, sl)
 
 
+@pytest.mark.parametrize("q_len", [1, 6, 180])
+def test_a_row_of_nan_stays_alone(ops, q_len):
+    """Infinities and NaN in one query row leave every other row as it is."""
+    rng = np.random.default_rng(14)
+    got, _, _, (q, d, args, mq) = _attend(ops, rng, [q_len, 3], [700, 40], 16, 2, 4, 64, torch.bfloat16)
+    bad = q.clone()
+    bad[0, 1, 5], bad[0, 2, 7] = float("nan"), float("inf")
+    again = ops.kv8_attention(bad, *d, *args, max_q=mq, out=torch.full_like(got, 3.0))
+    same = torch.ones(got.shape[:2], dtype=torch.bool)
+    same[0, 1:3] = False
+    assert torch.equal(again[same.cuda()], got[same.cuda()]) and torch.isnan(again[0, 1]).all()
+
+
+def test_offsets_past_32_bits(ops):
+    """Blocks that lie behind the first four gigabytes of levels: append, read and both attention kernels."""
+    rng = np.random.default_rng(15)
+    blocks, heads, size, dim = 34000, 8, 128, 128  # 4.46 GB of keys, as much of values
+    k, v = (torch.zeros(blocks, heads, size, dim, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(blocks, heads, device="cuda") for _ in range(2))
+    ids = np.array([33999, 33990, 17, 33998, 33000], np.int32)
+    small = _cache(rng, 5, heads, size, dim)
+    at = dev(ids, torch.int64)
+    for big, part, kind in ((k, small[0], torch.int8), (v, small[1], torch.int8), (ks, small[2], torch.float32),
+                            (vs, small[3], torch.float32)):
+        big[at] = dev(part, kind)
+    for q_len, kv in ((1, 600), (300, 600), (5, 333)):
+        q = torch.from_numpy(rng.standard_normal((q_len, heads, dim))).half().cuda()
+        args = [dev([[0, 1, 2, 3, 4]]), dev([0, q_len]), dev([q_len]), dev([kv])]
+        want = ops.kv8_attention(q, *_dev_cache(small), *args, max_q=q_len)
+        got = ops.kv8_attention(q, k, v, ks, vs, dev(ids[None]), *args[1:], max_q=q_len)
+        assert torch.equal(got, want)
+    slots = np.array([33998 * size + 7, 33998 * size + 8, 33000 * size + 127], np.int64).astype(np.int32)
+    x = rng.standard_normal((3, 2 * heads * dim)).astype(np.float32)
+    xt = torch.from_numpy(x).half().cuda()
+    ops.kv8_append(xt, k, v, ks, vs, dev(slots))
+    local = np.array([3 * size + 7, 3 * size + 8, 4 * size + 127], np.int32)
+    rows = xt.float().cpu().numpy().reshape(3, -1, dim)
+    for big, scale, i, part in ((k, ks, 0, rows[:, :heads]), (v, vs, 1, rows[:, heads:])):
+        levels, scales = kv8_ref.append(part, small[i], small[2 + i], local)
+        assert np.array_equal(big[at].cpu().numpy(), levels) and np.array_equal(scale[at].cpu().numpy(), scales)
+    a, b = ops.kv8_read(k, v, ks, vs, dev(ids), torch.float16)
+    assert torch.equal(a, (k[at].float() * ks[at][..., None, None]).half())
+    assert torch.equal(b, (v[at].float() * vs[at][..., None, None]).half())
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_two_streams_at_once(ops, captured):
+    """Calls that need a workspace on two streams, and two captured graphs of them, run side by side."""
+    rng = np.random.default_rng(16)
+    cases = []
+    for i in range(2):
+        got, _, _, (q, d, args, mq) = _attend(ops, rng, [1, 2], [9000, 5000 + i], 16, 2, 8, 128, torch.float16)
+        cases.append((got, lambda q=q, d=d, args=args, mq=mq, got=got: ops.kv8_attention(
+            q, *d, *args, max_q=mq, out=torch.full_like(got, 3.0))))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    runs, results = [], []
+    for s, (_, call) in zip(streams, cases):
+        if captured:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                results.append(call())
+            runs.append(g.replay)
+        else:
+            results.append(None)
+            runs.append(call)
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                r = runs[i]()
+                results[i] = results[i] if captured else r
+    torch.cuda.synchronize()
+    for (want, _), r in zip(cases, results):
+        assert torch.equal(r, want)
+
+
+def test_many_requests_with_few_prompts_among_them(ops):
+    """More requests than a warp, prompts scattered between single tokens and empty ones."""
+    rng = np.random.default_rng(17)
+    n = 70
+    q_lens = [1] * n
+    for i, v in ((3, 150), (33, 90), (40, 0), (69, 200)):
+        q_lens[i] = v
+    kv_lens = [max(v, int(rng.integers(1, 120))) for v in q_lens]
+    got, want, slack, _ = _attend(ops, rng, q_lens, kv_lens, 16, 2, 4, 64, torch.float16)
+    _check(got, want, slack)
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("captured", [False, True])
 def test_decode_steps_together(ops, captured):

@@ -131,6 +131,14 @@ def test_attention(lib):
     _refused(lib, fn, args(ld_out=4 * 64 + 4), "16-byte")
     _refused(lib, fn, args(out=0x1008), "16-byte")
     _refused(lib, fn, args(scale=0.0), "positive")
+    # a long cache wants its workspace, whole and aligned; a short one none
+    need = lib.disc_b200_kv8_attention_workspace_bytes(64, 513)
+    assert need > 0 and lib.disc_b200_kv8_attention_workspace_bytes(64, L.KV8_DIRECT_KEYS) == 0
+    for kw in (dict(), dict(workspace=0x1000, workspace_bytes=need - 1), dict(workspace=0x1008, workspace_bytes=need)):
+        _refused(lib, fn, args(max_kv=513, **kw), "workspace")
+    a = args()
+    a.cache.num_blocks = 0
+    _refused(lib, fn, a, "without blocks")
     _refused(lib, fn, args(scale=float("nan")), "positive")
     for name in ("q", "out", "table", "q_start", "q_lens", "kv_lens"):
         _refused(lib, fn, args(**{name: None}), "null operand")
