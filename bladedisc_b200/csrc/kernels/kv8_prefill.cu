@@ -13,8 +13,14 @@
 //                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
 // Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
 // loader keeps (O is in its units), so that P stays in the range of f16; see kPScaleLog2.
-// Bound by the tensor core and, as closely, by exp2: at dim 128 a tile of 128 x 128 costs 1024 cycles of products
-// and 1024 cycles of the SM's 16 exp2 per cycle.
+// What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all): shared memory 3070 cycles (levels in
+// and out 512, operands out 512, Q and K into S 1536 at 64 keys a product, V into O 512), exp2 2048 at 16 a cycle less
+// the quarter that goes to the FMA pipe, products 2560.  Measured at 4095 tokens behind 12289, 32 over 8 heads: 0.98 ms
+// = 980 TFLOP/s, 0.59 of the measured bf16 rate; one of eight CTA rounds is not full.  What was measured on the way there:
+// scores of 128 keys in one buffer 1.07 ms (the chain softmax, P V, S is exposed), one issuer for both tiles 1.44,
+// products issued behind `lane == 0` 1.20, levels to registers instead of TMA 1.40, exp2 all on the MUFU 1.01, half of
+// them on the FMA pipe 1.08, taking turns in exp2 1.02.  Short prompts pay for the start of a CTA (8300 cycles to the
+// first score) and its end (3900): 4 prompts of 256 to 2048 tokens, 32 heads: 130 us = 505 TFLOP/s.
 #include "kv8.h"
 
 #include <type_traits>
@@ -69,8 +75,8 @@ struct Smem {
   static constexpr int kInfoAt = kRawV + kRaw;
   static constexpr int kBars = kInfoAt + kInfo * static_cast<int>(sizeof(TileInfo));
   // q_full[2], raw_full[2], raw_free[2], op_full[2][2], op_free[2][2], s_full[2][2], p_full[2][2], pv_done[2][2],
-  // info_full[4], turn[2][4]
-  static constexpr int kNumBars = 26 + kInfo + 2 * kSoftmaxWarps;
+  // info_full[4]
+  static constexpr int kNumBars = 26 + kInfo;
   static constexpr int kMisc = kBars + kNumBars * 8;
   static constexpr int kTotal = kMisc + 16;
   static constexpr int kDynamic = kTotal + 1024;
@@ -198,9 +204,7 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
 }
 // Scores of one row and step -> P in TMEM and the row's sum.  EDGE: some keys are hidden from some rows.
 // `left` keys are visible from the step's first on; groups that are not `present` are not.
-#ifndef POLY
-#define POLY 0x20
-#endif
+constexpr uint32_t kOnFma = 0x22;  // of the eight pairs of a group, those whose exp2 is a polynomial
 template <bool EDGE>
 __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, float rmul, float off, uint32_t t_p,
                                              int left, uint32_t present, uint64_t* sum) {
@@ -217,7 +221,7 @@ __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs,
       for (int e = 0; e < 8; ++e) {
         float a, b;
         const uint64_t x = fma2(pair(__uint_as_float(s[g * 16 + 2 * e]), __uint_as_float(s[g * 16 + 2 * e + 1])), f2, off2);
-        if (!EDGE && (POLY >> e & 1)) {
+        if (!EDGE && (kOnFma >> e & 1)) {
           unpair(exp2_pair(x), a, b);
         } else {
           unpair(x, a, b);
@@ -274,7 +278,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   auto p_full = [&](int q, int u) { return bar(9 + q, u & 1); };
   auto pv_done = [&](int q, int u) { return bar(11 + q, u & 1); };
   auto info_full = [&](int i) { return bars + 8u * (26 + i); };
-  auto turn = [&](int q, int w) { return bars + 8u * (26 + kInfo + q * kSoftmaxWarps + w); };
   TileInfo* info = reinterpret_cast<TileInfo*>(smem + L::kInfoAt);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
@@ -359,7 +362,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       }
     }
     for (int i = 0; i < kInfo; ++i) mbar_init(info_full(i), 1);
-    for (int i = 0; i < 2 * kSoftmaxWarps; ++i) mbar_init(turn(0, i), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -389,7 +391,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const int lim = there ? static_cast<int>(max(static_cast<int64_t>(0), behind + i_tok)) : INT32_MAX;
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp % kSoftmaxWarps) * 32) << 16);
     const uint32_t t_o = t_lane + 256 + q * D;
-    const bool active = q * kTile < rows, both = false;
+    const bool active = q * kTile < rows;
     float mul = 1.f;
     if (active && nt > 0) {
       const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q + (head * G + h) * D : 0);
@@ -501,16 +503,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
       }
       const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
-      // the exponentials of the two query tiles take turns: while one warp of a scheduler is in them the other loads
-      // its scores and finds its maximum
-      if (both && (q == 1 || u > 0)) {
-        ok = wait(turn(q, warp % kSoftmaxWarps), (q == 1 ? u : u - 1) & 1, 66);
-        ok = __all_sync(~0u, ok);
-        if (!ok) break;
-      }
       if (!edge) softmax_step<false>(s, fs, ws, rmul, off, t_s, 0, 0, sum);
       else softmax_step<true>(s, fs, ws, rmul, off, t_s, lim - key0, present, sum);
-      if (both && lane == 0) mbar_arrive(turn(q ^ 1, warp % kSoftmaxWarps));
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
