@@ -5,7 +5,7 @@
 // new scale: level' = rne(level * (s_old / s)); the error that adds is at most half a level each time the maximum
 // grows.  Keys are rotated (pairs (i, i + dim / 2)) in fp32 and quantized without a rounding in between.
 //
-// Bound by memory for prompts: 9816 tokens with 32 query and 8 + 8 key / value heads of 128 values in bf16 move 225 MB
+// Bound by memory for prompts: 9815 tokens with 32 query and 8 + 8 key / value heads of 128 values in bf16 move 225 MB
 // in 52 us (0.66 of the measured copy rate), reading 315 blocks back 65 MB in 14 us; by latency for decode steps: 64
 // tokens with 32 + 32 + 32 heads 10 us.
 #include "kv8.h"
@@ -63,7 +63,7 @@ constexpr int kQPasses = 4;       // (token, query head) pairs per thread
 // The first kv_blocks CTAs take a segment of `seg` consecutive tokens and four key / value heads each, a warp per head:
 // every run whose first token lies in the segment, once for the maximum and once for the levels, eight values of each
 // half of the head per lane; the second read comes from the caches (keeping a run in registers instead took 128 of
-// them and was slower: 79 against 72 us for 9800 tokens).  Nothing is shared between warps but the slots.  The other CTAs rotate q, a thread
+// them and was slower: 79 against 72 us for 9815 tokens).  Nothing is shared between warps but the slots.  The other CTAs rotate q, a thread
 // for eight values of each half of kQPasses heads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_constant__ Kv8AppendParams p, int seg, int kv_blocks) {
