@@ -537,16 +537,8 @@ int32_t disc_b200_kv8_read(const disc_b200_kv8_read_args* a, void* stream) {
   return finish(st, "kv8_read", detail);
 }
 
-int64_t disc_b200_kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv) {
-  static_assert(DISC_B200_KV8_DIRECT_KEYS == disc_b200::kKv8DirectKeys, "the header's threshold is the kernel's");
-  return disc_b200::kv8_attention_workspace_bytes(dim, max_kv);
-}
-
-int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* a, void* stream) {
-  if (!a) {
-    g_last_error = "kv8_attention: null args";
-    return 1;
-  }
+namespace {
+disc_b200::Kv8AttentionParams kv8_attention_params(const disc_b200_kv8_attention_args* a) {
   disc_b200::Kv8AttentionParams p;
   p.q = a->q;
   p.out = a->out;
@@ -567,8 +559,22 @@ int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* a, void* str
   p.workspace = a->workspace;
   p.workspace_bytes = a->workspace_bytes;
   p.type = a->type;
+  return p;
+}
+}  // namespace
+
+int64_t disc_b200_kv8_attention_workspace_bytes(const disc_b200_kv8_attention_args* a) {
+  static_assert(DISC_B200_KV8_DIRECT_KEYS == disc_b200::kKv8DirectKeys, "the header's threshold is the kernel's");
+  return a ? disc_b200::kv8_attention_workspace_bytes(kv8_attention_params(a)) : -1;
+}
+
+int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* a, void* stream) {
+  if (!a) {
+    g_last_error = "kv8_attention: null args";
+    return 1;
+  }
   const char* detail = nullptr;
-  const cudaError_t st = disc_b200::kv8_attention_launch(p, static_cast<cudaStream_t>(stream), &detail);
+  const cudaError_t st = disc_b200::kv8_attention_launch(kv8_attention_params(a), static_cast<cudaStream_t>(stream), &detail);
   return finish(st, "kv8_attention", detail);
 }
 

@@ -85,8 +85,8 @@ struct Kv8AttentionParams {
   void* workspace;         // kv8_attention_workspace_bytes, 16-byte aligned
   int64_t workspace_bytes;
 };
-// Device memory a call on the current device needs: fixed per device and head size, none for short caches.
-int64_t kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv);
+// Device memory that a call on the current device needs, from its sizes alone; none for short caches.
+int64_t kv8_attention_workspace_bytes(const Kv8AttentionParams& p);
 cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t stream, const char** err);
 int kv8_status_fetch_and_clear();
 

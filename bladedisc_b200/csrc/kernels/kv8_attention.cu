@@ -706,8 +706,14 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int max_rows, cudaStream_t str
 
 }  // namespace
 
-int64_t kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv) {
-  return max_kv > kKv8DirectKeys ? ws_bytes(stream_ctas(), dim) : 0;
+int64_t kv8_attention_workspace_bytes(const Kv8AttentionParams& p) {
+  if (p.max_kv <= kKv8DirectKeys || kv8_cache_problem(p.cache) || p.q_heads < p.cache.kv_heads || p.q_heads > 65535 ||
+      p.tokens <= 0 || p.tokens > INT32_MAX)
+    return 0;
+  const bool many = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads) > kSplitRows;
+  // one after the other on the stream: they may share it
+  return std::max(!many || p.requests > 1 ? ws_bytes(stream_ctas(), p.cache.dim) : 0,
+                  many ? kv8_prefill_workspace_bytes(p) : 0);
 }
 
 cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t stream, const char** err) {
@@ -735,7 +741,8 @@ cudaError_t kv8_attention_launch(const Kv8AttentionParams& p, cudaStream_t strea
   // Which requests go where is decided on the device, from q_lens; the host knows the bound.
   const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
   const bool many = rows > kSplitRows, few = !many || p.requests > 1;
-  if (few && p.max_kv > kKv8DirectKeys && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < ws_bytes(stream_ctas(), p.cache.dim)))
+  const int64_t need = kv8_attention_workspace_bytes(p);
+  if (need > 0 && (!p.workspace || misaligned(p.workspace, 16) || p.workspace_bytes < need))
     *err = "the workspace is too small or not 16-byte aligned";
   if (p.cache.num_blocks == 0) *err = "a cache without blocks";
   if (*err) return cudaErrorInvalidValue;

@@ -80,6 +80,7 @@ inline bool make_map(CUtensorMap* tm, const int8_t* base, const Kv8Cache& c, int
 }
 
 // Many rows: requests with more than min_rows query rows per kv head (kv8_prefill.cu).
+int64_t kv8_prefill_workspace_bytes(const Kv8AttentionParams& p);
 cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err);
 
 }  // namespace disc_b200

@@ -11,6 +11,7 @@
 //                other tile's products run.
 //   softmax      a warpgroup per query tile, a thread per row: running maximum in the scale of log2, exp2, sums in
 //                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
+// Few rows over a long cache: several CTAs take shares of an item's keys (shares_for) and a second kernel joins them.
 // Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
 // loader keeps (O is in its units), so that P stays in the range of f16; see kPScaleLog2.
 // What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all): shared memory 3070 cycles (levels in
@@ -23,6 +24,7 @@
 // first score) and its end (3900): 4 prompts of 256 to 2048 tokens, 32 heads: 130 us = 505 TFLOP/s.
 #include "kv8.h"
 
+#include <algorithm>
 #include <type_traits>
 
 #include "device_info.h"
@@ -83,17 +85,6 @@ struct Smem {
 };
 static_assert(Smem<128>::kDynamic <= 227 * 1024, "shared memory of one SM");
 
-// 32 bytes at once: a whole sector per lane.
-__device__ __forceinline__ void ldg256(const void* p, uint32_t* r) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "l"(p));
-}
-__device__ __forceinline__ void stg256(void* p, const uint32_t* r) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 __device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t"
@@ -258,10 +249,86 @@ __device__ __forceinline__ int nth_bit(uint32_t mask, int n, int lane) {
   return __ffs(__ballot_sync(~0u, it)) - 1;
 }
 
-template <typename T, int D>
+// What CTA `index` works on: 256 query rows of a kv head of a request.
+struct Item {
+  int r, head, row0, rows;
+  int keys;        // that its last row sees
+  int64_t tok0;    // row of q of the request's first token
+  int64_t behind;  // token i sees behind + i keys
+};
+// Heads vary fastest, then requests; the rows with the most keys come first.  (Requests that are not for this kernel
+// come last of all, so that their CTAs, which end at once, hold up nobody.)  A converged warp; false: nothing.
+__device__ __forceinline__ bool item_of(const Kv8AttentionParams& p, uint32_t index, uint32_t blocks, int min_rows,
+                                        int lane, Item& it) {
+  const uint32_t KH = p.cache.kv_heads, round = index / KH;
+  it.head = static_cast<int>(index - round * KH);
+  // up to 32 requests: a lane per request has all that is needed of it, one load latency in all
+  int my_len = 0, my_kv = 0, my_start = 0;
+  if (lane < p.requests) {
+    my_len = p.q_lens[lane];
+    my_kv = p.kv_lens[lane];
+    my_start = p.q_start[lane];
+  }
+  uint32_t here = 0, mask = 0;
+  if (p.requests <= 32) {
+    mask = __ballot_sync(~0u, lane < p.requests && rows_of(p, my_len) > min_rows);
+    here = __popc(mask);
+  } else if (p.requests <= kScan) {
+    for (int i = 0; i < p.requests; i += 32)
+      here += __popc(__ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows));
+  } else {
+    here = p.requests;
+  }
+  if (here == 0 || round / here >= blocks) return false;
+  const uint32_t from_last = round / here;
+  int r = static_cast<int>(round - from_last * here);
+  int q_asked, kv_have;
+  if (p.requests <= 32) {
+    r = nth_bit(mask, r, lane);
+    q_asked = __shfl_sync(~0u, my_len, r);
+    kv_have = __shfl_sync(~0u, my_kv, r);
+    it.tok0 = __shfl_sync(~0u, my_start, r);
+  } else {
+    if (p.requests <= kScan) {
+      int nth = r;
+      for (int i = 0; i < p.requests; i += 32) {
+        const uint32_t m =
+            __ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows);
+        if (nth < __popc(m)) {
+          r = i + nth_bit(m, nth, lane);
+          break;
+        }
+        nth -= __popc(m);
+      }
+    }
+    q_asked = p.q_lens[r];
+    kv_have = p.kv_lens[r];
+    it.tok0 = p.q_start[r];
+  }
+  it.r = r;
+  const int rows_all = rows_of(p, q_asked);
+  it.row0 = static_cast<int>(blocks - 1 - from_last) * 2 * kTile;
+  if (rows_all <= min_rows || it.row0 >= rows_all) return false;
+  it.rows = min(2 * kTile, rows_all - it.row0);
+  const int kv_len = min(max(kv_have, 0), p.table_width * p.cache.block_size);
+  it.behind = static_cast<int64_t>(kv_len) - max(q_asked, 0) + 1;
+  const int G = p.q_heads / p.cache.kv_heads;
+  it.keys = static_cast<int>(max(static_cast<int64_t>(0), it.behind + (it.row0 + it.rows - 1) / G));
+  return true;
+}
+
+// What a share of the keys leaves of a row when an item has several: row = token * query heads + head.
+struct ShareWs {
+  float* o;    // [shares][rows][dim], of weights that add up to one: nothing overflows on the way to the join
+  float2* ml;  // [shares][rows] maximum and sum
+  int64_t rows;
+};
+
+template <typename T, int D, bool SHARES>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-               const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, int box_rows, int wide) {
+               const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, uint32_t shares, ShareWs ws,
+               int box_rows) {
   using L = Smem<D>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -285,66 +352,18 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   const Kv8Cache& c = p.cache;
   const int bs = c.block_size, G = p.q_heads / c.kv_heads;
 
-  // ---- the item: heads vary fastest, then requests; the rows with the most keys come first
   grid_dep_wait();
   grid_dep_launch();
-  // (the requests that are not for this kernel come last of all, so that their CTAs, which end at once, hold up nobody)
-  const uint32_t KH = c.kv_heads, round = blockIdx.x / KH;
-  const int head = static_cast<int>(blockIdx.x - round * KH);
-  // up to 32 requests: a lane per request has all that is needed of it, one load latency in all
-  int my_len = 0, my_kv = 0, my_start = 0;
-  if (lane < p.requests) {
-    my_len = p.q_lens[lane];
-    my_kv = p.kv_lens[lane];
-    my_start = p.q_start[lane];
-  }
-  uint32_t here = 0, mask = 0;
-  if (p.requests <= 32) {
-    mask = __ballot_sync(~0u, lane < p.requests && rows_of(p, my_len) > min_rows);
-    here = __popc(mask);
-  } else if (p.requests <= kScan) {
-    for (int i = 0; i < p.requests; i += 32)
-      here += __popc(__ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows));
-  } else {
-    here = p.requests;
-  }
-  if (here == 0 || round / here >= blocks) return;
-  const uint32_t from_last = round / here;
-  int r = static_cast<int>(round - from_last * here);
-  int q_asked, kv_have;
-  int64_t tok0;
-  if (p.requests <= 32) {
-    r = nth_bit(mask, r, lane);
-    q_asked = __shfl_sync(~0u, my_len, r);
-    kv_have = __shfl_sync(~0u, my_kv, r);
-    tok0 = __shfl_sync(~0u, my_start, r);
-  } else {
-    if (p.requests <= kScan) {
-      int nth = r;
-      for (int i = 0; i < p.requests; i += 32) {
-        const uint32_t m =
-            __ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows);
-        if (nth < __popc(m)) {
-          r = i + nth_bit(m, nth, lane);
-          break;
-        }
-        nth -= __popc(m);
-      }
-    }
-    q_asked = p.q_lens[r];
-    kv_have = p.kv_lens[r];
-    tok0 = p.q_start[r];
-  }
-  q_asked = max(q_asked, 0);
-  const int q_len = min(q_asked, p.max_q);
-  const int rows_all = q_len * G;  // max_q * G fits
-  const int row0 = static_cast<int>(blocks - 1 - from_last) * 2 * kTile;
-  if (rows_all <= min_rows || row0 >= rows_all) return;
-  const int rows = min(2 * kTile, rows_all - row0);
-  const int kv_len = min(max(kv_have, 0), p.table_width * bs);
-  const int64_t behind = static_cast<int64_t>(kv_len) - q_asked + 1;  // token i sees behind + i keys
-  const int keys = static_cast<int>(max(static_cast<int64_t>(0), behind + (row0 + rows - 1) / G));
-  const int nt = (keys + kTile - 1) / kTile, nu = (keys + kKeys - 1) / kKeys;
+  Item it;
+  if (!item_of(p, SHARES ? blockIdx.x / shares : blockIdx.x, blocks, min_rows, lane, it)) return;
+  const int head = it.head, r = it.r, row0 = it.row0, rows = it.rows, keys = it.keys;
+  const int64_t behind = it.behind, tok0 = it.tok0;
+  // this CTA's share of the key tiles: nt tiles from key_first on, nu steps
+  const int share = SHARES ? static_cast<int>(blockIdx.x % shares) : 0, tiles_all = (keys + kTile - 1) / kTile;
+  const int t_first = SHARES ? static_cast<int>(static_cast<int64_t>(tiles_all) * share / shares) : 0;
+  const int nt = SHARES ? static_cast<int>(static_cast<int64_t>(tiles_all) * (share + 1) / shares) - t_first : tiles_all;
+  const int key_first = t_first * kTile;
+  const int nu = ((SHARES ? min(keys - key_first, nt * kTile) : keys) + kKeys - 1) / kKeys;
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tk);
@@ -392,46 +411,52 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp % kSoftmaxWarps) * 32) << 16);
     const uint32_t t_o = t_lane + 256 + q * D;
     const bool active = q * kTile < rows;
+    // Rows of q come, and those of the output go, through the tile of q in shared memory: piece i of a warp's 32 rows
+    // is kAtOnce rows, one 16-byte chunk per lane.
+    constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+    const int chunk = lane % kLanes;
+    auto stage = [&](int r, int c) {
+      return smem + L::kQ + q * L::kOp + (c / 8) * kSubTile + r * 128 + (((c % 8) ^ (r & 7)) << 4);
+    };
+    auto staged = [&](int i) { return stage((warp % kSoftmaxWarps) * 32 + i * kAtOnce + lane / kLanes, chunk); };
     float mul = 1.f;
     if (active && nt > 0) {
-      const T* x = static_cast<const T*>(p.q) + (there ? at * p.ld_q + (head * G + h) * D : 0);
-      uint32_t w[D / 2];
-      if (there) {
-        if (wide) {
+      // whole rows by neighbouring lanes, all loads before the first use
+      const int64_t from = there ? at * p.ld_q + (head * G + h) * D : -1;
+      uint4 w[kLanes];
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i) ldg256(x + 16 * i, w + 8 * i);
-        } else {
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(w + 4 * i) = *reinterpret_cast<const uint4*>(x + 8 * i);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) w[i] = 0;
+      for (int i = 0; i < kLanes; ++i) {
+        const int64_t f = __shfl_sync(~0u, from, i * kAtOnce + lane / kLanes);
+        w[i] = f >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + f + chunk * 8) : make_uint4(0, 0, 0, 0);
       }
-      if constexpr (!std::is_same<T, __half>::value) {
-        uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) top = max(top, max(w[i] & 0x7fffu, w[i] >> 16 & 0x7fffu));
-        mul = row_power(top << 16);
+      for (int i = 0; i < kLanes; ++i) {
+        if constexpr (!std::is_same<T, __half>::value) {
+          uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w}, top = 0;
 #pragma unroll
-        for (int i = 0; i < D / 2; ++i) {
-          float a, b;
-          unpack2(w[i], a, b, T());
-          w[i] = pack2(a * mul, b * mul, __half());
+          for (int e = 0; e < 4; ++e) top = max(top, max(x[e] & 0x7fffu, x[e] >> 16 & 0x7fffu));
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(~0u, top, o));
+          const float k = row_power(top << 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a, b;
+            unpack2(x[e], a, b, T());
+            x[e] = pack2(a * k, b * k, __half());
+          }
+          w[i] = make_uint4(x[0], x[1], x[2], x[3]);
+          const float mine = __shfl_sync(~0u, k, lane % kAtOnce * kLanes);
+          if (lane / kAtOnce == i) mul = mine;
         }
+        *reinterpret_cast<uint4*>(staged(i)) = w[i];
       }
-      uint8_t* dst = smem + L::kQ + q * L::kOp + row * 128;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        *reinterpret_cast<uint4*>(dst + (i / 8) * kSubTile + (((i % 8) ^ (row & 7)) << 4)) =
-            make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full(q));
     }
     const float rmul = p.scale * 1.4426950408889634f / mul;
     // the first step in which some row of this warp does not see every key
-    const int first_masked = __reduce_min_sync(~0u, lim) / kKeys;
+    const int first_masked = (__reduce_min_sync(~0u, lim) - key_first) / kKeys;
     float m = -INFINITY;
     uint64_t sum[2] = {0, 0};  // four partial sums
     bool ok = true;
@@ -456,7 +481,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       const uint32_t present = in.there >> first_group & ((1u << kStepGroups) - 1);
       const float down = (u & 1) == 0 ? in.down : 1.f;
       const bool edge = u >= first_masked || present != (1u << kStepGroups) - 1;
-      const int key0 = u * kKeys;
+      const int key0 = key_first + u * kKeys;
 #pragma unroll
       for (int cc = 0; cc < kKeys / 32; ++cc) tmem_ld_wait32(s + cc * 32);
       float mx = -INFINITY;
@@ -513,10 +538,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     // ---- epilogue
     if (active) {
       T* dst = static_cast<T*>(p.out) + (there ? at * p.ld_out + (head * G + h) * D : 0);
+      const int64_t slot = there ? share * ws.rows + at * p.q_heads + head * G + h : 0;
       if (nt == 0) {
-        if (there)
+        if (SHARES && there) {
+          ws.ml[slot] = make_float2(-INFINITY, 0.f);
+        } else if (there) {
 #pragma unroll
           for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
+        }
       } else {
         if (ok) ok = wait(pv_done(q, nu - 1), ((nu - 1) >> 1) & 1, 53);
         ok = __all_sync(~0u, ok);
@@ -526,28 +555,47 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           unpair(add2(sum[0], sum[1]), a, b);
           const float l = a + b;
           const float k = l == 0.f ? 0.f : info[(nt - 1) % kInfo].ref / l;
+          if (SHARES && there) ws.ml[slot] = make_float2(m, l);
+          // the scores of all steps are done with q: its tile takes the output, f32 in two halves
+          const int64_t to = !there ? -1 : SHARES ? slot * D : at * p.ld_out + (head * G + h) * D;
 #pragma unroll
-          for (int cc = 0; cc < D / 32; ++cc) {
-            uint32_t o[32];
-            tmem_ld_x32(t_o + cc * 32, o);
-            tmem_ld_wait32(o);
-            if (there) {
+          for (int half = 0; half < (SHARES ? 2 : 1); ++half) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 16) {
-                uint32_t w[8];
+            for (int sub = 0; sub < D / 64; ++sub) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float x = __uint_as_float(o[e + 2 * j]) * k, y = __uint_as_float(o[e + 2 * j + 1]) * k;
-                  w[j] = l == 0.f ? 0u : pack2(x, y, T());
-                }
-                if (wide) {
-                  stg256(dst + cc * 32 + e, w);
+              for (int e = 0; e < (SHARES ? 1 : 2); ++e) {
+                const int cc = SHARES ? half * (D / 64) + sub : sub * 2 + e;
+                uint32_t o[32];
+                tmem_ld_x32(t_o + cc * 32, o);
+                tmem_ld_wait32(o);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * k);
+                if constexpr (SHARES) {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<uint4*>(stage(row, sub * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                 } else {
-                  *reinterpret_cast<uint4*>(dst + cc * 32 + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                  *reinterpret_cast<uint4*>(dst + cc * 32 + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                  uint32_t w[16];
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    w[j] = pack2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]), T());
+#pragma unroll
+                  for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<uint4*>(stage(row, cc * 4 + j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 }
               }
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kLanes; ++i) {
+              const int64_t f = __shfl_sync(~0u, to, i * kAtOnce + lane / kLanes);
+              const uint4 x = *reinterpret_cast<const uint4*>(staged(i));
+              if (f >= 0) {
+                if constexpr (SHARES) *reinterpret_cast<uint4*>(ws.o + f + half * (D / 2) + chunk * 4) = x;
+                else *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + f + chunk * 8) = x;
+              }
+            }
+            __syncwarp();
           }
         }
       }
@@ -605,7 +653,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     float ref = kRef0;
     bool ok = true;
     auto block_of = [&](int t) {  // -1: no such block, or no key of the group is seen
-      const int key = t * kTile + lane * 16;
+      const int key = key_first + t * kTile + lane * 16;
       int id = -1;
       if (t < nt && lane < kGroups && key < keys) {
         const int b = p.table[static_cast<int64_t>(r) * p.table_width + key / bs];
@@ -741,11 +789,78 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   }
 }
 
+// Joins the shares of the rows of item blockIdx.x: a warp per row, a lane per share for the weights.
+constexpr int kJoinThreads = 256, kMostShares = 32;
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+prefill_join_kernel(const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, int shares, ShareWs ws) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int lane = threadIdx.x & 31, i = (blockIdx.y * kJoinThreads + threadIdx.x) / 32;
+  Item it;
+  if (!item_of(p, blockIdx.x, blocks, min_rows, lane, it) || i >= it.rows) return;
+  const int G = p.q_heads / p.cache.kv_heads;
+  const int64_t at = it.tok0 + (it.row0 + i) / G;
+  if (at < 0 || at >= p.tokens) return;
+  const int col = it.head * G + (it.row0 + i) % G;
+  const int64_t row = at * p.q_heads + col;
+  const float2 ml = lane < shares ? ws.ml[lane * ws.rows + row] : make_float2(-INFINITY, 0.f);
+  float top = ml.x;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+  // a share that saw no key has a sum of 0, and its output may not even be written
+  float w = ml.y == 0.f ? 0.f : ml.y * exp2_approx(ml.x - top), sum = w;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  w = sum == 0.f ? 0.f : w / sum;
+  constexpr int E = D / 32;
+  float acc[E] = {};
+#pragma unroll 8
+  for (int k = 0; k < shares; ++k) {
+    const float wk = __shfl_sync(~0u, w, k);
+    const float* v = ws.o + (k * ws.rows + row) * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 x = wk != 0.f ? *reinterpret_cast<const float2*>(v + e) : make_float2(0.f, 0.f);
+      acc[e] += x.x * wk;
+      acc[e + 1] += x.y * wk;
+    }
+  }
+  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at * p.ld_out + col * D + lane * E);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) out[e / 2] = pack2(acc[e], acc[e + 1], T());
+}
+
+// Shares that the keys of an item are cut into, so that few rows over long caches fill the GPU: as many as make one to
+// three full rounds of CTAs, where the rounds (as measured 2.1 us per key tile and 8 per CTA) and the join (5 us, and
+// its bytes at 6 TB/s) come to a tenth less than they do without shares.  The host has bounds only: the rows of the
+// batch, and the longest cache.  (8 kv heads of 128 with 4 query heads each, one request: 64 tokens over 8 000
+// 139 -> 33 us, 100 over 30 000 492 -> 82 us, 512 over 8 192 146 -> 94 us.)
+int shares_for(const Kv8AttentionParams& p) {
+  const int64_t rows = p.tokens * (p.q_heads / p.cache.kv_heads);
+  const int64_t items = (rows + 2 * kTile - 1) / (2 * kTile) * p.cache.kv_heads, sms = device_sm_count();
+  const double tiles = static_cast<double>((p.max_kv + kTile - 1) / kTile);
+  double best = 0.9 * static_cast<double>((items + sms - 1) / sms) * (tiles * 2.1 + 8);
+  int shares = 1;
+  for (int64_t round = 1; round <= 3; ++round) {
+    const int64_t n = std::min<int64_t>(std::min<int64_t>(round * sms / items, kMostShares), static_cast<int64_t>(tiles) / 4);
+    if (n < 2) continue;
+    const double t = static_cast<double>((items * n + sms - 1) / sms) * (tiles / n * 2.1 + 8) + 5 +
+                     static_cast<double>(rows * p.cache.kv_heads * n) * p.cache.dim * 8 / 6e6;
+    if (t < best) {
+      best = t;
+      shares = static_cast<int>(n);
+    }
+  }
+  return shares;
+}
+
 template <typename T, int D>
 cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
   const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
-  const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile);
-  if (rows > INT32_MAX - 2 * kTile || blocks * p.cache.kv_heads * p.requests > INT32_MAX) {
+  const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile), items = blocks * p.cache.kv_heads * p.requests;
+  const int shares = shares_for(p);
+  if (rows > INT32_MAX - 2 * kTile || items > INT32_MAX / 32) {
     *err = "too many query rows";
     return cudaErrorInvalidValue;
   }
@@ -755,19 +870,30 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
     *err = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = prefill_kernel<T, D>;
+  auto kern = shares > 1 ? prefill_kernel<T, D, true> : prefill_kernel<T, D, false>;
   constexpr int smem = Smem<D>::kDynamic;
-  static std::atomic<uint64_t> ready{0};
-  cudaError_t st = allow_smem(kern, smem, ready);
+  static std::atomic<uint64_t> ready[2] = {{0}, {0}};
+  cudaError_t st = allow_smem(kern, smem, ready[shares > 1]);
   if (st != cudaSuccess) return st;
-  const dim3 grid(static_cast<unsigned>(blocks * p.cache.kv_heads * p.requests));
-  // rows of q and out on 32-byte boundaries take whole sectors per lane
-  const int wide = ((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0 &&
-                   p.ld_q % 16 == 0 && p.ld_out % 16 == 0;
-  return launch_dependent(kern, grid, dim3(kThreads), smem, stream, tk, tv, p, min_rows, static_cast<uint32_t>(blocks), box, wide);
+  ShareWs ws = {};
+  if (shares > 1) {
+    ws.rows = p.tokens * p.q_heads;
+    ws.o = static_cast<float*>(p.workspace);
+    ws.ml = reinterpret_cast<float2*>(ws.o + shares * ws.rows * D);
+  }
+  st = launch_dependent(kern, dim3(static_cast<unsigned>(items * shares)), dim3(kThreads), smem, stream, tk, tv, p,
+                        min_rows, static_cast<uint32_t>(blocks), static_cast<uint32_t>(shares), ws, box);
+  if (st != cudaSuccess || shares == 1) return st;
+  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(items), 2 * kTile * 32 / kJoinThreads),
+                          dim3(kJoinThreads), 0, stream, p, min_rows, static_cast<uint32_t>(blocks), shares, ws);
 }
 
 }  // namespace
+
+int64_t kv8_prefill_workspace_bytes(const Kv8AttentionParams& p) {
+  const int shares = shares_for(p);
+  return shares > 1 ? shares * p.tokens * p.q_heads * (static_cast<int64_t>(p.cache.dim) * 4 + 8) : 0;
+}
 
 cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
   if (p.cache.dim == 128)

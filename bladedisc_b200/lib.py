@@ -183,7 +183,7 @@ SIGNATURES = {
     "disc_b200_kv_blocks_trim": (c_int32, [POINTER(KvBlocksArgs), c_void_p]),
     "disc_b200_kv8_append": (c_int32, [POINTER(Kv8AppendArgs), c_void_p]),
     "disc_b200_kv8_read": (c_int32, [POINTER(Kv8ReadArgs), c_void_p]),
-    "disc_b200_kv8_attention_workspace_bytes": (c_int64, [c_int32, c_int64]),
+    "disc_b200_kv8_attention_workspace_bytes": (c_int64, [POINTER(Kv8AttentionArgs)]),
     "disc_b200_kv8_attention": (c_int32, [POINTER(Kv8AttentionArgs), c_void_p]),
     "disc_b200_nccl_available": (c_int32, []),
     "disc_b200_nccl_unique_id": (c_int32, [c_void_p]),

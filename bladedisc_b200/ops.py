@@ -739,20 +739,6 @@ def kv8_read(k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: t
     return ko, vo
 
 
-_kv8_workspace = {}
-
-
-def _kv8_workspace_bytes(dev: int, dim: int, max_kv: int) -> int:
-    """Bytes of workspace; they depend on the device and the head size, and on max_kv only by a threshold."""
-    if max_kv <= _lib.KV8_DIRECT_KEYS:
-        return 0
-    key = (dev, dim)
-    if key not in _kv8_workspace:
-        with torch.cuda.device(dev):
-            _kv8_workspace[key] = _lib.load().disc_b200_kv8_attention_workspace_bytes(dim, max_kv)
-    return _kv8_workspace[key]
-
-
 def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                   table: torch.Tensor, q_start: torch.Tensor, q_lens: torch.Tensor, kv_lens: torch.Tensor, *,
                   max_q: int, scale: Optional[float] = None, max_kv: Optional[int] = None,
@@ -800,11 +786,17 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
                               heads * dim, heads, kind, cache, table.data_ptr(), q_start.data_ptr(),
                               q_lens.data_ptr(), kv_lens.data_ptr(), n, width, max_q, max_kv,
                               dim ** -0.5 if scale is None else scale)
-    need = _kv8_workspace_bytes(dev, dim, max_kv)
-    if need:  # from torch's allocator: ordered with this stream, a captured graph keeps its own
-        work = k.new_empty(need)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-    _call(dev, _lib.load().disc_b200_kv8_attention, a)
+    lib = _lib.load()
+    if max_kv > _lib.KV8_DIRECT_KEYS:
+        if torch._C._cuda_getDevice() == dev:
+            need = lib.disc_b200_kv8_attention_workspace_bytes(a)
+        else:
+            with torch.cuda.device(dev):
+                need = lib.disc_b200_kv8_attention_workspace_bytes(a)
+        if need:  # from torch's allocator: ordered with this stream, a captured graph keeps its own
+            work = k.new_empty(need)
+            a.workspace, a.workspace_bytes = work.data_ptr(), need
+    _call(dev, lib.disc_b200_kv8_attention, a)
     return out
 
 

@@ -579,9 +579,10 @@ typedef struct disc_b200_kv8_attention_args {
 } disc_b200_kv8_attention_args;
 /* Caches up to this many keys need no workspace. */
 enum { DISC_B200_KV8_DIRECT_KEYS = 512 };
-/* Workspace of a call with this head size and max_kv on the current device (the same for every batch; 0 for short
- * caches).  Calls that overlap on the GPU need one each; its contents mean nothing between calls. */
-int64_t disc_b200_kv8_attention_workspace_bytes(int32_t dim, int64_t max_kv);
+/* Workspace of a call with these arguments on the current device: from the sizes (tokens, heads, requests, max_q,
+ * max_kv, the cache's), no pointer is looked at; -1 for NULL.  Calls that overlap on the GPU need one each; its contents
+ * mean nothing between calls. */
+int64_t disc_b200_kv8_attention_workspace_bytes(const disc_b200_kv8_attention_args* args);
 int32_t disc_b200_kv8_attention(const disc_b200_kv8_attention_args* args, void* stream);
 
 /* ---- Collectives of the column-parallel (N-split) configuration.

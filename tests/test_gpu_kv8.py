@@ -264,6 +264,8 @@ SHAPES = [
     ([16, 9], [16, 640], 16, 2, 16, 128), ([24], [1000], 64, 5, 5, 64),
     ([128], [128], 16, 1, 1, 128), ([129, 1], [129, 1], 64, 2, 2, 64), ([300, 257], [300, 1000], 32, 2, 4, 128),
     ([1, 500, 1, 77, 1], [600, 500, 33, 200, 1025], 16, 2, 6, 128), ([640], [1500], 128, 1, 7, 64),
+    # many rows over long caches: the keys in shares
+    ([150], [6000], 16, 1, 2, 64), ([70, 1, 300], [4000, 9, 2500], 32, 2, 4, 128), ([200], [5003], 64, 1, 1, 128),
     ([255], [511], 16, 1, 3, 64), ([65, 190], [129, 190], 16, 2, 10, 128), ([1030], [1030], 64, 1, 2, 128),
 ]
 
@@ -435,6 +437,15 @@ def test_offsets_past_32_bits(ops):
     a, b = ops.kv8_read(k, v, ks, vs, dev(ids), torch.float16)
     assert torch.equal(a, (k[at].float() * ks[at][..., None, None]).half())
     assert torch.equal(b, (v[at].float() * vs[at][..., None, None]).half())
+
+
+def test_shares_without_keys(ops):
+    """A bound on the lengths that promises a long cache, requests that are short or empty: shares of nothing."""
+    rng = np.random.default_rng(18)
+    got, want, slack, (q, d, args, mq) = _attend(ops, rng, [100, 80, 90], [130, 3, 90], 16, 1, 2, 64, torch.float16,
+                                                 width=2000, gap=2)
+    _check(got, want, slack)
+    assert (got[100:102] == 3).all() and not got[102:179].any()
 
 
 @pytest.mark.parametrize("captured", [False, True])

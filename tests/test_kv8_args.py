@@ -132,10 +132,15 @@ def test_attention(lib):
     _refused(lib, fn, args(out=0x1008), "16-byte")
     _refused(lib, fn, args(scale=0.0), "positive")
     # a long cache wants its workspace, whole and aligned; a short one none
-    need = lib.disc_b200_kv8_attention_workspace_bytes(64, 513)
-    assert need > 0 and lib.disc_b200_kv8_attention_workspace_bytes(64, L.KV8_DIRECT_KEYS) == 0
+    need_of = lambda **kw: lib.disc_b200_kv8_attention_workspace_bytes(ctypes.byref(args(**kw)))  # noqa: E731
+    need = need_of(max_kv=513)
+    assert need > 0 and need_of(max_kv=L.KV8_DIRECT_KEYS) == 0 and lib.disc_b200_kv8_attention_workspace_bytes(None) == -1
     for kw in (dict(), dict(workspace=0x1000, workspace_bytes=need - 1), dict(workspace=0x1008, workspace_bytes=need)):
         _refused(lib, fn, args(max_kv=513, **kw), "workspace")
+    # many rows of one request over a long cache: their keys are cut into shares
+    big = dict(tokens=300, max_q=300, max_kv=100000, requests=1)
+    assert need_of(**big) >= 2 * 300 * 4 * (64 * 4 + 8) and need_of(**{**big, "max_kv": 600}) == 0
+    _refused(lib, fn, args(workspace=0x1000, workspace_bytes=need_of(**big) - 1, **big), "workspace")
     a = args()
     a.cache.num_blocks = 0
     _refused(lib, fn, a, "without blocks")
