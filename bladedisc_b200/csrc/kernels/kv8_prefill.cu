@@ -17,7 +17,7 @@
 // What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all): shared memory 3070 cycles (levels in
 // and out 512, operands out 512, Q and K into S 1536 at 64 keys a product, V into O 512), exp2 2048 at 16 a cycle less
 // the quarter that goes to the FMA pipe, products 2560.  Measured at 4095 tokens behind 12289, 32 over 8 heads: 0.98 ms
-// = 980 TFLOP/s, 0.59 of the measured bf16 rate; one of eight CTA rounds is not full.  What was measured on the way there:
+// (1.04 on the slowest card seen) = 980 TFLOP/s, 0.59 of the measured bf16 rate; one of eight CTA rounds is not full.  What was measured on the way there:
 // scores of 128 keys in one buffer 1.07 ms (the chain softmax, P V, S is exposed), one issuer for both tiles 1.44,
 // products issued behind `lane == 0` 1.20, levels to registers instead of TMA 1.40, exp2 all on the MUFU 1.01, half of
 // them on the FMA pipe 1.08, taking turns in exp2 1.02.  Short prompts pay for the start of a CTA (8300 cycles to the
@@ -238,9 +238,15 @@ __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs,
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-constexpr int kScan = 1024;  // requests among which a CTA looks for those that this kernel serves
 __device__ __forceinline__ int rows_of(const Kv8AttentionParams& p, int q_len) {
   return min(max(q_len, 0), p.max_q) * (p.q_heads / p.cache.kv_heads);  // max_q * group fits
+}
+// Blocks of 256 rows that a request has here: none if its rows are few, none for rows behind the batch.
+__device__ __forceinline__ int blocks_of(const Kv8AttentionParams& p, int q_len, int start, int min_rows) {
+  if (rows_of(p, q_len) <= min_rows) return 0;
+  const int64_t left = p.tokens - start;
+  const int rows = rows_of(p, left < q_len ? static_cast<int>(max(left, static_cast<int64_t>(0))) : q_len);
+  return (rows + 2 * kTile - 1) / (2 * kTile);
 }
 
 // Position of the n-th set bit (from 0), found by a converged warp.
@@ -256,60 +262,94 @@ struct Item {
   int64_t tok0;    // row of q of the request's first token
   int64_t behind;  // token i sees behind + i keys
 };
-// Heads vary fastest, then requests; the rows with the most keys come first.  (Requests that are not for this kernel
-// come last of all, so that their CTAs, which end at once, hold up nobody.)  A converged warp; false: nothing.
+// Heads vary fastest, then requests; of a request its last rows, with the most keys, come first: item by item through
+// the list of (block from high to low, request that has it).  The host knows the rows of the batch only, which bound
+// the list; a grid of requests x longest instead starts CTAs for nothing (64 single tokens and a prompt of 500 over
+// 4 000 keys, 32 over 8 heads: 500 -> 180 us).  A converged warp; false: the list is shorter.
 __device__ __forceinline__ bool item_of(const Kv8AttentionParams& p, uint32_t index, uint32_t blocks, int min_rows,
                                         int lane, Item& it) {
-  const uint32_t KH = p.cache.kv_heads, round = index / KH;
-  it.head = static_cast<int>(index - round * KH);
+  const uint32_t KH = p.cache.kv_heads;
+  int nth = static_cast<int>(index / KH);
+  it.head = static_cast<int>(index % KH);
   // up to 32 requests: a lane per request has all that is needed of it, one load latency in all
-  int my_len = 0, my_kv = 0, my_start = 0;
-  if (lane < p.requests) {
+  int my_len = 0, my_kv = 0, my_start = 0, my_blocks = 0;
+  if (p.requests <= 32 && lane < p.requests) {
     my_len = p.q_lens[lane];
     my_kv = p.kv_lens[lane];
     my_start = p.q_start[lane];
+    my_blocks = blocks_of(p, my_len, my_start, min_rows);
   }
-  uint32_t here = 0, mask = 0;
+  int block = -1, r = 0, q_asked, kv_have;
   if (p.requests <= 32) {
-    mask = __ballot_sync(~0u, lane < p.requests && rows_of(p, my_len) > min_rows);
-    here = __popc(mask);
-  } else if (p.requests <= kScan) {
-    for (int i = 0; i < p.requests; i += 32)
-      here += __popc(__ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows));
-  } else {
-    here = p.requests;
-  }
-  if (here == 0 || round / here >= blocks) return false;
-  const uint32_t from_last = round / here;
-  int r = static_cast<int>(round - from_last * here);
-  int q_asked, kv_have;
-  if (p.requests <= 32) {
-    r = nth_bit(mask, r, lane);
+    // runs of blocks that the same requests have
+    int b = static_cast<int>(__reduce_max_sync(~0u, static_cast<uint32_t>(my_blocks))) - 1;
+    while (b >= 0) {
+      const uint32_t m = __ballot_sync(~0u, my_blocks > b);
+      const int low = static_cast<int>(__reduce_max_sync(~0u, my_blocks > b ? 0u : static_cast<uint32_t>(my_blocks)));
+      const int c = __popc(m), n = (b - low + 1) * c;
+      if (nth < n) {
+        const int down = nth / c;
+        block = b - down;
+        r = nth_bit(m, nth - down * c, lane);
+        break;
+      }
+      nth -= n;
+      b = low - 1;
+    }
+    if (block < 0) return false;
     q_asked = __shfl_sync(~0u, my_len, r);
     kv_have = __shfl_sync(~0u, my_kv, r);
     it.tok0 = __shfl_sync(~0u, my_start, r);
   } else {
-    if (p.requests <= kScan) {
-      int nth = r;
+    auto blocks_at = [&](int i) {  // of request i + lane
+      return i + lane < p.requests ? blocks_of(p, p.q_lens[i + lane], p.q_start[i + lane], min_rows) : 0;
+    };
+    // 32 blocks at a time, one per lane: how many requests have it
+    for (int top = static_cast<int>(blocks) - 1; top >= 0 && block < 0; top -= 32) {
+      const int levels = min(top, 31) + 1;
+      int have = 0;
+#pragma unroll 1
       for (int i = 0; i < p.requests; i += 32) {
-        const uint32_t m =
-            __ballot_sync(~0u, i + lane < p.requests && rows_of(p, p.q_lens[min(i + lane, p.requests - 1)]) > min_rows);
-        if (nth < __popc(m)) {
-          r = i + nth_bit(m, nth, lane);
-          break;
+        const int n = blocks_at(i);
+        uint32_t m = __ballot_sync(~0u, n > top + 1 - levels);
+        if (__popc(m) > levels) {
+          for (int k = 0; k < levels; ++k) {
+            const int c = __popc(__ballot_sync(~0u, n > top - k));
+            if (lane == k) have += c;
+          }
+        } else {
+          for (; m != 0; m &= m - 1) have += __shfl_sync(~0u, n, __ffs(m) - 1) > top - lane;
         }
-        nth -= __popc(m);
       }
+      if (lane >= levels) have = 0;
+      int upto = have;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(~0u, upto, o);
+        if (lane >= o) upto += u;
+      }
+      const uint32_t behind = __ballot_sync(~0u, upto > nth);
+      const int at = behind != 0 ? __ffs(behind) - 1 : 31;
+      if (behind != 0) block = top - at;
+      nth -= __shfl_sync(~0u, behind != 0 ? upto - have : upto, at);
+    }
+    if (block < 0) return false;
+#pragma unroll 1
+    for (int i = 0; i < p.requests; i += 32) {
+      const uint32_t m = __ballot_sync(~0u, blocks_at(i) > block);
+      if (nth < __popc(m)) {
+        r = i + nth_bit(m, nth, lane);
+        break;
+      }
+      nth -= __popc(m);
     }
     q_asked = p.q_lens[r];
     kv_have = p.kv_lens[r];
     it.tok0 = p.q_start[r];
   }
   it.r = r;
-  const int rows_all = rows_of(p, q_asked);
-  it.row0 = static_cast<int>(blocks - 1 - from_last) * 2 * kTile;
-  if (rows_all <= min_rows || it.row0 >= rows_all) return false;
-  it.rows = min(2 * kTile, rows_all - it.row0);
+  it.row0 = block * 2 * kTile;
+  it.rows = min(2 * kTile, rows_of(p, q_asked) - it.row0);
   const int kv_len = min(max(kv_have, 0), p.table_width * p.cache.block_size);
   it.behind = static_cast<int64_t>(kv_len) - max(q_asked, 0) + 1;
   const int G = p.q_heads / p.cache.kv_heads;
@@ -796,39 +836,40 @@ __global__ void __launch_bounds__(kJoinThreads)
 prefill_join_kernel(const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, int shares, ShareWs ws) {
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, i = (blockIdx.y * kJoinThreads + threadIdx.x) / 32;
+  const int lane = threadIdx.x & 31, G = p.q_heads / p.cache.kv_heads;
   Item it;
-  if (!item_of(p, blockIdx.x, blocks, min_rows, lane, it) || i >= it.rows) return;
-  const int G = p.q_heads / p.cache.kv_heads;
-  const int64_t at = it.tok0 + (it.row0 + i) / G;
-  if (at < 0 || at >= p.tokens) return;
-  const int col = it.head * G + (it.row0 + i) % G;
-  const int64_t row = at * p.q_heads + col;
-  const float2 ml = lane < shares ? ws.ml[lane * ws.rows + row] : make_float2(-INFINITY, 0.f);
-  float top = ml.x;
+  if (!item_of(p, blockIdx.x, blocks, min_rows, lane, it)) return;
+  for (int i = (blockIdx.y * kJoinThreads + threadIdx.x) / 32; i < it.rows; i += gridDim.y * (kJoinThreads / 32)) {
+    const int64_t at = it.tok0 + (it.row0 + i) / G;
+    if (at < 0 || at >= p.tokens) continue;
+    const int col = it.head * G + (it.row0 + i) % G;
+    const int64_t row = at * p.q_heads + col;
+    const float2 ml = lane < shares ? ws.ml[lane * ws.rows + row] : make_float2(-INFINITY, 0.f);
+    float top = ml.x;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-  // a share that saw no key has a sum of 0, and its output may not even be written
-  float w = ml.y == 0.f ? 0.f : ml.y * exp2_approx(ml.x - top), sum = w;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    // a share that saw no key has a sum of 0, and its output may not even be written
+    float w = ml.y == 0.f ? 0.f : ml.y * exp2_approx(ml.x - top), sum = w;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  w = sum == 0.f ? 0.f : w / sum;
-  constexpr int E = D / 32;
-  float acc[E] = {};
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    w = sum == 0.f ? 0.f : w / sum;
+    constexpr int E = D / 32;
+    float acc[E] = {};
 #pragma unroll 8
-  for (int k = 0; k < shares; ++k) {
-    const float wk = __shfl_sync(~0u, w, k);
-    const float* v = ws.o + (k * ws.rows + row) * D + lane * E;
+    for (int k = 0; k < shares; ++k) {
+      const float wk = __shfl_sync(~0u, w, k);
+      const float* v = ws.o + (k * ws.rows + row) * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 x = wk != 0.f ? *reinterpret_cast<const float2*>(v + e) : make_float2(0.f, 0.f);
-      acc[e] += x.x * wk;
-      acc[e + 1] += x.y * wk;
+      for (int e = 0; e < E; e += 2) {
+        const float2 x = wk != 0.f ? *reinterpret_cast<const float2*>(v + e) : make_float2(0.f, 0.f);
+        acc[e] += x.x * wk;
+        acc[e + 1] += x.y * wk;
+      }
     }
-  }
-  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at * p.ld_out + col * D + lane * E);
+    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at * p.ld_out + col * D + lane * E);
 #pragma unroll
-  for (int e = 0; e < E; e += 2) out[e / 2] = pack2(acc[e], acc[e + 1], T());
+    for (int e = 0; e < E; e += 2) out[e / 2] = pack2(acc[e], acc[e + 1], T());
+  }
 }
 
 // Shares that the keys of an item are cut into, so that few rows over long caches fill the GPU: as many as make one to
@@ -858,9 +899,12 @@ int shares_for(const Kv8AttentionParams& p) {
 template <typename T, int D>
 cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
   const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
-  const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile), items = blocks * p.cache.kv_heads * p.requests;
+  const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile);
+  // no more blocks than the rows of the batch make, and one more for the rest of each request
+  const int64_t most = p.tokens * (p.q_heads / p.cache.kv_heads) / (2 * kTile) + std::min<int64_t>(p.requests, p.tokens);
+  const int64_t items = std::min(blocks * p.requests, most) * p.cache.kv_heads;
   const int shares = shares_for(p);
-  if (rows > INT32_MAX - 2 * kTile || items > INT32_MAX / 32) {
+  if (rows > INT32_MAX - 2 * kTile || items > INT32_MAX / kMostShares) {
     *err = "too many query rows";
     return cudaErrorInvalidValue;
   }
@@ -884,7 +928,9 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
   st = launch_dependent(kern, dim3(static_cast<unsigned>(items * shares)), dim3(kThreads), smem, stream, tk, tv, p,
                         min_rows, static_cast<uint32_t>(blocks), static_cast<uint32_t>(shares), ws, box);
   if (st != cudaSuccess || shares == 1) return st;
-  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(items), 2 * kTile * 32 / kJoinThreads),
+  // two rounds of CTAs, a row per warp at least
+  const int slices = static_cast<int>(std::clamp<int64_t>(16 * device_sm_count() / items, 1, 2 * kTile * 32 / kJoinThreads));
+  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(items), slices),
                           dim3(kJoinThreads), 0, stream, p, min_rows, static_cast<uint32_t>(blocks), shares, ws);
 }
 

@@ -746,7 +746,8 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     """Causal attention of ``q [tokens, q heads, head size]`` over one layer of the 8-bit cache.
 
     Request ``r`` has the rows ``q_start[r] ... q_start[r] + q_lens[r] - 1`` of ``q``, its last tokens; they see its
-    ``kv_lens[r]`` cached tokens (their own included: append first) up to their own position.  The index tensors
+    ``kv_lens[r]`` cached tokens (their own included: append first) up to their own position.  Requests may not share
+    rows; rows of a request behind the end of ``q`` are not there.  The index tensors
     are int32 and stay on the device; ``max_q`` bounds ``q_lens`` and shapes the launch (rows behind it are not
     computed), ``max_kv`` bounds ``kv_lens`` and only steers how the work is split (default: the table's width).
     Query heads are a multiple of the kv heads.  ``scale`` defaults to ``head size ** -0.5``.  Rows that belong to

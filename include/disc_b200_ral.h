@@ -557,9 +557,10 @@ int32_t disc_b200_kv8_read(const disc_b200_kv8_read_args* args, void* stream);
 /* Causal attention of q over the cache: token i of the q_lens[r] tokens of request r, row q_start[r] + i of q,
  * sees the keys 0 .. kv_lens[r] - q_lens[r] + i.  Query head h reads kv head h / (q_heads / kv_heads).  Scores,
  * softmax and sums are fp32.  A row without keys gives 0; keys whose table entry is not a block of the cache are
- * left out; rows that belong to no request are left as they were.  max_q and max_kv: bounds on q_lens and
+ * left out; rows that belong to no request are left as they were, rows of a request behind `tokens` are not there.
+ * Requests may not share rows of q (some would not be computed).  max_q and max_kv: bounds on q_lens and
  * kv_lens known to the host (the launch is shaped by them: tokens of a request behind its first max_q are not
- * computed, keys behind max_kv do count).  One kernel serves any mix of single tokens and prompts. */
+ * computed, keys behind max_kv do count).  One call serves any mix of single tokens and prompts. */
 typedef struct disc_b200_kv8_attention_args {
   const void* q;   /* f16 / bf16, row stride ld_q */
   void* out;       /* same type, row stride ld_out; may not overlap q */

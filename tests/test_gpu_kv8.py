@@ -439,6 +439,20 @@ def test_offsets_past_32_bits(ops):
     assert torch.equal(b, (v[at].float() * vs[at][..., None, None]).half())
 
 
+@pytest.mark.parametrize("requests", [5, 33, 70])
+@pytest.mark.parametrize("kv", [200, 3000])
+def test_rows_behind_the_batch(ops, requests, kv):
+    """q ends before the rows of its requests do; prompts of many lengths among requests of a few rows."""
+    rng = np.random.default_rng(19)
+    q_lens = [300 if i == 2 else 90 if i % 7 == 4 else 10 * (i % 3) + 1 for i in range(requests)]
+    kv_lens = [max(q, kv - 13 * i) if i % 2 else q for i, q in enumerate(q_lens)]
+    got, want, slack, (q, d, args, mq) = _attend(ops, rng, q_lens, kv_lens, 32, 1, 2, 64, torch.float16, gap=1)
+    _check(got, want, slack)
+    for cut in (311, q.shape[0] - 3, 17):
+        part = ops.kv8_attention(q[:cut], *d, *args, max_q=mq, out=torch.full_like(got[:cut], 3.0))
+        _check(part, want[:cut], slack[:cut])
+
+
 def test_shares_without_keys(ops):
     """A bound on the lengths that promises a long cache, requests that are short or empty: shares of nothing."""
     rng = np.random.default_rng(18)
