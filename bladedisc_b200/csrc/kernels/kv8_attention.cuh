@@ -81,6 +81,8 @@ inline bool make_map(CUtensorMap* tm, const int8_t* base, const Kv8Cache& c, int
 
 // Many rows: requests with more than min_rows query rows per kv head (kv8_prefill.cu).
 int64_t kv8_prefill_workspace_bytes(const Kv8AttentionParams& p);
-cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err);
+cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, void* workspace, cudaStream_t stream,
+                               const char** err);
+cudaError_t kv8_prefill_join_launch(const Kv8AttentionParams& p, int min_rows, void* workspace, cudaStream_t stream);
 
 }  // namespace disc_b200

@@ -896,15 +896,31 @@ int shares_for(const Kv8AttentionParams& p) {
   return shares;
 }
 
-template <typename T, int D>
-cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
-  const int64_t rows = static_cast<int64_t>(p.max_q) * (p.q_heads / p.cache.kv_heads);
-  const int64_t blocks = (rows + 2 * kTile - 1) / (2 * kTile);
+struct Launch {
+  int64_t rows, blocks, items;
+  int shares;
+  ShareWs ws;
+};
+Launch launch_of(const Kv8AttentionParams& p, void* workspace) {
+  Launch l = {};
+  const int64_t G = p.q_heads / p.cache.kv_heads;
+  l.rows = p.max_q * G;
+  l.blocks = (l.rows + 2 * kTile - 1) / (2 * kTile);
   // no more blocks than the rows of the batch make, and one more for the rest of each request
-  const int64_t most = p.tokens * (p.q_heads / p.cache.kv_heads) / (2 * kTile) + std::min<int64_t>(p.requests, p.tokens);
-  const int64_t items = std::min(blocks * p.requests, most) * p.cache.kv_heads;
-  const int shares = shares_for(p);
-  if (rows > INT32_MAX - 2 * kTile || items > INT32_MAX / kMostShares) {
+  const int64_t most = p.tokens * G / (2 * kTile) + std::min<int64_t>(p.requests, p.tokens);
+  l.items = std::min(l.blocks * p.requests, most) * p.cache.kv_heads;
+  l.shares = shares_for(p);
+  if (l.shares > 1) {
+    l.ws.rows = p.tokens * p.q_heads;
+    l.ws.o = static_cast<float*>(workspace);
+    l.ws.ml = reinterpret_cast<float2*>(l.ws.o + l.shares * l.ws.rows * p.cache.dim);
+  }
+  return l;
+}
+
+template <typename T, int D>
+cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, const Launch& l, cudaStream_t stream, const char** err) {
+  if (l.rows > INT32_MAX - 2 * kTile || l.items > INT32_MAX / kMostShares) {
     *err = "too many query rows";
     return cudaErrorInvalidValue;
   }
@@ -914,24 +930,21 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, cudaStream_t str
     *err = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = shares > 1 ? prefill_kernel<T, D, true> : prefill_kernel<T, D, false>;
+  auto kern = l.shares > 1 ? prefill_kernel<T, D, true> : prefill_kernel<T, D, false>;
   constexpr int smem = Smem<D>::kDynamic;
   static std::atomic<uint64_t> ready[2] = {{0}, {0}};
-  cudaError_t st = allow_smem(kern, smem, ready[shares > 1]);
+  const cudaError_t st = allow_smem(kern, smem, ready[l.shares > 1]);
   if (st != cudaSuccess) return st;
-  ShareWs ws = {};
-  if (shares > 1) {
-    ws.rows = p.tokens * p.q_heads;
-    ws.o = static_cast<float*>(p.workspace);
-    ws.ml = reinterpret_cast<float2*>(ws.o + shares * ws.rows * D);
-  }
-  st = launch_dependent(kern, dim3(static_cast<unsigned>(items * shares)), dim3(kThreads), smem, stream, tk, tv, p,
-                        min_rows, static_cast<uint32_t>(blocks), static_cast<uint32_t>(shares), ws, box);
-  if (st != cudaSuccess || shares == 1) return st;
+  return launch_dependent(kern, dim3(static_cast<unsigned>(l.items * l.shares)), dim3(kThreads), smem, stream, tk, tv, p,
+                          min_rows, static_cast<uint32_t>(l.blocks), static_cast<uint32_t>(l.shares), l.ws, box);
+}
+
+template <typename T, int D>
+cudaError_t join_t(const Kv8AttentionParams& p, int min_rows, const Launch& l, cudaStream_t stream) {
   // two rounds of CTAs, a row per warp at least
-  const int slices = static_cast<int>(std::clamp<int64_t>(16 * device_sm_count() / items, 1, 2 * kTile * 32 / kJoinThreads));
-  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(items), slices),
-                          dim3(kJoinThreads), 0, stream, p, min_rows, static_cast<uint32_t>(blocks), shares, ws);
+  const int slices = static_cast<int>(std::clamp<int64_t>(16 * device_sm_count() / l.items, 1, 2 * kTile * 32 / kJoinThreads));
+  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(l.items), slices), dim3(kJoinThreads), 0,
+                          stream, p, min_rows, static_cast<uint32_t>(l.blocks), l.shares, l.ws);
 }
 
 }  // namespace
@@ -941,12 +954,24 @@ int64_t kv8_prefill_workspace_bytes(const Kv8AttentionParams& p) {
   return shares > 1 ? shares * p.tokens * p.q_heads * (static_cast<int64_t>(p.cache.dim) * 4 + 8) : 0;
 }
 
-cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, cudaStream_t stream, const char** err) {
+cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, void* workspace, cudaStream_t stream,
+                               const char** err) {
+  const Launch l = launch_of(p, workspace);
   if (p.cache.dim == 128)
-    return p.type == kKvF16 ? launch_t<__half, 128>(p, min_rows, stream, err)
-                            : launch_t<__nv_bfloat16, 128>(p, min_rows, stream, err);
-  return p.type == kKvF16 ? launch_t<__half, 64>(p, min_rows, stream, err)
-                          : launch_t<__nv_bfloat16, 64>(p, min_rows, stream, err);
+    return p.type == kKvF16 ? launch_t<__half, 128>(p, min_rows, l, stream, err)
+                            : launch_t<__nv_bfloat16, 128>(p, min_rows, l, stream, err);
+  return p.type == kKvF16 ? launch_t<__half, 64>(p, min_rows, l, stream, err)
+                          : launch_t<__nv_bfloat16, 64>(p, min_rows, l, stream, err);
+}
+
+cudaError_t kv8_prefill_join_launch(const Kv8AttentionParams& p, int min_rows, void* workspace, cudaStream_t stream) {
+  const Launch l = launch_of(p, workspace);
+  if (l.shares == 1) return cudaSuccess;
+  if (p.cache.dim == 128)
+    return p.type == kKvF16 ? join_t<__half, 128>(p, min_rows, l, stream)
+                            : join_t<__nv_bfloat16, 128>(p, min_rows, l, stream);
+  return p.type == kKvF16 ? join_t<__half, 64>(p, min_rows, l, stream)
+                          : join_t<__nv_bfloat16, 64>(p, min_rows, l, stream);
 }
 
 int kv8_status_fetch_and_clear() {

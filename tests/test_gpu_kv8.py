@@ -462,6 +462,38 @@ def test_shares_without_keys(ops):
     assert (got[100:102] == 3).all() and not got[102:179].any()
 
 
+@pytest.mark.parametrize("kv", [300, 3000])
+def test_steps_that_follow_at_once_read_what_was_appended(ops, kv):
+    """Appends over the same slots and attention of prompts beside single tokens, waited for and not."""
+    size, heads, q_heads, dim = 32, 2, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(20)
+    q_lens = [1] * 40 + [130, 200] + [1] * 3
+    kv_lens = [kv - i if q == 1 else kv for i, q in enumerate(q_lens)]
+    n, width, tokens = len(q_lens), -(-kv // size), sum(q_lens)
+    table = torch.randperm(n * width, generator=gen, device="cuda").to(torch.int32).view(n, width)
+    start = dev(np.cumsum([0] + q_lens))
+    ql, kl = dev(q_lens), dev(kv_lens)
+    at = [(r, kv_lens[r] - q + i) for r, q in enumerate(q_lens) for i in range(q)]
+    slots = torch.stack([table[r, pos // size] * size + pos % size for r, pos in at]).to(torch.int32)
+    first = [torch.randint(-127, 128, (n * width, heads, size, dim), dtype=torch.int8, generator=gen, device="cuda")
+             for _ in range(2)] + [torch.full((n * width, heads), 0.01, device="cuda") for _ in range(2)]
+    rows = [torch.randn(tokens, (q_heads + 2 * heads) * dim, generator=gen, device="cuda").half() for _ in range(12)]
+    outs = []
+    for waits in (True, False):
+        cache = [t.clone() for t in first]
+        got = []
+        for x in rows:
+            q = ops.kv8_append(x, *cache, slots)
+            if waits:
+                torch.cuda.synchronize()
+            got.append(ops.kv8_attention(q, *cache, table, start, ql, kl, max_q=200))
+            got.append(got[-1] + 1)  # a reader of all rows
+            if waits:
+                torch.cuda.synchronize()
+        outs.append(torch.stack(got).cpu())
+    assert torch.equal(*outs)
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_two_streams_at_once(ops, captured):
     """Calls that need a workspace on two streams, and two captured graphs of them, run side by side."""
