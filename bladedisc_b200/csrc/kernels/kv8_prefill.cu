@@ -11,17 +11,18 @@
 //                other tile's products run.
 //   softmax      a warpgroup per query tile, a thread per row: running maximum in the scale of log2, exp2, sums in
 //                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
-// Few rows over a long cache: several CTAs take shares of an item's keys (shares_for) and a second kernel joins them.
+// Few rows over a long cache: several CTAs take shares of an item's keys (launch_of) and a second kernel joins them.
 // Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
 // loader keeps (O is in its units), so that P stays in the range of f16; see kPScaleLog2.
 // What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all): shared memory 3070 cycles (levels in
 // and out 512, operands out 512, Q and K into S 1536 at 64 keys a product, V into O 512), exp2 2048 at 16 a cycle less
-// the quarter that goes to the FMA pipe, products 2560.  Measured at 4095 tokens behind 12289, 32 over 8 heads: 0.98 ms
-// (1.04 on the slowest card seen) = 980 TFLOP/s, 0.59 of the measured bf16 rate; one of eight CTA rounds is not full.  What was measured on the way there:
-// scores of 128 keys in one buffer 1.07 ms (the chain softmax, P V, S is exposed), one issuer for both tiles 1.44,
+// the quarter that goes to the FMA pipe, products 2560.  Measured at 4095 tokens behind 12289, 32 over 8 heads: 0.95 ms
+// (0.90 to 1.0 as the card's power allows) = 1010 TFLOP/s, 0.61 of the measured bf16 rate.  What was measured on the way
+// there, in the order of the steps, beside 0.98: scores of 128 keys in one buffer 1.07 ms (the chain softmax, P V, S is
+// exposed), one issuer for both tiles 1.44,
 // products issued behind `lane == 0` 1.20, levels to registers instead of TMA 1.40, exp2 all on the MUFU 1.01, half of
 // them on the FMA pipe 1.08, taking turns in exp2 1.02.  Short prompts pay for the start of a CTA (8300 cycles to the
-// first score) and its end (3900): 4 prompts of 256 to 2048 tokens, 32 heads: 130 us = 505 TFLOP/s.
+// first score) and its end (3900): 4 prompts of 256 to 2048 tokens, 32 heads: 127 us = 517 TFLOP/s.
 #include "kv8.h"
 
 #include <algorithm>
@@ -357,18 +358,21 @@ __device__ __forceinline__ bool item_of(const Kv8AttentionParams& p, uint32_t in
   return true;
 }
 
-// What a share of the keys leaves of a row when an item has several: row = token * query heads + head.
-struct ShareWs {
-  float* o;    // [shares][rows][dim], of weights that add up to one: nothing overflows on the way to the join
-  float2* ml;  // [shares][rows] maximum and sum
-  int64_t rows;
+// The items whose keys n CTAs share, and what a share leaves of their rows (256 of each item).
+struct Shares {
+  uint32_t from, to, n;
+  int64_t rows;  // (to - from) * 256
+  float* o;      // [n][rows][dim], of weights that add up to one: nothing overflows on the way to the join
+  float2* ml;    // [n][rows] maximum and sum
 };
 
-template <typename T, int D, bool SHARES>
+// Which items' keys are shared; a way of writing a row that is not needed would cost registers (2 to 9 %).
+enum class Cut { kNone, kAll, kSome };
+
+template <typename T, int D, Cut CUT>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-               const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, uint32_t shares, ShareWs ws,
-               int box_rows) {
+               const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, Shares sh, int box_rows) {
   using L = Smem<D>;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -394,12 +398,29 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 
   grid_dep_wait();
   grid_dep_launch();
+  uint32_t index = blockIdx.x, share = 0, shares = 1;
+  constexpr bool SHARES = CUT != Cut::kNone;
+  if constexpr (CUT == Cut::kAll) {
+    shares = sh.n;
+    share = index % shares;
+    index /= shares;
+  } else if (SHARES && index >= sh.from) {
+    index -= sh.from;
+    const uint32_t span = (sh.to - sh.from) * sh.n;
+    if (index < span) {
+      shares = sh.n;
+      share = index % shares;
+      index = sh.from + index / shares;
+    } else {
+      index += sh.to - span;
+    }
+  }
   Item it;
-  if (!item_of(p, SHARES ? blockIdx.x / shares : blockIdx.x, blocks, min_rows, lane, it)) return;
+  if (!item_of(p, index, blocks, min_rows, lane, it)) return;
   const int head = it.head, r = it.r, row0 = it.row0, rows = it.rows, keys = it.keys;
   const int64_t behind = it.behind, tok0 = it.tok0;
   // this CTA's share of the key tiles: nt tiles from key_first on, nu steps
-  const int share = SHARES ? static_cast<int>(blockIdx.x % shares) : 0, tiles_all = (keys + kTile - 1) / kTile;
+  const int tiles_all = (keys + kTile - 1) / kTile;
   const int t_first = SHARES ? static_cast<int>(static_cast<int64_t>(tiles_all) * share / shares) : 0;
   const int nt = SHARES ? static_cast<int>(static_cast<int64_t>(tiles_all) * (share + 1) / shares) - t_first : tiles_all;
   const int key_first = t_first * kTile;
@@ -578,10 +599,11 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     // ---- epilogue
     if (active) {
       T* dst = static_cast<T*>(p.out) + (there ? at * p.ld_out + (head * G + h) * D : 0);
-      const int64_t slot = there ? share * ws.rows + at * p.q_heads + head * G + h : 0;
+      const bool joined = CUT == Cut::kAll || (SHARES && shares > 1);
+      const int64_t slot = SHARES ? share * sh.rows + (index - sh.from) * (2 * kTile) + q * kTile + row : 0;
       if (nt == 0) {
-        if (SHARES && there) {
-          ws.ml[slot] = make_float2(-INFINITY, 0.f);
+        if (there && joined) {
+          sh.ml[slot] = make_float2(-INFINITY, 0.f);
         } else if (there) {
 #pragma unroll
           for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0, 0, 0, 0);
@@ -595,48 +617,54 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           unpair(add2(sum[0], sum[1]), a, b);
           const float l = a + b;
           const float k = l == 0.f ? 0.f : info[(nt - 1) % kInfo].ref / l;
-          if (SHARES && there) ws.ml[slot] = make_float2(m, l);
+          if (there && joined) sh.ml[slot] = make_float2(m, l);
           // the scores of all steps are done with q: its tile takes the output, f32 in two halves
-          const int64_t to = !there ? -1 : SHARES ? slot * D : at * p.ld_out + (head * G + h) * D;
+          const int64_t to = !there ? -1 : joined ? slot * D : at * p.ld_out + (head * G + h) * D;
+          auto emit = [&](auto f32) {
+            constexpr bool F32 = decltype(f32)::value;
 #pragma unroll
-          for (int half = 0; half < (SHARES ? 2 : 1); ++half) {
+            for (int half = 0; half < (F32 ? 2 : 1); ++half) {
 #pragma unroll
-            for (int sub = 0; sub < D / 64; ++sub) {
+              for (int sub = 0; sub < D / 64; ++sub) {
 #pragma unroll
-              for (int e = 0; e < (SHARES ? 1 : 2); ++e) {
-                const int cc = SHARES ? half * (D / 64) + sub : sub * 2 + e;
-                uint32_t o[32];
-                tmem_ld_x32(t_o + cc * 32, o);
-                tmem_ld_wait32(o);
+                for (int e = 0; e < (F32 ? 1 : 2); ++e) {
+                  const int cc = F32 ? half * (D / 64) + sub : sub * 2 + e;
+                  uint32_t o[32];
+                  tmem_ld_x32(t_o + cc * 32, o);
+                  tmem_ld_wait32(o);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * k);
-                if constexpr (SHARES) {
+                  for (int j = 0; j < 32; ++j) o[j] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * k);
+                  if constexpr (F32) {
 #pragma unroll
-                  for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<uint4*>(stage(row, sub * 8 + j)) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                } else {
-                  uint32_t w[16];
+                    for (int j = 0; j < 32; j += 4)
+                      *reinterpret_cast<uint4*>(stage(row, sub * 8 + j / 4)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                  } else {
+                    uint32_t w[16];
 #pragma unroll
-                  for (int j = 0; j < 16; ++j)
-                    w[j] = pack2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]), T());
+                    for (int j = 0; j < 16; ++j)
+                      w[j] = pack2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]), T());
 #pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<uint4*>(stage(row, cc * 4 + j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                    for (int j = 0; j < 16; j += 4)
+                      *reinterpret_cast<uint4*>(stage(row, cc * 4 + j / 4)) = make_uint4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+                  }
                 }
               }
-            }
-            __syncwarp();
+              __syncwarp();
 #pragma unroll
-            for (int i = 0; i < kLanes; ++i) {
-              const int64_t f = __shfl_sync(~0u, to, i * kAtOnce + lane / kLanes);
-              const uint4 x = *reinterpret_cast<const uint4*>(staged(i));
-              if (f >= 0) {
-                if constexpr (SHARES) *reinterpret_cast<uint4*>(ws.o + f + half * (D / 2) + chunk * 4) = x;
-                else *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + f + chunk * 8) = x;
+              for (int i = 0; i < kLanes; ++i) {
+                const int64_t f = __shfl_sync(~0u, to, i * kAtOnce + lane / kLanes);
+                const uint4 x = *reinterpret_cast<const uint4*>(staged(i));
+                if (f >= 0) {
+                  if constexpr (F32) *reinterpret_cast<uint4*>(sh.o + f + half * (D / 2) + chunk * 4) = x;
+                  else *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + f + chunk * 8) = x;
+                }
               }
+              __syncwarp();
             }
-            __syncwarp();
-          }
+          };
+          if constexpr (CUT != Cut::kSome) emit(std::bool_constant<SHARES>());
+          else if (joined) emit(std::true_type());
+          else emit(std::false_type());
         }
       }
     }
@@ -829,22 +857,22 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   }
 }
 
-// Joins the shares of the rows of item blockIdx.x: a warp per row, a lane per share for the weights.
-constexpr int kJoinThreads = 256, kMostShares = 32;
+// Joins the shares of the rows of the blockIdx.x-th item that has them: a warp per row, a lane per share for the weights.
+constexpr int kJoinThreads = 256, kMostShares = 32, kMostPieces = 512;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-prefill_join_kernel(const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, int shares, ShareWs ws) {
+prefill_join_kernel(const __grid_constant__ Kv8AttentionParams p, int min_rows, uint32_t blocks, Shares sh) {
   grid_dep_wait();
   grid_dep_launch();
-  const int lane = threadIdx.x & 31, G = p.q_heads / p.cache.kv_heads;
+  const int lane = threadIdx.x & 31, G = p.q_heads / p.cache.kv_heads, shares = static_cast<int>(sh.n);
   Item it;
-  if (!item_of(p, blockIdx.x, blocks, min_rows, lane, it)) return;
+  if (!item_of(p, sh.from + blockIdx.x, blocks, min_rows, lane, it)) return;
   for (int i = (blockIdx.y * kJoinThreads + threadIdx.x) / 32; i < it.rows; i += gridDim.y * (kJoinThreads / 32)) {
     const int64_t at = it.tok0 + (it.row0 + i) / G;
     if (at < 0 || at >= p.tokens) continue;
     const int col = it.head * G + (it.row0 + i) % G;
-    const int64_t row = at * p.q_heads + col;
-    const float2 ml = lane < shares ? ws.ml[lane * ws.rows + row] : make_float2(-INFINITY, 0.f);
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (2 * kTile) + i;
+    const float2 ml = lane < shares ? sh.ml[lane * sh.rows + row] : make_float2(-INFINITY, 0.f);
     float top = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
@@ -858,7 +886,7 @@ prefill_join_kernel(const __grid_constant__ Kv8AttentionParams p, int min_rows, 
 #pragma unroll 8
     for (int k = 0; k < shares; ++k) {
       const float wk = __shfl_sync(~0u, w, k);
-      const float* v = ws.o + (k * ws.rows + row) * D + lane * E;
+      const float* v = sh.o + (k * sh.rows + row) * D + lane * E;
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
         const float2 x = wk != 0.f ? *reinterpret_cast<const float2*>(v + e) : make_float2(0.f, 0.f);
@@ -872,55 +900,54 @@ prefill_join_kernel(const __grid_constant__ Kv8AttentionParams p, int min_rows, 
   }
 }
 
-// Shares that the keys of an item are cut into, so that few rows over long caches fill the GPU: as many as make one to
-// three full rounds of CTAs, where the rounds (as measured 2.1 us per key tile and 8 per CTA) and the join (5 us, and
-// its bytes at 6 TB/s) come to a tenth less than they do without shares.  The host has bounds only: the rows of the
-// batch, and the longest cache.  (8 kv heads of 128 with 4 query heads each, one request: 64 tokens over 8 000
-// 139 -> 33 us, 100 over 30 000 492 -> 82 us, 512 over 8 192 146 -> 94 us.)
-int shares_for(const Kv8AttentionParams& p) {
-  const int64_t rows = p.tokens * (p.q_heads / p.cache.kv_heads);
-  const int64_t items = (rows + 2 * kTile - 1) / (2 * kTile) * p.cache.kv_heads, sms = device_sm_count();
-  const double tiles = static_cast<double>((p.max_kv + kTile - 1) / kTile);
-  double best = 0.9 * static_cast<double>((items + sms - 1) / sms) * (tiles * 2.1 + 8);
-  int shares = 1;
-  for (int64_t round = 1; round <= 3; ++round) {
-    const int64_t n = std::min<int64_t>(std::min<int64_t>(round * sms / items, kMostShares), static_cast<int64_t>(tiles) / 4);
-    if (n < 2) continue;
-    const double t = static_cast<double>((items * n + sms - 1) / sms) * (tiles / n * 2.1 + 8) + 5 +
-                     static_cast<double>(rows * p.cache.kv_heads * n) * p.cache.dim * 8 / 6e6;
-    if (t < best) {
-      best = t;
-      shares = static_cast<int>(n);
-    }
-  }
-  return shares;
-}
-
 struct Launch {
   int64_t rows, blocks, items;
-  int shares;
-  ShareWs ws;
+  Shares sh;
 };
+// The grid, and which items' keys are cut into shares: all of them, so that few rows over long caches fill the GPU, or
+// those that would not fill the last round of CTAs.  As many shares as make one to three full rounds, where the rounds
+// (as measured 2.1 us per key tile and 8 per CTA) and the join (5 us, and its bytes at 6 TB/s) come to 6 % less than they
+// do without shares.  The host has bounds only: the rows of the batch, and the longest cache.  (8 kv heads of 128 with 4
+// query heads each, one request: 64 tokens over 8 000 139 -> 33 us, 100 over 30 000 492 -> 82 us, 512 over 8 192
+// 146 -> 94 us; 4095 over 16 384, 3.46 rounds: the last round alone, 0.99 -> 0.95 ms; 1500 over 12 000, 1.3 rounds:
+// 339 -> 295 us.)
 Launch launch_of(const Kv8AttentionParams& p, void* workspace) {
   Launch l = {};
-  const int64_t G = p.q_heads / p.cache.kv_heads;
+  const int64_t G = p.q_heads / p.cache.kv_heads, KH = p.cache.kv_heads, sms = device_sm_count();
   l.rows = p.max_q * G;
   l.blocks = (l.rows + 2 * kTile - 1) / (2 * kTile);
   // no more blocks than the rows of the batch make, and one more for the rest of each request
-  const int64_t most = p.tokens * G / (2 * kTile) + std::min<int64_t>(p.requests, p.tokens);
-  l.items = std::min(l.blocks * p.requests, most) * p.cache.kv_heads;
-  l.shares = shares_for(p);
-  if (l.shares > 1) {
-    l.ws.rows = p.tokens * p.q_heads;
-    l.ws.o = static_cast<float*>(workspace);
-    l.ws.ml = reinterpret_cast<float2*>(l.ws.o + l.shares * l.ws.rows * p.cache.dim);
+  l.items = std::min(l.blocks * p.requests, p.tokens * G / (2 * kTile) + std::min<int64_t>(p.requests, p.tokens)) * KH;
+  const int64_t likely = std::min(l.items, (p.tokens * G + 2 * kTile - 1) / (2 * kTile) * KH);
+  const double tiles = static_cast<double>((p.max_kv + kTile - 1) / kTile);
+  auto rounds = [&](int64_t ctas, int64_t n) { return static_cast<double>((ctas + sms - 1) / sms) * (tiles / n * 2.1 + 8); };
+  double best = 0.94 * rounds(likely, 1);
+  l.sh.n = 1;
+  for (const int64_t from : {int64_t{0}, likely / sms * sms}) {
+    const int64_t cut = likely - from;
+    for (int64_t round = 1; round <= 3 && cut > 0; ++round) {
+      const int64_t n = std::min({round * sms / cut, int64_t{kMostShares}, static_cast<int64_t>(tiles) / 4});
+      if (n < 2) continue;
+      const double t = rounds(from, 1) + rounds(cut * n, n) + 5 + static_cast<double>(cut * n) * (2 * kTile) * p.cache.dim * 8 / 6e6;
+      if (t < best) {
+        best = t;
+        l.sh.n = static_cast<uint32_t>(n);
+        l.sh.from = static_cast<uint32_t>(from);
+      }
+    }
+  }
+  if (l.sh.n > 1) {
+    l.sh.to = static_cast<uint32_t>(std::min<int64_t>(l.items, l.sh.from + kMostPieces / l.sh.n));
+    l.sh.rows = static_cast<int64_t>(l.sh.to - l.sh.from) * (2 * kTile);
+    l.sh.o = static_cast<float*>(workspace);
+    if (workspace) l.sh.ml = reinterpret_cast<float2*>(l.sh.o + l.sh.n * l.sh.rows * p.cache.dim);
   }
   return l;
 }
 
 template <typename T, int D>
 cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, const Launch& l, cudaStream_t stream, const char** err) {
-  if (l.rows > INT32_MAX - 2 * kTile || l.items > INT32_MAX / kMostShares) {
+  if (l.rows > INT32_MAX - 2 * kTile || l.items > INT32_MAX / 2) {
     *err = "too many query rows";
     return cudaErrorInvalidValue;
   }
@@ -930,28 +957,32 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int min_rows, const Launch& l,
     *err = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = l.shares > 1 ? prefill_kernel<T, D, true> : prefill_kernel<T, D, false>;
+  const Cut cut = l.sh.n == 1 ? Cut::kNone : l.sh.from == 0 && l.sh.to == l.items ? Cut::kAll : Cut::kSome;
+  auto kern = cut == Cut::kNone  ? prefill_kernel<T, D, Cut::kNone>
+              : cut == Cut::kAll ? prefill_kernel<T, D, Cut::kAll>
+                                 : prefill_kernel<T, D, Cut::kSome>;
   constexpr int smem = Smem<D>::kDynamic;
-  static std::atomic<uint64_t> ready[2] = {{0}, {0}};
-  const cudaError_t st = allow_smem(kern, smem, ready[l.shares > 1]);
+  static std::atomic<uint64_t> ready[3] = {{0}, {0}, {0}};
+  const cudaError_t st = allow_smem(kern, smem, ready[static_cast<int>(cut)]);
   if (st != cudaSuccess) return st;
-  return launch_dependent(kern, dim3(static_cast<unsigned>(l.items * l.shares)), dim3(kThreads), smem, stream, tk, tv, p,
-                          min_rows, static_cast<uint32_t>(l.blocks), static_cast<uint32_t>(l.shares), l.ws, box);
+  const int64_t ctas = l.items + static_cast<int64_t>(l.sh.to - l.sh.from) * (l.sh.n - 1);
+  return launch_dependent(kern, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), smem, stream, tk, tv, p, min_rows,
+                          static_cast<uint32_t>(l.blocks), l.sh, box);
 }
 
 template <typename T, int D>
 cudaError_t join_t(const Kv8AttentionParams& p, int min_rows, const Launch& l, cudaStream_t stream) {
-  // two rounds of CTAs, a row per warp at least
-  const int slices = static_cast<int>(std::clamp<int64_t>(16 * device_sm_count() / l.items, 1, 2 * kTile * 32 / kJoinThreads));
-  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(l.items), slices), dim3(kJoinThreads), 0,
-                          stream, p, min_rows, static_cast<uint32_t>(l.blocks), l.shares, l.ws);
+  const int64_t items = l.sh.to - l.sh.from;  // two rounds of CTAs, a row per warp at least
+  const int slices = static_cast<int>(std::clamp<int64_t>(16 * device_sm_count() / items, 1, 2 * kTile * 32 / kJoinThreads));
+  return launch_dependent(prefill_join_kernel<T, D>, dim3(static_cast<unsigned>(items), slices), dim3(kJoinThreads), 0,
+                          stream, p, min_rows, static_cast<uint32_t>(l.blocks), l.sh);
 }
 
 }  // namespace
 
 int64_t kv8_prefill_workspace_bytes(const Kv8AttentionParams& p) {
-  const int shares = shares_for(p);
-  return shares > 1 ? shares * p.tokens * p.q_heads * (static_cast<int64_t>(p.cache.dim) * 4 + 8) : 0;
+  const Launch l = launch_of(p, nullptr);
+  return l.sh.n > 1 ? l.sh.n * l.sh.rows * (static_cast<int64_t>(p.cache.dim) * 4 + 8) : 0;
 }
 
 cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, void* workspace, cudaStream_t stream,
@@ -966,7 +997,7 @@ cudaError_t kv8_prefill_launch(const Kv8AttentionParams& p, int min_rows, void* 
 
 cudaError_t kv8_prefill_join_launch(const Kv8AttentionParams& p, int min_rows, void* workspace, cudaStream_t stream) {
   const Launch l = launch_of(p, workspace);
-  if (l.shares == 1) return cudaSuccess;
+  if (l.sh.n == 1) return cudaSuccess;
   if (p.cache.dim == 128)
     return p.type == kKvF16 ? join_t<__half, 128>(p, min_rows, l, stream)
                             : join_t<__nv_bfloat16, 128>(p, min_rows, l, stream);
