@@ -22,7 +22,7 @@ namespace {
 // per SM: ragged lengths balance to one step.  A share that ends inside an item leaves its partial maximum, sum and
 // output in the workspace, and a second small kernel joins them.  Short caches (max_kv <= kKv8DirectKeys) take one CTA
 // per item and need neither, and so do those up to kDirectMost keys when there are items for two rounds of CTAs: 32
-// requests of up to 2048 tokens and 32 heads take 61 us that way and 73 in shares; 8 requests of up to 32700 tokens and
+// requests of up to 2048 tokens and 32 heads take 65 us that way and 73 in shares; 8 requests of up to 32700 tokens and
 // 8 kv heads take 252 us that way and 61 in shares.
 //
 // Inside a CTA a warp runs by itself: it fetches its steps with 16-byte asynchronous copies into its own ring (TMA
@@ -36,7 +36,10 @@ namespace {
 //                fragment layout with one 8 x 8 transpose.
 // Query rows in bf16 are scaled by a power of two per row to f16 (exact but for values 2^-24 of the row's largest).
 // P goes to f16 times 2^11 so that a probability keeps its 11 bits down to 2^-25 of the largest; the
-// value scale is multiplied in relative to a running reference that O is kept in units of.
+// value scale is multiplied in relative to a running reference that O is kept in units of.  With f16 results what the
+// rounding of P leaves out is multiplied too: over values of either sign it weighs as much as the rounding of the result
+// (error 0.00021, that of one rounding, instead of 0.00025 to 0.00031; 61 -> 64.6 us for the 32 requests).  In bf16 results
+// (0.0017) it does not show.
 // Rows in the ring are swizzled (16-byte chunk c of row r at c ^ (r & 7), for dim 64 c ^ (r / 2 & 3)); that and the key
 // order perm(n) = n ^ ((n & 1) << 2) make the 16-byte shared-memory reads free of bank conflicts.
 //
@@ -146,6 +149,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
   constexpr int KQ = D / 16;  // k steps of the first product
   constexpr int NV = D / 16;  // m tiles of the second
   constexpr int ROWS = 8 * NQ;
+  constexpr bool kRest = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float part_m[W][ROWS], part_l[W][ROWS];
   __shared__ long long sums[W];
@@ -451,7 +455,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           }
         }
       }
-      uint32_t pb[2][NQ][2];
+      uint32_t pb[2][NQ][2], pr[2][NQ][2];  // P in f16, and what that rounding left out (kRest)
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         const float base[2] = {(m[j][0] == -INFINITY ? 0.f : m[j][0]) - kPScaleLog2,
@@ -471,8 +475,16 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
             for (int e = 0; e < 4; ++e)
               if (key0 + mt * 16 + (e >> 1) * 8 + prow >= lim[j][e & 1] || (mt == 0 ? id0 : id1) < 0) pv[e] = 0.f;
           }
-          pb[mt][j][0] = transpose8x8(pack2(pv[0], pv[1], __half()));
-          pb[mt][j][1] = transpose8x8(pack2(pv[2], pv[3], __half()));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t high = pack2(pv[2 * e], pv[2 * e + 1], __half());
+            pb[mt][j][e] = transpose8x8(high);
+            if constexpr (kRest) {
+              float a, b;
+              unpack2(high, a, b, __half());
+              pr[mt][j][e] = transpose8x8(pack2(pv[2 * e] - a, pv[2 * e + 1] - b, __half()));
+            }
+          }
         }
       }
 #pragma unroll
@@ -501,7 +513,10 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
             const uint32_t a[4] = {bytes_to_f16(lo, 0x4140), bytes_to_f16(lo, 0x4342), bytes_to_f16(hi, 0x4140),
                                    bytes_to_f16(hi, 0x4342)};
 #pragma unroll
-            for (int j = 0; j < NQ; ++j) mma_f16(o[j][q4 * 2 + u], a, pb[mt][j][0], pb[mt][j][1]);
+            for (int j = 0; j < NQ; ++j) {
+              mma_f16(o[j][q4 * 2 + u], a, pb[mt][j][0], pb[mt][j][1]);
+              if constexpr (kRest) mma_f16(o[j][q4 * 2 + u], a, pr[mt][j][0], pr[mt][j][1]);
+            }
           }
         }
       }

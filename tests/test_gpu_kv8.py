@@ -462,6 +462,21 @@ def test_shares_without_keys(ops):
     assert (got[100:102] == 3).all() and not got[102:179].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("q_lens, kv_lens, width", [
+    ([330], [1100], 100),              # a whole round of items, and a few whose keys are in shares
+    ([200, 1, 131], [900, 40, 700], 100),
+    ([331] + [1] * 40, [1000] + [20] * 40, 120),   # room for more items than there are
+])
+def test_last_round_in_shares(ops, q_lens, kv_lens, width, dtype):
+    """Up to 33 row blocks of 8 kv heads with 24 query heads each: more than one CTA per SM, the rest in shares."""
+    rng = np.random.default_rng(21)
+    got, want, slack, (q, d, args, mq) = _attend(ops, rng, q_lens, kv_lens, 16, 8, 192, 64, dtype, width=width)
+    _check(got, want, slack)
+    again = ops.kv8_attention(q, *d, *args, max_q=mq)
+    assert torch.equal(got, again)
+
+
 @pytest.mark.parametrize("kv", [300, 3000])
 def test_steps_that_follow_at_once_read_what_was_appended(ops, kv):
     """Appends over the same slots and attention of prompts beside single tokens, waited for and not."""
