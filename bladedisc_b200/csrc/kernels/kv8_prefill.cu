@@ -22,7 +22,7 @@
 // exposed), one issuer for both tiles 1.44,
 // products issued behind `lane == 0` 1.20, levels to registers instead of TMA 1.40, exp2 all on the MUFU 1.01, half of
 // them on the FMA pipe 1.08, taking turns in exp2 1.02.  Short prompts pay for the start of a CTA (8300 cycles to the
-// first score) and its end (3900): 4 prompts of 256 to 2048 tokens, 32 heads: 127 us = 517 TFLOP/s.
+// first score) and its end (3900): 4 prompts of 256 to 2048 tokens, 32 heads: 140 us = 470 TFLOP/s in f16.
 #include "kv8.h"
 
 #include <algorithm>
@@ -59,6 +59,7 @@ constexpr int kSubTile = kTile * 128;    // 128 rows of 64 f16
 struct TileInfo {
   float f[kGroups];   // key scale * softmax scale * log2 e
   float w[kGroups];   // value scale / reference
+  float back[kGroups];  // its inverse, or 0 where P rounded to f16 does not stand for its part of the sum (kRoundedSum)
   float down;         // old reference / new one
   float ref;
   uint32_t there;     // bit per group: the block exists and has keys that some row sees
@@ -197,8 +198,12 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
 // Scores of one row and step -> P in TMEM and the row's sum.  EDGE: some keys are hidden from some rows.
 // `left` keys are visible from the step's first on; groups that are not `present` are not.
 constexpr uint32_t kOnFma = 0x22;  // of the eight pairs of a group, those whose exp2 is a polynomial
-template <bool EDGE>
-__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, float rmul, float off, uint32_t t_p,
+// ROUNDED: the row's sum is that of P as f16 holds it (divided by its value scale again), so that the rounding of the
+// largest ones cancels where the output is divided by it.  For f16 results only: their error falls from 0.00029 (up to
+// 0.00032, 1.5 roundings, in batches with few prompts) to 0.00025, for 10 % of the time (4 prompts 127 -> 140 us, mixed
+// 67 -> 72 us); with the sum corrected by what the rounding took, at edges too, 148 us.
+template <bool EDGE, bool ROUNDED>
+__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back, float rmul, float off, uint32_t t_p,
                                              int left, uint32_t present, uint64_t* sum) {
   const uint64_t off2 = pair(off, off);
 #pragma unroll
@@ -207,7 +212,7 @@ __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs,
 #pragma unroll
     for (int g = cc * 2; g < cc * 2 + 2; ++g) {
       const float f = fs[g] * rmul, vw = ws[g];
-      const uint64_t f2 = pair(f, f), w2 = pair(vw, vw);
+      const uint64_t f2 = pair(f, f), w2 = pair(vw, vw), back2 = ROUNDED ? pair(back[g], back[g]) : 0;
       const int see = EDGE ? ((present >> g & 1) ? left - g * 16 : 0) : 16;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -225,13 +230,19 @@ __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs,
           if (2 * e + 1 >= see) b = 0.f;
         }
         const uint64_t ab = pair(a, b);
-        sum[e & 1] = add2(sum[e & 1], ab);
+        if constexpr (!ROUNDED) sum[e & 1] = add2(sum[e & 1], ab);
         unpair(mul2(ab, w2), a, b);
         if (EDGE) {  // 0 whatever the scale is
           if (2 * e >= see) a = 0.f;
           if (2 * e + 1 >= see) b = 0.f;
         }
-        w[(g & 1) * 8 + e] = pack2(a, b, __half());
+        const uint32_t word = pack2(a, b, __half());
+        if constexpr (ROUNDED) {
+          float ra, rb;
+          unpack2(word, ra, rb, __half());
+          sum[e & 1] = fma2(pair(ra, rb), back2, sum[e & 1]);
+        }
+        w[(g & 1) * 8 + e] = word;
       }
     }
     tmem_st_x16(t_p + cc * 16, w);
@@ -400,6 +411,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
   grid_dep_launch();
   uint32_t index = blockIdx.x, share = 0, shares = 1;
   constexpr bool SHARES = CUT != Cut::kNone;
+  constexpr bool kRoundedSum = std::is_same<T, __half>::value;
   if constexpr (CUT == Cut::kAll) {
     shares = sh.n;
     share = index % shares;
@@ -589,8 +601,17 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
       }
       const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
-      if (!edge) softmax_step<false>(s, fs, ws, rmul, off, t_s, 0, 0, sum);
-      else softmax_step<true>(s, fs, ws, rmul, off, t_s, lim - key0, present, sum);
+      const float* back = in.back + first_group;
+      bool rounded = kRoundedSum;
+#pragma unroll
+      for (int g = 0; g < kStepGroups; ++g) rounded = rounded && back[g] != 0.f;
+      if (edge) {
+        softmax_step<true, false>(s, fs, ws, back, rmul, off, t_s, lim - key0, present, sum);
+      } else if (kRoundedSum && rounded) {
+        softmax_step<false, kRoundedSum>(s, fs, ws, back, rmul, off, t_s, 0, 0, sum);
+      } else {
+        softmax_step<false, false>(s, fs, ws, back, rmul, off, t_s, 0, 0, sum);
+      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -771,7 +792,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       TileInfo& in = info[t % kInfo];
       if (lane < kGroups) {
         in.f[lane] = ks;
-        in.w[lane] = vs / ref;
+        const float w = vs / ref;
+        in.w[lane] = w;
+        if (kRoundedSum) in.back[lane] = w >= 0.0625f && w <= kRefSlack ? 1.f / w : 0.f;
       }
       if (lane == 0) {
         in.down = down;
