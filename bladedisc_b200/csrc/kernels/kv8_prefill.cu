@@ -933,7 +933,7 @@ struct Launch {
 // do without shares.  The host has bounds only: the rows of the batch, and the longest cache.  (8 kv heads of 128 with 4
 // query heads each, one request: 64 tokens over 8 000 139 -> 33 us, 100 over 30 000 492 -> 82 us, 512 over 8 192
 // 146 -> 94 us; 4095 over 16 384, 3.46 rounds: the last round alone, 0.99 -> 0.95 ms; 1500 over 12 000, 1.3 rounds:
-// 339 -> 295 us.)
+// 339 -> 295 us.  In f16, before its sums were those of P as rounded, which adds up to 10 % to both sides.)
 Launch launch_of(const Kv8AttentionParams& p, void* workspace) {
   Launch l = {};
   const int64_t G = p.q_heads / p.cache.kv_heads, KH = p.cache.kv_heads, sms = device_sm_count();
