@@ -129,11 +129,16 @@ class QuantDecoder:
         return ColumnParallelQLinear(wq, scale, None, self.comm, rows=(0, wq.shape[0]))
 
     # ------------------------------------------------------------------ pieces
-    def _rope_tables(self, upto: int) -> None:
+    def _rope_of(self, upto: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Cosines and sines of the positions below ``upto``, ``[upto, head_dim / 2]`` float32 each."""
         half = self.cfg.head_dim // 2
         inv = self.cfg.rope_theta ** (-torch.arange(half, device=self.device, dtype=torch.float32) / half)
         ang = torch.arange(upto, device=self.device, dtype=torch.float32)[:, None] * inv[None, :]
-        self._cos, self._sin = ang.cos(), ang.sin()
+        return ang.cos(), ang.sin()
+
+    def _rope_tables(self, upto: int) -> None:
+        """The tables of the dense cache; a paged one keeps its own."""
+        self._cos, self._sin = self._rope_of(upto)
 
     def _rope(self, x: torch.Tensor, pos0: int) -> torch.Tensor:
         """x [B, S, h, d]; rotates pairs (i, i + d/2) by position * theta^(-2i/d)."""
@@ -206,13 +211,17 @@ class QuantDecoder:
         return ops.rmsnorm(prev, self.g_final, cfg.eps, residual=h, x_gathered=True)
 
     def start_paged(self, requests: int, num_blocks: int, max_seq: int, block_size: int = 64) -> PagedKVCache8:
-        """A paged 8-bit cache for ``requests`` requests with lengths of their own (see `forward_paged`)."""
+        """A paged 8-bit cache for ``requests`` requests with lengths of their own (see `forward_paged`).  It stands
+        beside the cache of `start`: neither call changes what steps over the other, or over an earlier paged cache that
+        is still held, read and write."""
         cfg = self.cfg
-        self.paged = PagedKVCache8(cfg.layers, requests, num_blocks, cfg.heads // self.world, cfg.head_dim, max_seq,
-                                   block_size, self.device)
-        room = self.paged.table.shape[1] * block_size  # positions that a request can reach
-        self._rope_tables(max(room, 0 if self._cos is None else self._cos.shape[0]))
-        return self.paged
+        cache = PagedKVCache8(cfg.layers, requests, num_blocks, cfg.heads // self.world, cfg.head_dim, max_seq,
+                              block_size, self.device)
+        cache.rope = self._rope_of(cache.table.shape[1] * block_size)  # positions that a request can reach
+        if self.kv is None:  # no dense cache, nothing holds its tables
+            self._cos, self._sin = cache.rope
+        self.paged = cache
+        return cache
 
     def forward_paged(self, ids: torch.Tensor, tokens: torch.Tensor, max_q: int,
                       max_kv: Optional[int] = None) -> torch.Tensor:
@@ -224,11 +233,13 @@ class QuantDecoder:
         if self.paged is None:
             raise RuntimeError("call start_paged(requests, num_blocks, max_seq) first")
         cache = self.paged
+        if cache.rope is None:
+            raise RuntimeError("the paged cache has no rotation tables: start_paged makes one that has")
         total = ids.numel()
         plan = cache.extend(tokens, total)
 
         def attention(L: _Layer, idx: int, qkv: torch.Tensor) -> torch.Tensor:
-            q = cache.append(idx, qkv, plan, self._cos, self._sin)
+            q = cache.append(idx, qkv, plan, *cache.rope)
             # zeros where no request has rows: the linears behind quantize every row
             out = cache.attend(idx, q, plan, max_q, max_kv, out=torch.zeros_like(q))
             return out.view(total, -1)

@@ -5,7 +5,7 @@ length of every request, and the stack of free blocks.  Everything lies on the G
 operators of :mod:`bladedisc_b200.ops`; no call reads it back, so a decode step can be captured into a CUDA graph.
 Steps must follow one another on one stream (or be ordered by the caller): they share the state.
 """
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -15,7 +15,10 @@ from . import ops
 class PagedKVCache8:
     """``requests`` rows of up to ``max_seq`` tokens over ``num_blocks`` blocks of ``block_size`` tokens.
 
-    Memory: ``2 * layers * num_blocks * kv_heads * (block_size * head_dim + 4)`` bytes."""
+    Memory: ``2 * layers * num_blocks * kv_heads * (block_size * head_dim + 4)`` bytes.
+
+    ``rope``: the cosines and sines of the positions that a request can reach, where a decoder keeps them with its cache:
+    a step that was captured into a graph holds their addresses as it does those of the cache."""
 
     def __init__(self, layers: int, requests: int, num_blocks: int, kv_heads: int, head_dim: int, max_seq: int,
                  block_size: int = 64, device="cuda"):
@@ -37,6 +40,7 @@ class PagedKVCache8:
         self.table = torch.full((requests, -(-max_seq // block_size)), -1, **i32)
         self.free_list = torch.arange(num_blocks - 1, -1, -1, **i32)  # block 0 is handed out first
         self.free_count = torch.full((1,), num_blocks, **i32)
+        self.rope: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
 
     def extend(self, tokens: torch.Tensor, max_tokens: int) -> ops.KvPlan:
         """Room for ``tokens[r]`` new tokens of each request; see :func:`ops.kv_blocks_extend`."""
