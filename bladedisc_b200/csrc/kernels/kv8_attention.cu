@@ -114,7 +114,6 @@ struct SplitShape {
   int stream;       // 1: equal shares of all steps; 0: one CTA per item
   int row_tiles;    // per kv head, from max_q (stream = 0)
   int max_rows;     // requests with more query rows per kv head than this are left to the other kernel
-  int beside;       // 1: runs while the other kernel, launched just before, still does
 };
 
 template <int D>
@@ -600,19 +599,15 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
   }
 }
 
-// Beside the prompts' kernel (which does not read what this one writes, nor the other way round) it starts on the SMs
-// that the last prompt CTAs leave free.  Those have all begun by then, that is what was launched before them is complete;
-// the fence drops what the L1 may hold from before.  One CTA stays until they have ended, so that the end of this grid
-// means the end of both.  (21 single tokens and 3 prompts of up to 511: 74 -> 66 us; 100 and one of 1000, 16 000 keys:
-// 826 -> 776 us; the f16 prompts' rounded sums came later and add 5 us to the first.)
+// After the prompts' kernel of a mixed batch it waits for that one like any other.  (Starting on the SMs that the last
+// prompt CTAs leave free took 71 us instead of 82 for 21 single tokens and 3 prompts of up to 511; but what the kernels
+// before the prompts' wrote is promised behind the wait only, and another thread may launch something between the two.)
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(kSplitThreads, 3)
 split_kernel(const __grid_constant__ Kv8AttentionParams p, SplitShape shape, SplitWs ws) {
-  if (shape.beside) __threadfence();
-  else grid_dep_wait();
+  grid_dep_wait();
   grid_dep_launch();
   split_body<T, D, NQ>(p, shape, ws);
-  if (shape.beside && blockIdx.x == 0 && blockIdx.y == 0) grid_dep_wait();
 }
 
 // Joins the pieces of the item that CTA blockIdx.x of split_kernel started.  D / 4 threads hold an output row; the
@@ -722,7 +717,6 @@ cudaError_t launch_t(const Kv8AttentionParams& p, int max_rows, cudaStream_t str
   const int64_t items = row_tiles * p.cache.kv_heads * p.requests;
   SplitShape shape;
   shape.max_rows = max_rows;
-  shape.beside = max_rows == kSplitRowsMixed ? 1 : 0;
   shape.row_tiles = static_cast<int>(row_tiles);
   // one CTA per item: at most what kDirectMost keys take if the others have nothing to do meanwhile
   shape.stream = p.max_kv > kKv8DirectKeys && (p.max_kv > kDirectMost || items < 2 * stream_ctas()) ? 1 : 0;
