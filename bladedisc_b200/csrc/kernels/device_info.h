@@ -3,6 +3,7 @@
 // per process: the cache is indexed by the ordinal of the current device.
 #pragma once
 #include <cuda_runtime.h>
+#include <stdint.h>
 
 #include <atomic>
 
@@ -27,6 +28,18 @@ inline int device_sm_count() {
     cache[dev].store(n, std::memory_order_relaxed);
   }
   return n;
+}
+
+// Dynamic shared memory above 48 KB, asked for once per kernel and device (`ready`: a bit per device).  `bytes` is the
+// most that any call of the kernel takes: the limit belongs to the process, and one set for a call's own size could be
+// lowered by another thread before that call is launched.
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& ready) {
+  const uint64_t bit = uint64_t{1} << current_device_ordinal();
+  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (st == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  return st;
 }
 
 }  // namespace disc_b200

@@ -2,8 +2,6 @@
 #pragma once
 #include "kv8.h"
 
-#include <atomic>
-
 #include "device_info.h"
 #include "kv8_types.cuh"
 #include "sm100_ptx.cuh"
@@ -53,16 +51,6 @@ __device__ __forceinline__ uint32_t top_q16(const __nv_bfloat16* p) {
 __device__ __forceinline__ float row_power(uint32_t top) {
   const int n = min(max(13 - (static_cast<int>(top >> 23) - 127), -120), 120);
   return __uint_as_float(static_cast<uint32_t>(n + 127) << 23);
-}
-
-// Dynamic shared memory above 48 KB, asked for once per kernel and device (`ready`: a bit per device).
-template <typename K>
-inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& ready) {
-  const uint64_t bit = uint64_t{1} << current_device_ordinal();
-  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  const cudaError_t st = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (st == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
-  return st;
 }
 
 // One box is `rows` tokens of one block and head.

@@ -318,11 +318,15 @@ const char* problem(const KvBlocksParams& p) {
   return nullptr;
 }
 
-cudaError_t launch(void (*kern)(KvBlocksParams), const KvBlocksParams& p, int ctas, int threads, size_t smem,
-                   cudaStream_t stream) {
+// Shared memory of a kernel with `arrays` values per request, and one.
+size_t smem_of(int arrays, int requests) { return sizeof(int32_t) * (arrays * static_cast<size_t>(requests) + 1); }
+
+template <void (*kern)(KvBlocksParams), int ARRAYS>
+cudaError_t launch(const KvBlocksParams& p, int ctas, int threads, cudaStream_t stream) {
+  const size_t smem = smem_of(ARRAYS, p.requests);
   if (smem > 48 * 1024) {
-    const cudaError_t st =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    static std::atomic<uint64_t> ready{0};
+    const cudaError_t st = allow_smem(kern, static_cast<int>(smem_of(ARRAYS, kKvMaxRequests)), ready);
     if (st != cudaSuccess) return st;
   }
   cudaLaunchConfig_t cfg = {};
@@ -362,12 +366,12 @@ cudaError_t kv_blocks_extend_launch(const KvBlocksParams& p, cudaStream_t stream
     }
     return st;
   }
-  const size_t smem = sizeof(int32_t) * (3 * static_cast<size_t>(p.requests) + 1);
   if (p.max_tokens <= 8 * kMaxThreads) {  // a token per thread
-    return launch(extend_kernel<true>, p, p.max_tokens <= kMaxThreads ? 1 : 8,
-                  threads_for(std::max(p.requests, p.max_tokens)), smem, stream);
+    return launch<extend_kernel<true>, 3>(p, p.max_tokens <= kMaxThreads ? 1 : 8,
+                                          threads_for(std::max(p.requests, p.max_tokens)), stream);
   }
-  const cudaError_t st = launch(extend_kernel<false>, p, 8, threads_for(std::max(p.requests, p.num_blocks / 8)), smem, stream);
+  const cudaError_t st =
+      launch<extend_kernel<false>, 3>(p, 8, threads_for(std::max(p.requests, p.num_blocks / 8)), stream);
   if (st != cudaSuccess) return st;
   const int64_t blocks = (static_cast<int64_t>(p.max_tokens) + 4 * kSlotThreads - 1) / (4 * kSlotThreads);
   return launch_dependent(slots_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kSlotThreads), 0, stream, p);
@@ -378,8 +382,8 @@ cudaError_t kv_blocks_trim_launch(const KvBlocksParams& p, cudaStream_t stream, 
   if (*err) return cudaErrorInvalidValue;
   if (p.requests == 0) return cudaSuccess;
   const int64_t most = static_cast<int64_t>(p.requests) * p.table_width;  // blocks that can come back
-  return launch(trim_kernel, p, most <= 8 * kMaxThreads ? 1 : 8, threads_for(std::max<int64_t>(p.requests, most / 4)),
-                sizeof(int32_t) * (2 * static_cast<size_t>(p.requests) + 1), stream);
+  return launch<trim_kernel, 2>(p, most <= 8 * kMaxThreads ? 1 : 8,
+                                threads_for(std::max<int64_t>(p.requests, most / 4)), stream);
 }
 
 }  // namespace disc_b200
