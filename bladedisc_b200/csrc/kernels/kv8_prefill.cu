@@ -163,19 +163,26 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Maxima that are NaN when one of their operands is.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float max16(const uint32_t* s) {
   auto f = [&](int i) { return __uint_as_float(s[i]); };
   const float a = max3(f(0), f(1), f(2)), b = max3(f(3), f(4), f(5)), c = max3(f(6), f(7), f(8));
   const float d = max3(f(9), f(10), f(11)), e = max3(f(12), f(13), f(14));
-  return max3(max3(a, b, c), max3(d, e, f(15)), -INFINITY);
+  return max2(max3(a, b, c), max3(d, e, f(15)));
 }
 // 2^x for a pair on the FMA pipe: x = n + f with |f| <= 1/2 by adding 1.5 2^23, a polynomial of degree 5 in f (the
-// minimax one, relative error 2^-22.6), n into the exponent.  Below 2^-125 the result stays there.
+// minimax one, relative error 2^-22.6, 2^-22.1 with the roundings), n into the exponent.  Below 2^-125 the result stays
+// there, and for NaN it is there too: the kernel does not count on this to show one.
 __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   float a, b;
   unpair(x, a, b);
@@ -560,15 +567,15 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       float mx = -INFINITY;
       if (!edge) {
 #pragma unroll
-        for (int g = 0; g < kStepGroups; ++g) mx = fmaxf(mx, max16(s + g * 16) * fs[g]);
+        for (int g = 0; g < kStepGroups; ++g) mx = max2(mx, max16(s + g * 16) * fs[g]);
       } else {
 #pragma unroll
         for (int g = 0; g < kStepGroups; ++g) {
           const int see = (present >> g & 1) ? lim - key0 - g * 16 : 0;
           float top = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = e < see ? fmaxf(top, __uint_as_float(s[g * 16 + e])) : top;
-          mx = see > 0 ? fmaxf(mx, top * fs[g]) : mx;
+          for (int e = 0; e < 16; ++e) top = e < see ? max2(top, __uint_as_float(s[g * 16 + e])) : top;
+          mx = see > 0 ? max2(mx, top * fs[g]) : mx;
         }
       }
       mx *= rmul;
@@ -600,6 +607,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           }
         }
       }
+      // A score that is NaN or +infinity makes all of the row's probabilities NaN, from here on: exp2_pair alone would
+      // lose it where only its keys have one.
+      if (!(mx < INFINITY)) m = __uint_as_float(0x7fc00000u);
       const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
       const float* back = in.back + first_group;
       bool rounded = kRoundedSum;
