@@ -35,8 +35,8 @@ namespace {
 //   O' += V' P'  a lane's fragments pair bytes of two keys: two byte permutes, again exact in f16; P changes its
 //                fragment layout with one 8 x 8 transpose.
 // Query rows in bf16 are scaled by a power of two per row to f16 (exact but for values 2^-24 of the row's largest).
-// P goes to f16 times 2^11 so that a probability keeps its 11 bits down to 2^-25 of the largest; the
-// value scale is multiplied in relative to a running reference that O is kept in units of.  With f16 results what the
+// P, a probability times its value scale, goes to f16 as 2^11 for a row's largest, so that it keeps its 11 bits down to
+// 2^-25 of that; a row of O is in units of the largest so far.  With f16 results what the
 // rounding of P leaves out is multiplied too: over values of either sign it weighs as much as the rounding of the result
 // (error 0.00021, that of one rounding, instead of 0.00025 to 0.00031; 61 -> 64.6 us for the 32 requests).  In bf16 results
 // (0.0017) it does not show.
@@ -53,9 +53,8 @@ constexpr int kSplitRows = 64;    // query rows per request and kv head up to wh
 constexpr int kDirectMost = 4096;  // longest cache that is not cut when there are items for two rounds of CTAs
 constexpr int kSplitRowsMixed = 8;  // and with prompts in the batch: what fits one tile of eight rows
 constexpr float kPScaleLog2 = 11.f;
-constexpr float kMaxSlack = 2.f;  // a score may exceed the running maximum by this much (in log2) and
-constexpr float kRefSlack = 4.f;  // a value scale the reference by this factor before O is rescaled: P < 2^15
-constexpr float kRef0 = 1e-30f;
+constexpr float kMaxSlack = 2.f;  // maxima may be stale by this much (in log2) before O is rescaled: P < 2^14
+constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;  // what a value scale counts as: factors stay floats
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm(
@@ -250,11 +249,12 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
     const int mine = last > first ? (last - first + W - 1) / W : 0;
 
     // what a lane knows of half a step, 16 keys: half lane & 1 of step 16 * group + (lane >> 1)
-    struct Info { int id; float ks, vs; } cur, next;
+    struct Info { int id; float ks, vs, lv; } cur, next;  // lv: log2 of the value scale, -infinity if 0 or no number
     auto lookup = [&](int base) {
       Info f;
       f.id = -1;
       f.ks = f.vs = 0.f;
+      f.lv = -INFINITY;
       const int n = base + (lane >> 1);
       const int key = (first + n * W) * kStep + (lane & 1) * 16;
       if (n < mine && key < keys) {
@@ -263,6 +263,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           f.id = id;
           f.ks = c.k_scale[static_cast<int64_t>(id) * KH + head];
           f.vs = c.v_scale[static_cast<int64_t>(id) * KH + head];
+          if (f.vs > 0.f && f.vs < INFINITY) f.lv = fminf(fmaxf(__log2f(f.vs), kLeastLog2), kMostLog2);
         }
       }
       return f;
@@ -298,7 +299,8 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
 
     // Q fragments, while the first keys are on their way: this lane loads row 8 j + g; its scores belong to the rows 8 j + 2 t + e
     uint32_t qb[NQ][KQ][2];
-    float qmul[NQ][2], m[NQ][2], l[NQ][2];
+    // maximum of log2 p, sum of p, maximum of log2 p + log2 of its value scale (O is in units of 2^mw), 2^(m - mw)
+    float qmul[NQ][2], m[NQ][2], l[NQ][2], mw[NQ][2], unit[NQ][2];
     int lim[NQ][2];
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
@@ -333,8 +335,8 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
       for (int e = 0; e < 2; ++e) {
         qmul[j][e] = __shfl_sync(~0u, f, (2 * t + e) * 4);
         lim[j][e] = __shfl_sync(~0u, see, (2 * t + e) * 4);
-        m[j][e] = -INFINITY;
-        l[j][e] = 0.f;
+        m[j][e] = mw[j][e] = -INFINITY;
+        l[j][e] = unit[j][e] = 0.f;
       }
     }
 
@@ -344,7 +346,6 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
 #pragma unroll
       for (int i = 0; i < NV; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
     }
-    float ref = kRef0, inv_ref = 1.f / kRef0;
 
     for (int n = 0; n < mine; ++n) {
       const int stage = n % S;
@@ -354,11 +355,12 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
       }
       const int src = 2 * (n & 15);
       const int id0 = __shfl_sync(~0u, cur.id, src), id1 = __shfl_sync(~0u, cur.id, src + 1);
-      float ks[2], vs[2];
+      float ks[2], vs[2], lv[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         ks[i] = __shfl_sync(~0u, cur.ks, src + i);
         vs[i] = __shfl_sync(~0u, cur.vs, src + i);
+        lv[i] = __shfl_sync(~0u, cur.lv, src + i);
       }
       cp_async_wait<S - 1>();  // one group per step: this step's copies of this lane have landed,
       __syncwarp();            // and the other lanes'
@@ -413,39 +415,43 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           }
         }
       }
-      float mn[NQ][2];
+      float mn[NQ][2], wn[NQ][2];
       bool up = false;
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(s[0][j][e], s[0][j][2 + e]), fmaxf(s[1][j][e], s[1][j][2 + e]));
+          const float top[2] = {fmaxf(s[0][j][e], s[0][j][2 + e]), fmaxf(s[1][j][e], s[1][j][2 + e])};
+          float mx = fmaxf(top[0], top[1]);
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
+          float tx = mx + lv[0];
+          if (lv[0] != lv[1]) {  // halves of two blocks, for the whole warp
+            tx = fmaxf(top[0] + lv[0], top[1] + lv[1]);
+            tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, 4));
+            tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, 8));
+            tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, 16));
+          }
           mn[j][e] = fmaxf(m[j][e], mx);
-          up = up || mn[j][e] > m[j][e] + kMaxSlack;
+          wn[j][e] = fmaxf(mw[j][e], tx);
+          up = up || mn[j][e] > m[j][e] + kMaxSlack || wn[j][e] > mw[j][e] + kMaxSlack;
         }
       }
-      float vtop = vs[0] < INFINITY ? vs[0] : 0.f;
-      vtop = vs[1] < INFINITY ? fmaxf(vtop, vs[1]) : vtop;
-      const bool grow = vtop > kRefSlack * ref;
-      if (__any_sync(~0u, up) || grow) {
-        float down = 1.f;
-        if (grow) {
-          down = ref / vtop;
-          ref = vtop;
-          inv_ref = 1.f / vtop;
-        }
+      if (__any_sync(~0u, up)) {
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
           float a[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            a[e] = mn[j][e] == -INFINITY ? 1.f : exp2_approx(m[j][e] - mn[j][e]);
+            l[j][e] *= mn[j][e] == -INFINITY ? 1.f : exp2_approx(m[j][e] - mn[j][e]);
+            a[e] = 1.f;
+            if (wn[j][e] > -INFINITY) {  // else the row's values so far are zeros
+              a[e] = exp2_approx(mw[j][e] - wn[j][e]);
+              unit[j][e] = exp2f(mn[j][e] - wn[j][e]);
+            }
             m[j][e] = mn[j][e];
-            l[j][e] *= a[e];
-            a[e] *= down;
+            mw[j][e] = wn[j][e];
           }
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
@@ -460,28 +466,28 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
         const float base[2] = {(m[j][0] == -INFINITY ? 0.f : m[j][0]) - kPScaleLog2,
                                (m[j][1] == -INFINITY ? 0.f : m[j][1]) - kPScaleLog2};
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const float w = vs[mt] * inv_ref;
+        for (int h = 0; h < 2; ++h) {
+          const float w[2] = {vs[h] * unit[j][0], vs[h] * unit[j][1]};
           float pv[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = exp2_approx(s[mt][j][e] - base[e & 1]);
+            const float x = exp2_approx(s[h][j][e] - base[e & 1]);
             l[j][e & 1] += x;
-            pv[e] = x * w;
+            pv[e] = x * w[e & 1];
           }
           if (edge) {  // 0 whatever the scale is
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (key0 + mt * 16 + (e >> 1) * 8 + prow >= lim[j][e & 1] || (mt == 0 ? id0 : id1) < 0) pv[e] = 0.f;
+              if (key0 + h * 16 + (e >> 1) * 8 + prow >= lim[j][e & 1] || (h == 0 ? id0 : id1) < 0) pv[e] = 0.f;
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t high = pack2(pv[2 * e], pv[2 * e + 1], __half());
-            pb[mt][j][e] = transpose8x8(high);
+            pb[h][j][e] = transpose8x8(high);
             if constexpr (kRest) {
               float a, b;
               unpack2(high, a, b, __half());
-              pr[mt][j][e] = transpose8x8(pack2(pv[2 * e] - a, pv[2 * e + 1] - b, __half()));
+              pr[h][j][e] = transpose8x8(pack2(pv[2 * e] - a, pv[2 * e + 1] - b, __half()));
             }
           }
         }
@@ -544,18 +550,18 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
     }
     __syncthreads();  // no ring is in use: partial outputs take their place
     float* parts = reinterpret_cast<float*>(smem);
-    const float unit = ref * exp2f(-kPScaleLog2);
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = j * 8 + 2 * t + e;
+        const float back = mw[j][e] == -INFINITY ? 0.f : exp2f(mw[j][e] - m[j][e] - kPScaleLog2);
         if (row < rows) {
           float4* po = reinterpret_cast<float4*>(parts + (warp * ROWS + row) * D + g * (D / 8));
 #pragma unroll
           for (int i = 0; i < NV; i += 2)
-            po[i / 2] = make_float4(o[j][i][e] * unit, o[j][i][2 + e] * unit, o[j][i + 1][e] * unit,
-                                    o[j][i + 1][2 + e] * unit);
+            po[i / 2] = make_float4(o[j][i][e] * back, o[j][i][2 + e] * back, o[j][i + 1][e] * back,
+                                    o[j][i + 1][2 + e] * back);
         }
       }
     }

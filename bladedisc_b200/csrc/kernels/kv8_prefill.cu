@@ -12,8 +12,9 @@
 //   softmax      a warpgroup per query tile, a thread per row: running maximum in the scale of log2, exp2, sums in
 //                fp32; O is rescaled only when a maximum has grown by 2^kSlack.
 // Few rows over a long cache: several CTAs take shares of an item's keys (launch_of) and a second kernel joins them.
-// Key scales multiply the scores of their 16 keys; value scales multiply P relative to a running reference that the
-// loader keeps (O is in its units), so that P stays in the range of f16; see kPScaleLog2.
+// Key scales multiply the scores of their 16 keys.  Value scales multiply P: a row of O is in units of the largest
+// product of a probability and its value scale so far, so that P stays in the range of f16 and keeps its bits whatever
+// scales the blocks have that have little part in it; see kPScaleLog2.
 // What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all): shared memory 3070 cycles (levels in
 // and out 512, operands out 512, Q and K into S 1536 at 64 keys a product, V into O 512), exp2 2048 at 16 a cycle less
 // the quarter that goes to the FMA pipe, products 2560.  Measured at 4095 tokens behind 12289, 32 over 8 heads: 0.95 ms
@@ -50,19 +51,18 @@ constexpr int kThreads = 16 * 32;         // four warpgroups; the last two warps
 constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * (65536 / kThreads), "what setmaxnreg hands out was launched");
 constexpr int kInfo = 4;                 // key tiles whose scales are held
-constexpr float kPScaleLog2 = 8.f;       // P = 2^8 p: 11 bits down to 2^-22 of the row's (stale) maximum
-constexpr float kSlack = 5.f;            // a maximum may be stale by 2^5 and
-constexpr float kRefSlack = 4.f;         // a value scale above the reference by 4: P < 2^15
-constexpr float kRef0 = 1e-30f;
+constexpr float kPScaleLog2 = 8.f;       // P = 2^8 of a row's largest: 11 bits down to 2^-22 of that
+constexpr float kSlack = 5.f;            // maxima may be stale by 2^5: P < 2^14
+constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;  // what a value scale counts as: factors stay floats
 constexpr int kSubTile = kTile * 128;    // 128 rows of 64 f16
 
 struct TileInfo {
-  float f[kGroups];   // key scale * softmax scale * log2 e
-  float w[kGroups];   // value scale / reference
-  float back[kGroups];  // its inverse, or 0 where P rounded to f16 does not stand for its part of the sum (kRoundedSum)
-  float down;         // old reference / new one
-  float ref;
-  uint32_t there;     // bit per group: the block exists and has keys that some row sees
+  float f[kGroups];     // key scale
+  float w[kGroups];     // value scale
+  float lw[kGroups];    // log2 of it, -infinity where it is 0 or no number
+  float back[kGroups];  // its inverse (kRoundedSum)
+  float least[2];       // per step: the smallest value scale, 0 if one is no number (kRoundedSum)
+  uint32_t there;       // bit per group: the block exists and has keys that some row sees
   uint32_t pad;
 };
 
@@ -210,16 +210,16 @@ constexpr uint32_t kOnFma = 0x22;  // of the eight pairs of a group, those whose
 // 0.00032, 1.5 roundings, in batches with few prompts) to 0.00025, for 10 % of the time (4 prompts 127 -> 140 us, mixed
 // 67 -> 72 us); with the sum corrected by what the rounding took, at edges too, 148 us.
 template <bool EDGE, bool ROUNDED>
-__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back, float rmul, float off, uint32_t t_p,
-                                             int left, uint32_t present, uint64_t* sum) {
+__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back, float rmul, float off, float unit,
+                                             float per_unit, uint32_t t_p, int left, uint32_t present, uint64_t* sum) {
   const uint64_t off2 = pair(off, off);
 #pragma unroll
   for (int cc = 0; cc < kKeys / 32; ++cc) {
     uint32_t w[16];
 #pragma unroll
     for (int g = cc * 2; g < cc * 2 + 2; ++g) {
-      const float f = fs[g] * rmul, vw = ws[g];
-      const uint64_t f2 = pair(f, f), w2 = pair(vw, vw), back2 = ROUNDED ? pair(back[g], back[g]) : 0;
+      const float f = fs[g] * rmul, vw = ws[g] * unit, vb = ROUNDED ? back[g] * per_unit : 0.f;
+      const uint64_t f2 = pair(f, f), w2 = pair(vw, vw), back2 = pair(vb, vb);
       const int see = EDGE ? ((present >> g & 1) ? left - g * 16 : 0) : 16;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -537,7 +537,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     const float rmul = p.scale * 1.4426950408889634f / mul;
     // the first step in which some row of this warp does not see every key
     const int first_masked = (__reduce_min_sync(~0u, lim) - key_first) / kKeys;
-    float m = -INFINITY;
+    float m = -INFINITY;   // maximum of log2 p, and
+    float mw = -INFINITY;  // of log2 p + log2 of its value scale: O is in units of 2^mw
+    float unit = 0.f, per_unit = 0.f;  // 2^(m - mw) and its inverse
     uint64_t sum[2] = {0, 0};  // four partial sums
     bool ok = true;
     for (int u = 0; u < nu && active; ++u) {
@@ -552,22 +554,26 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       uint32_t s[kKeys];
 #pragma unroll
       for (int cc = 0; cc < kKeys / 32; ++cc) tmem_ld_x32(t_s + cc * 32, s + cc * 32);
-      float fs[kStepGroups], ws[kStepGroups];
+      float fs[kStepGroups], ws[kStepGroups], lw[kStepGroups];
 #pragma unroll
       for (int g = 0; g < kStepGroups; ++g) {
         fs[g] = in.f[first_group + g];
         ws[g] = in.w[first_group + g];
+        lw[g] = in.lw[first_group + g];
       }
       const uint32_t present = in.there >> first_group & ((1u << kStepGroups) - 1);
-      const float down = (u & 1) == 0 ? in.down : 1.f;
       const bool edge = u >= first_masked || present != (1u << kStepGroups) - 1;
       const int key0 = key_first + u * kKeys;
 #pragma unroll
       for (int cc = 0; cc < kKeys / 32; ++cc) tmem_ld_wait32(s + cc * 32);
-      float mx = -INFINITY;
+      float mx = -INFINITY, tx = -INFINITY;
       if (!edge) {
 #pragma unroll
-        for (int g = 0; g < kStepGroups; ++g) mx = max2(mx, max16(s + g * 16) * fs[g]);
+        for (int g = 0; g < kStepGroups; ++g) {
+          const float top = max16(s + g * 16) * fs[g];
+          mx = max2(mx, top);
+          tx = fmaxf(tx, fmaf(top, rmul, lw[g]));
+        }
       } else {
 #pragma unroll
         for (int g = 0; g < kStepGroups; ++g) {
@@ -576,20 +582,25 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
 #pragma unroll
           for (int e = 0; e < 16; ++e) top = e < see ? max2(top, __uint_as_float(s[g * 16 + e])) : top;
           mx = see > 0 ? max2(mx, top * fs[g]) : mx;
+          tx = see > 0 ? fmaxf(tx, fmaf(top * fs[g], rmul, lw[g])) : tx;
         }
       }
       mx *= rmul;
-      const float mn = fmaxf(m, mx);
-      const bool up = mn > m + kSlack;
-      if (__any_sync(~0u, up) || down != 1.f) {
-        // a row that stays keeps its maximum: its factor is the reference's alone
-        float a = down;
+      const float mn = fmaxf(m, mx), wn = fmaxf(mw, tx);
+      const bool up = mn > m + kSlack || wn > mw + kSlack;
+      if (__any_sync(~0u, up)) {
+        float a = 1.f;  // a row that stays keeps its maxima
         if (up) {
           const float k = exp2_approx(m - mn);
           sum[0] = mul2(sum[0], pair(k, k));
           sum[1] = mul2(sum[1], pair(k, k));
-          a *= k;
+          if (wn > -INFINITY) {  // else its values so far are zeros
+            a = exp2_approx(mw - wn);
+            unit = exp2f(mn - wn);
+            per_unit = exp2f(wn - mn);
+          }
           m = mn;
+          mw = wn;
         }
         if (u > 0) {
           ok = wait(pv_done(q, u - 1), ((u - 1) >> 1) & 1, 65);  // nothing is being added to O
@@ -612,15 +623,14 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       if (!(mx < INFINITY)) m = __uint_as_float(0x7fc00000u);
       const float off = kPScaleLog2 - (m == -INFINITY ? 0.f : m);
       const float* back = in.back + first_group;
-      bool rounded = kRoundedSum;
-#pragma unroll
-      for (int g = 0; g < kStepGroups; ++g) rounded = rounded && back[g] != 0.f;
+      // P stands for its part of the sum where what f16 cannot hold of it is nothing beside that
+      const bool rounded = kRoundedSum && __all_sync(~0u, in.least[u & 1] * unit >= 0.0625f);
       if (edge) {
-        softmax_step<true, false>(s, fs, ws, back, rmul, off, t_s, lim - key0, present, sum);
+        softmax_step<true, false>(s, fs, ws, back, rmul, off, unit, per_unit, t_s, lim - key0, present, sum);
       } else if (kRoundedSum && rounded) {
-        softmax_step<false, kRoundedSum>(s, fs, ws, back, rmul, off, t_s, 0, 0, sum);
+        softmax_step<false, kRoundedSum>(s, fs, ws, back, rmul, off, unit, per_unit, t_s, 0, 0, sum);
       } else {
-        softmax_step<false, false>(s, fs, ws, back, rmul, off, t_s, 0, 0, sum);
+        softmax_step<false, false>(s, fs, ws, back, rmul, off, unit, per_unit, t_s, 0, 0, sum);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -647,7 +657,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           float a, b;
           unpair(add2(sum[0], sum[1]), a, b);
           const float l = a + b;
-          const float k = l == 0.f ? 0.f : info[(nt - 1) % kInfo].ref / l;
+          // 2^(mw - m) / l, over 2^16 at a time so that neither end passes the range of floats before the other
+          const float k = l == 0.f || mw == -INFINITY ? 0.f : exp2f(mw - m - 16.f) / (l * 0x1p-16f);
           if (there && joined) sh.ml[slot] = make_float2(m, l);
           // the scores of all steps are done with q: its tile takes the output, f32 in two halves
           const int64_t to = !there ? -1 : joined ? slot * D : at * p.ld_out + (head * G + h) * D;
@@ -749,7 +760,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
     }
   } else if (warp == kLoaderWarp) {
     // ------------------------------------------------------------------ loader: lane g < 8 knows group g of the tile
-    float ref = kRef0;
     bool ok = true;
     auto block_of = [&](int t) {  // -1: no such block, or no key of the group is seen
       const int key = key_first + t * kTile + lane * 16;
@@ -789,26 +799,23 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
       // Tile t - 4, whose entry this overwrites, is done with: the keys of tile t - 1 are converted, into the buffer
       // of tile t - 3, so the scores of its second step were complete, and they were begun when P V of the second
       // step of tile t - 4 was, for which its entry was read.
-      float top = vs < INFINITY ? vs : 0.f;
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-      top = __shfl_sync(~0u, top, 0);
-      float down = 1.f;
-      if (top > kRefSlack * ref) {
-        down = ref / top;
-        ref = top;
-      }
       const uint32_t there = __ballot_sync(~0u, id >= 0);
       TileInfo& in = info[t % kInfo];
       if (lane < kGroups) {
         in.f[lane] = ks;
-        const float w = vs / ref;
-        in.w[lane] = w;
-        if (kRoundedSum) in.back[lane] = w >= 0.0625f && w <= kRefSlack ? 1.f / w : 0.f;
+        in.w[lane] = vs;
+        in.lw[lane] = vs > 0.f && vs < INFINITY ? fminf(fmaxf(__log2f(vs), kLeastLog2), kMostLog2) : -INFINITY;
+      }
+      if (kRoundedSum) {
+        float least = vs >= 0.f ? vs : 0.f;
+        least = fminf(least, __shfl_xor_sync(~0u, least, 1));
+        least = fminf(least, __shfl_xor_sync(~0u, least, 2));
+        if (lane < kGroups) {
+          in.back[lane] = 1.f / vs;
+          if (lane % kStepGroups == 0) in.least[lane / kStepGroups] = least;
+        }
       }
       if (lane == 0) {
-        in.down = down;
-        in.ref = ref;
         in.there = there;
       }
       __syncwarp();

@@ -77,3 +77,76 @@ def test_infinite_queries_show(ops, q_len, kv, level, dim, dtype):
         want, slack = reference(finite, cache, q_len, kv, dim ** -0.5)
         err = np.abs(got - want)[1::2]
         assert (err <= 1.001 * slack[1::2] + HALF_STEP[dtype] * np.abs(want[1::2]) + SMALLEST[dtype]).all()
+
+
+def plain(q, cache, q_len, kv, scale):
+    """One request in 64 bits: outputs, and what a kernel may be off by before it rounds its result.
+
+    Probabilities times value scales enter the second product as f16, half a step 2^-11 relative to each, and 2^-25
+    absolute where they are subnormal, in units that bring a row's largest one to 2^8 at least: 2^-33 of that for each key.
+    Scores: (d + 4) 2^-23 of the magnitudes they are summed from, twice that in a probability; 2^-19 for exp2 and the rest."""
+    k, v, ks, vs, table = cache
+    g, d = q.shape[1] // k.shape[1], q.shape[2]
+    q = q.double().cpu().numpy()
+    want, allowed = np.zeros(q.shape), np.zeros(q.shape)
+    hidden = np.arange(kv)[None] > (kv - q_len + np.arange(q_len))[:, None]
+    each = np.repeat
+    for h in range(q.shape[1]):
+        kk, vv = (by_position(t, table)[h // g, :kv].astype(np.float64) for t in (k, v))
+        ksh, vsh = (each(s[table[0], h // g].astype(np.float64), k.shape[2])[:kv] for s in (ks, vs))
+        s = np.where(hidden, -np.inf, (q[:, h] @ kk.T) * ksh * scale)
+        mag = np.where(hidden, 0, (np.abs(q[:, h]) @ np.abs(kk).T) * ksh * scale).max(axis=1, keepdims=True)
+        p = np.exp(s - s.max(axis=1, keepdims=True))
+        p /= p.sum(axis=1, keepdims=True)
+        want[:, h] = p @ (vv * vsh[:, None])
+        largest = (p * vsh).max(axis=1, keepdims=True)
+        allowed[:, h] = (p @ np.abs(vv * vsh[:, None])) * (2.0 ** -11 + 2 * mag * (d + 4) * 2.0 ** -23 + 2.0 ** -19) \
+            + kv * 2.0 ** -33 * largest * 127
+    return want, allowed
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,size", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("ratio,gap", [(20, 60), (30, 60), (20, 14), (-20, 0), (-30, 0)])
+def test_a_block_of_other_magnitude(ops, ratio, gap, where, dim, size, dtype):
+    """Values of one block 2^ratio times those of the others, its scores `gap` lower: with a large gap it has no part in
+    the result, which has to keep its bits all the same; with 14 its part is like that of all others together."""
+    rng = np.random.default_rng(2)
+    for q_len, kv in ((1, 700), (5, 3000), (100, 700), (70, 5000)):
+        cache = k, v, ks, vs, table = cache_of(rng, kv, size, 1, dim)
+        blocks = k.shape[0]
+        odd = table[0, {"first": 0, "middle": blocks // 2, "last": blocks - 1}[where]]
+        ks[:] = 1 / 127
+        k[:, :, :, 0] = 0
+        k[odd, :, :, 0] = -127
+        vs[odd] *= 2.0 ** ratio
+        q = rng.standard_normal((q_len, 2, dim)).astype(np.float32) * 1.5
+        q[:, :, 0] = gap * dim ** 0.5
+        q = torch.from_numpy(q).to(dtype).cuda()
+        got = attend(ops, q, cache, q_len, kv, dim ** -0.5).double().cpu().numpy()
+        want, allowed = plain(q, cache, q_len, kv, dim ** -0.5)
+        assert (np.abs(want) < 2.0 ** 15).all() and np.isfinite(want).all()
+        bad = np.abs(got - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
+        assert not bad.any(), (q_len, kv, np.abs(got - want)[bad].max(), np.abs(want[bad]).max(), bad.mean())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("q_len,kv", [(2, 400), (3, 2500), (90, 400), (70, 5000)])
+def test_value_scales_over_the_whole_range(ops, q_len, kv, dtype):
+    """Blocks without values (scale 0) before, between and behind blocks of scales from 2^-60 to 2^8, in every order, and
+    rows that see nothing but zeros."""
+    rng = np.random.default_rng(3)
+    dim, size, heads = 64, 16, 6
+    cache = k, v, ks, vs, table = cache_of(rng, kv, size, heads, dim)
+    blocks = k.shape[0]
+    j = np.arange(blocks)
+    by_head = [np.where(j % 2, 2.0 ** -8, 0), np.where(j < blocks // 2, 0, 2.0 ** -7), np.where(j < 3, 2.0 ** -6, 0),
+               2.0 ** (-60 + 68 * j / blocks), 2.0 ** (8 - 68 * j / blocks), np.zeros(blocks)]
+    vs[table[0]] = np.stack(by_head, axis=1).astype(np.float32)
+    q = torch.from_numpy(rng.standard_normal((q_len, heads, dim)).astype(np.float32)).to(dtype).cuda()
+    got = attend(ops, q, cache, q_len, kv, dim ** -0.5).double().cpu().numpy()
+    want, allowed = plain(q, cache, q_len, kv, dim ** -0.5)
+    assert not got[:, 5].any()
+    bad = np.abs(got - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
+    assert not bad.any(), (np.abs(got - want)[bad].max(), np.argwhere(bad)[:5])
