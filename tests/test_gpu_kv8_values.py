@@ -150,3 +150,57 @@ def test_value_scales_over_the_whole_range(ops, q_len, kv, dtype):
     assert not got[:, 5].any()
     bad = np.abs(got - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
     assert not bad.any(), (np.abs(got - want)[bad].max(), np.argwhere(bad)[:5])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,size", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("where", ["first", "last"])
+@pytest.mark.parametrize("q_len,kv,gap", [(1, 480, 9), (1, 8192, 13), (7, 8192, 13), (100, 1124, 10), (70, 16400, 14),
+                                          (300, 2300, 11)])
+def test_one_large_probability_beside_thousands(ops, q_len, kv, gap, where, dim, size, dtype):
+    """One key 2^gap above 2^gap others, which together weigh as much as it does: half of the result comes from
+    probabilities of 2^-gap of the largest, with the largest met first or last."""
+    rng = np.random.default_rng(4)
+    cache = k, v, ks, vs, table = cache_of(rng, kv, size, 1, dim)
+    keys = by_position(k, table)
+    keys[:, :, 0] = 0
+    keys[0, 0 if where == "first" else kv - q_len, 0] = 127  # the last key that every row sees
+    put_positions(k, table, keys)
+    ks[:] = 1 / 127
+    q = 0.2 * rng.standard_normal((q_len, 2, dim)).astype(np.float32)
+    q[:, :, 0] = gap * np.log(2) * dim ** 0.5
+    q = torch.from_numpy(q).to(dtype).cuda()
+    s = (q.double().cpu().numpy() @ by_position(k, table)[0, :kv - q_len + 1].T) / 127 * dim ** -0.5
+    p = np.exp(s - s.max(axis=-1, keepdims=True))
+    largest = 1 / p.sum(axis=-1)
+    # scores vary by 0.2 times the spread of a level, 0.58: twelve times that is the factor of four allowed here
+    assert ((largest > 0.25) & (largest < 0.75)).all() and (np.sort(p, axis=-1)[..., -2] < 2.0 ** (2 - gap)).all()
+    got = attend(ops, q, cache, q_len, kv, dim ** -0.5).double().cpu().numpy()
+    want, allowed = plain(q, cache, q_len, kv, dim ** -0.5)
+    bad = np.abs(got - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
+    assert not bad.any(), (np.abs(got - want)[bad].max(), np.argwhere(bad)[:5])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,group,dim,q_lens,kv_lens", [
+    (1, 16, 64, [1, 120, 1, 1], [900, 333, 3000, 15]),        # single tokens of 16 rows
+    (2, 4, 128, [4, 3, 100, 16, 1], [700, 1500, 100, 33, 64]),  # drafts of 4 to 64 rows
+    (1, 33, 64, [1, 2, 70], [2000, 600, 70]),
+])
+def test_requests_of_a_few_rows_beside_prompts(ops, heads, group, dim, q_lens, kv_lens, dtype):
+    """Between one tile of eight rows and a prompt: 9 to 66 rows per request and kv head, in one batch with prompts."""
+    rng = np.random.default_rng(5)
+    size, n = 16, len(q_lens)
+    width = -(-max(kv_lens) // size)
+    k, v, ks, vs, order = cache_of(rng, n * width * size, size, heads, dim)
+    table = order.reshape(n, width)
+    start = np.cumsum([0] + q_lens)
+    q = torch.from_numpy(rng.standard_normal((start[-1], heads * group, dim)).astype(np.float32)).to(dtype).cuda()
+    i32 = lambda x: torch.as_tensor(np.asarray(x), dtype=torch.int32, device="cuda")  # noqa: E731
+    gpu = [torch.from_numpy(a).cuda() for a in (k, v, ks, vs, table)]
+    got = ops.kv8_attention(q, *gpu, i32(start), i32(q_lens), i32(kv_lens), max_q=max(q_lens)).double().cpu().numpy()
+    for r in range(n):
+        rows = slice(start[r], start[r + 1])
+        want, allowed = plain(q[rows], (k, v, ks, vs, table[r:r + 1]), q_lens[r], kv_lens[r], dim ** -0.5)
+        bad = np.abs(got[rows] - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
+        assert not bad.any(), (r, np.abs(got[rows] - want)[bad].max())
