@@ -1,7 +1,7 @@
 // Append to the 8-bit cache and reading blocks back.
 //
-// A block of tokens and a head share one scale s = max|x| / 127 over the tokens stored so far, levels are
-// rne(x / s).  When new tokens raise the maximum of a block that already holds tokens, those are moved to the
+// A block of tokens and a head share one scale s = max|x| / 127 over the tokens stored since its first one (those that
+// a trim took back too), levels are rne(x / s).  When new tokens raise the maximum of a block that already holds tokens, those are moved to the
 // new scale: level' = rne(level * (s_old / s)); the error that adds is at most half a level each time the maximum
 // grows.  Keys are rotated (pairs (i, i + dim / 2)) in fp32 and quantized without a rounding in between.
 //

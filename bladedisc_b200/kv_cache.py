@@ -48,7 +48,8 @@ class PagedKVCache8:
                                     max_tokens)
 
     def trim(self, keep: torch.Tensor) -> None:
-        """Keeps the first ``keep[r]`` tokens of each request: 0 ends it, fewer than cached takes drafts back."""
+        """Keeps the first ``keep[r]`` tokens of each request: 0 ends it, fewer than cached takes drafts back.  A block
+        that keeps tokens keeps its scales too, those of the drafts included; see :func:`ops.kv8_append`."""
         ops.kv_blocks_trim(keep, self.lens, self.table, self.free_list, self.free_count, self.block_size)
 
     def append(self, layer: int, qkv: torch.Tensor, plan: ops.KvPlan, cos: Optional[torch.Tensor] = None,

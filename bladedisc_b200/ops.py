@@ -648,7 +648,8 @@ def kv_blocks_extend(tokens: torch.Tensor, lens: torch.Tensor, table: torch.Tens
 def kv_blocks_trim(keep: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, free_list: torch.Tensor,
                    free_count: torch.Tensor, block_size: int) -> None:
     """Keeps the first ``keep[r]`` cached tokens of each request (0 releases it) and gives the blocks behind them
-    back to the stack, in place.  Trimming to the lengths before a `kv_blocks_extend` undoes it exactly."""
+    back to the stack, in place.  Trimming to the lengths before a `kv_blocks_extend` undoes it exactly; scales and levels
+    that a `kv8_append` changed in a block that keeps tokens stay as they are."""
     dev, a = _kv_blocks_args(keep, lens, table, free_list, free_count, block_size)
     _call(dev, _lib.load().disc_b200_kv_blocks_trim, a)
 
@@ -683,8 +684,9 @@ def kv8_append(qkv: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: tor
     rotated (a view of ``qkv`` without ``cos``), or None if there are no query heads.
 
     The cache is ``k``, ``v`` int8 ``[blocks, kv heads, block size, head size]`` with ``k_scale``, ``v_scale`` float32
-    ``[blocks, kv heads]``: a block and a head share the scale ``max|x| / 127`` of the tokens stored so far; tokens
-    that the block held before are moved to the new scale when it grows.  ``slots`` and ``positions`` are those of
+    ``[blocks, kv heads]``: a block and a head share the scale ``max|x| / 127`` of the tokens stored since its first one,
+    tokens that a trim took back among them; tokens that the block held before are moved to the new scale when it grows,
+    and a value that is not finite makes them NaN until the block is begun anew.  ``slots`` and ``positions`` are those of
     `kv_blocks_extend` (the first ``tokens`` entries are read; slot -1 = not stored)."""
     dev = _one_device(k, qkv, v, k_scale, v_scale, slots, positions, cos, sin)
     cache = _kv8_cache(k, v, k_scale, v_scale)

@@ -488,7 +488,8 @@ int32_t disc_b200_attention(const disc_b200_attention_args* args, void* stream);
  *   slots[t], positions[t]  of token row t; -1 for rows of refused requests and behind the last row.
  * trim: keeps the first tokens[r] (at most lens[r]; 0 releases the request) tokens of every request, pushes the
  * blocks behind them back and sets their table entries to -1.  trim to the lengths before an extend undoes it
- * bit for bit.  A block belongs to one request at a time.  requests <= 8192.  Calls that share state must be
+ * bit for bit; it does not undo what an append did to the scale and levels of a block that keeps tokens (below).
+ * A block belongs to one request at a time.  requests <= 8192.  Calls that share state must be
  * ordered by the caller. */
 typedef struct disc_b200_kv_blocks_args {
   const int32_t* tokens; /* [requests] */
@@ -523,6 +524,7 @@ typedef struct disc_b200_kv8_cache {
  *          holds tokens before the first new one (offset > 0)
  *   levels clamp(rne(x / s), -127, 127), 0 when s = 0; tokens that the block held before move to the new scale,
  *          rne(level * (s_old / s)).  A value that is not finite makes the scale NaN until the block is reused.
+ *          Tokens that trim took back count: the scale is that of all that was stored since offset 0 was written.
  * qkv: f16 / bf16 [tokens, (q_heads + 2 * kv_heads) * dim] with row stride ld_qkv, not modified; rotated q goes to
  * q_out [tokens, q_heads, dim].  cos_table NULL: no rotation, q_out and positions are not used.  slots: as extend
  * writes them (-1 = skip); the slots of one block must follow one another without a gap, and no slot may occur twice.
