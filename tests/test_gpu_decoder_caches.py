@@ -86,3 +86,66 @@ def test_captured_steps_of_both_caches_outlive_new_starts(decoder):
     assert torch.equal(z, want_dense)
     assert cache.lens.tolist() == [46, 23] and other.lens.tolist() == [0] and len(kv) == 2 and len(hold) == 4
     decoder.paged = None
+
+
+class TwoRanks:
+    """Collectives of two ranks that are two host threads and share a GPU and its default stream: a rank copies what it
+    needs of the other's tensor, between two meetings of the threads."""
+
+    def __init__(self, rank, box, gate):
+        self.rank, self.world, self.box, self.gate = rank, 2, box, gate
+
+    def _meet(self, t, copy):
+        self.box[self.rank] = t
+        self.gate.wait(60)
+        copy(self.box[1 - self.rank])
+        self.gate.wait(60)
+        return t
+
+    def all_gather_(self, buf):
+        return self._meet(buf, lambda other: buf[1 - self.rank].copy_(other[1 - self.rank]))
+
+    def all_reduce_max_(self, t):
+        mine = t.clone()
+
+        def copy(other):
+            torch.maximum(mine, other, out=mine)
+        self._meet(t, copy)
+        return t.copy_(mine)
+
+
+def test_two_ranks_have_half_of_the_heads_each(decoder):
+    """Ragged prompts and steps over paged caches that hold two of four heads, against one rank."""
+    import threading
+
+    from bladedisc_b200.decoder import QuantDecoder
+    steps = [[70, 5, 90], [1, 40, 1], [1, 1, 1]]
+
+    def run(d, out):
+        cache = d.start_paged(requests=3, num_blocks=30, max_seq=160, block_size=16)
+        assert cache.k[0].shape[1] == d.cfg.heads // d.world
+        for i, tokens in enumerate(steps):
+            out.append(d.forward_paged(_ids(30 + i, sum(tokens)), i32(tokens), max(tokens)).clone())
+        assert cache.lens.tolist() == [72, 46, 92]
+
+    want, box, gate, got, errors = [], [None, None], threading.Barrier(2), [[], []], []
+    run(decoder, want)
+
+    def rank(r):
+        try:
+            run(QuantDecoder(decoder.cfg, TwoRanks(r, box, gate), seed=3), got[r])
+        except Exception as e:  # raised below, in the thread that waits
+            errors.append(e)
+            gate.abort()
+
+    threads = [threading.Thread(target=rank, args=(r,)) for r in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b, w in zip(*got, want):
+        assert torch.equal(a, b)
+        # the same integers, scales and heads; sums over a row of the norms may be added in another order, which can turn
+        # an int8 rounding: as far as two runs of a quantized net differ
+        assert (a.float() - w.float()).abs().mean() < 0.01 * w.float().abs().mean()
