@@ -54,6 +54,7 @@ constexpr int kDirectMost = 4096;  // longest cache that is not cut when there a
 constexpr int kSplitRowsMixed = 8;  // and with prompts in the batch: what fits one tile of eight rows
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // maxima may be stale by this much (in log2) before O is rescaled: P < 2^14
+constexpr float kNone = -3.4028235e38f;  // maximum of a row that has seen no key: below it, -infinity alone
 constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;  // what a value scale counts as: factors stay floats
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -249,12 +250,11 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
     const int mine = last > first ? (last - first + W - 1) / W : 0;
 
     // what a lane knows of half a step, 16 keys: half lane & 1 of step 16 * group + (lane >> 1)
-    struct Info { int id; float ks, vs, lv; } cur, next;  // lv: log2 of the value scale, -infinity if 0 or no number
+    struct Info { int id; float ks, vs; } cur, next;
     auto lookup = [&](int base) {
       Info f;
       f.id = -1;
       f.ks = f.vs = 0.f;
-      f.lv = -INFINITY;
       const int n = base + (lane >> 1);
       const int key = (first + n * W) * kStep + (lane & 1) * 16;
       if (n < mine && key < keys) {
@@ -263,7 +263,6 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           f.id = id;
           f.ks = c.k_scale[static_cast<int64_t>(id) * KH + head];
           f.vs = c.v_scale[static_cast<int64_t>(id) * KH + head];
-          if (f.vs > 0.f && f.vs < INFINITY) f.lv = fminf(fmaxf(__log2f(f.vs), kLeastLog2), kMostLog2);
         }
       }
       return f;
@@ -335,7 +334,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
       for (int e = 0; e < 2; ++e) {
         qmul[j][e] = __shfl_sync(~0u, f, (2 * t + e) * 4);
         lim[j][e] = __shfl_sync(~0u, see, (2 * t + e) * 4);
-        m[j][e] = mw[j][e] = -INFINITY;
+        m[j][e] = mw[j][e] = kNone;
         l[j][e] = unit[j][e] = 0.f;
       }
     }
@@ -347,11 +346,16 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
       for (int i = 0; i < NV; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
     }
 
+    float log_vs = -INFINITY;  // log2 of cur.vs, -infinity if that is 0 or no number
     for (int n = 0; n < mine; ++n) {
       const int stage = n % S;
-      if ((n & 15) == 0 && n > 0) {
-        cur = next;
-        next = lookup(n + 16);
+      if ((n & 15) == 0) {
+        if (n > 0) {
+          cur = next;
+          next = lookup(n + 16);
+        }
+        // not where it is looked up: the copies would wait for the scale
+        log_vs = cur.vs > 0.f && cur.vs < INFINITY ? fminf(fmaxf(__log2f(cur.vs), kLeastLog2), kMostLog2) : -INFINITY;
       }
       const int src = 2 * (n & 15);
       const int id0 = __shfl_sync(~0u, cur.id, src), id1 = __shfl_sync(~0u, cur.id, src + 1);
@@ -360,8 +364,10 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
       for (int i = 0; i < 2; ++i) {
         ks[i] = __shfl_sync(~0u, cur.ks, src + i);
         vs[i] = __shfl_sync(~0u, cur.vs, src + i);
-        lv[i] = __shfl_sync(~0u, cur.lv, src + i);
+        lv[i] = __shfl_sync(~0u, log_vs, src + i);
       }
+      if (id1 < 0) lv[1] = lv[0];  // a half that is not there has no scores either
+      else if (id0 < 0) lv[0] = lv[1];
       cp_async_wait<S - 1>();  // one group per step: this step's copies of this lane have landed,
       __syncwarp();            // and the other lanes'
       const uint8_t* kt = ring_ptr + stage * 2 * L::kHalf;
@@ -415,27 +421,25 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           }
         }
       }
-      float mn[NQ][2], wn[NQ][2];
+      float mx[NQ][2], wx[NQ][2];  // maxima of this step, -infinity without a key
       bool up = false;
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float top[2] = {fmaxf(s[0][j][e], s[0][j][2 + e]), fmaxf(s[1][j][e], s[1][j][2 + e])};
-          float mx = fmaxf(top[0], top[1]);
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
-          float tx = mx + lv[0];
-          if (lv[0] != lv[1]) {  // halves of two blocks, for the whole warp
-            tx = fmaxf(top[0] + lv[0], top[1] + lv[1]);
-            tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, 4));
-            tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, 8));
-            tx = fmaxf(tx, __shfl_xor_sync(~0u, tx, 16));
+          float x = fmaxf(top[0], top[1]);
+          x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+          mx[j][e] = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+          wx[j][e] = mx[j][e] + lv[0];
+          if (lv[0] != lv[1]) {  // two blocks, for the whole warp
+            x = fmaxf(top[0] + lv[0], top[1] + lv[1]);
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+            wx[j][e] = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
           }
-          mn[j][e] = fmaxf(m[j][e], mx);
-          wn[j][e] = fmaxf(mw[j][e], tx);
-          up = up || mn[j][e] > m[j][e] + kMaxSlack || wn[j][e] > mw[j][e] + kMaxSlack;
+          up = up || mx[j][e] > m[j][e] + kMaxSlack || wx[j][e] > mw[j][e] + kMaxSlack;
         }
       }
       if (__any_sync(~0u, up)) {
@@ -444,14 +448,12 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           float a[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            l[j][e] *= mn[j][e] == -INFINITY ? 1.f : exp2_approx(m[j][e] - mn[j][e]);
-            a[e] = 1.f;
-            if (wn[j][e] > -INFINITY) {  // else the row's values so far are zeros
-              a[e] = exp2_approx(mw[j][e] - wn[j][e]);
-              unit[j][e] = exp2f(mn[j][e] - wn[j][e]);
-            }
-            m[j][e] = mn[j][e];
-            mw[j][e] = wn[j][e];
+            const float mn = fmaxf(m[j][e], mx[j][e]), wn = fmaxf(mw[j][e], wx[j][e]);
+            l[j][e] *= exp2_approx(m[j][e] - mn);
+            a[e] = exp2_approx(mw[j][e] - wn);
+            unit[j][e] = wn > kNone ? exp2f(mn - wn) : 0.f;  // 0: the row's values so far are zeros
+            m[j][e] = mn;
+            mw[j][e] = wn;
           }
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
@@ -463,8 +465,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
       uint32_t pb[2][NQ][2], pr[2][NQ][2];  // P in f16, and what that rounding left out (kRest)
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
-        const float base[2] = {(m[j][0] == -INFINITY ? 0.f : m[j][0]) - kPScaleLog2,
-                               (m[j][1] == -INFINITY ? 0.f : m[j][1]) - kPScaleLog2};
+        const float base[2] = {m[j][0] - kPScaleLog2, m[j][1] - kPScaleLog2};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float w[2] = {vs[h] * unit[j][0], vs[h] * unit[j][1]};
@@ -543,7 +544,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
         l[j][e] += __shfl_xor_sync(~0u, l[j][e], 8);
         l[j][e] += __shfl_xor_sync(~0u, l[j][e], 16);
         if (g == 0) {
-          part_m[warp][j * 8 + 2 * t + e] = m[j][e];
+          part_m[warp][j * 8 + 2 * t + e] = m[j][e] == kNone ? -INFINITY : m[j][e];
           part_l[warp][j * 8 + 2 * t + e] = l[j][e] * exp2f(-kPScaleLog2);
         }
       }
@@ -555,7 +556,7 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = j * 8 + 2 * t + e;
-        const float back = mw[j][e] == -INFINITY ? 0.f : exp2f(mw[j][e] - m[j][e] - kPScaleLog2);
+        const float back = mw[j][e] == kNone ? 0.f : exp2f(mw[j][e] - m[j][e] - kPScaleLog2);
         if (row < rows) {
           float4* po = reinterpret_cast<float4*>(parts + (warp * ROWS + row) * D + g * (D / 8));
 #pragma unroll
