@@ -55,7 +55,8 @@ constexpr int kSplitRowsMixed = 8;  // and with prompts in the batch: what fits 
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // maxima may be stale by this much (in log2) before O is rescaled: P < 2^14
 constexpr float kNone = -3.4028235e38f;  // maximum of a row that has seen no key: below it, -infinity alone
-constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;  // what a value scale counts as: factors stay floats
+// What a value scale counts as, and mw is above m at least: factors stay floats.
+constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;
 
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm(
@@ -448,7 +449,9 @@ __device__ __forceinline__ void split_body(const Kv8AttentionParams& p, const Sp
           float a[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m[j][e], mx[j][e]), wn = fmaxf(mw[j][e], wx[j][e]);
+            const float mn = fmaxf(m[j][e], mx[j][e]);
+            float wn = fmaxf(mw[j][e], wx[j][e]);
+            if (wn > kNone) wn = fmaxf(wn, mn + kLeastLog2);  // the largest p may belong to a block without values
             l[j][e] *= exp2_approx(m[j][e] - mn);
             a[e] = exp2_approx(mw[j][e] - wn);
             unit[j][e] = wn > kNone ? exp2f(mn - wn) : 0.f;  // 0: the row's values so far are zeros

@@ -53,7 +53,8 @@ static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * (65536 / kThreads), "what
 constexpr int kInfo = 4;                 // key tiles whose scales are held
 constexpr float kPScaleLog2 = 8.f;       // P = 2^8 of a row's largest: 11 bits down to 2^-22 of that
 constexpr float kSlack = 5.f;            // maxima may be stale by 2^5: P < 2^14
-constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;  // what a value scale counts as: factors stay floats
+// What a value scale counts as, and mw is above m at least: factors stay floats.
+constexpr float kLeastLog2 = -120.f, kMostLog2 = 122.f;
 constexpr int kSubTile = kTile * 128;    // 128 rows of 64 f16
 
 struct TileInfo {
@@ -586,7 +587,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         }
       }
       mx *= rmul;
-      const float mn = fmaxf(m, mx), wn = fmaxf(mw, tx);
+      const float mn = fmaxf(m, mx);
+      float wn = fmaxf(mw, tx);
       const bool up = mn > m + kSlack || wn > mw + kSlack;
       if (__any_sync(~0u, up)) {
         float a = 1.f;  // a row that stays keeps its maxima
@@ -595,6 +597,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           sum[0] = mul2(sum[0], pair(k, k));
           sum[1] = mul2(sum[1], pair(k, k));
           if (wn > -INFINITY) {  // else its values so far are zeros
+            wn = fmaxf(wn, mn + kLeastLog2);  // the largest p may belong to a block without values
             a = exp2_approx(mw - wn);
             unit = exp2f(mn - wn);
             per_unit = exp2f(wn - mn);

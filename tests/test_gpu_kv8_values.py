@@ -204,3 +204,28 @@ def test_requests_of_a_few_rows_beside_prompts(ops, heads, group, dim, q_lens, k
         want, allowed = plain(q[rows], (k, v, ks, vs, table[r:r + 1]), q_lens[r], kv_lens[r], dim ** -0.5)
         bad = np.abs(got[rows] - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
         assert not bad.any(), (r, np.abs(got[rows] - want)[bad].max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gap", [20, 80, 150, 1000])
+@pytest.mark.parametrize("where", ["first", "middle"])
+def test_the_largest_probabilities_belong_to_a_block_without_values(ops, where, gap, dtype):
+    """Keys of a block whose values are all zeros are e^gap times as probable as the others: what is left of those."""
+    rng = np.random.default_rng(7)
+    dim, size = 64, 16
+    for q_len, kv in ((1, 400), (9, 3000), (80, 700), (70, 5000)):
+        cache = k, v, ks, vs, table = cache_of(rng, kv, size, 1, dim)
+        k[:, :, :, 0] = 0
+        block = table[0, {"first": 0, "middle": k.shape[0] // 2}[where]]
+        k[block, :, :, 0] = 127
+        ks[:] = 1 / 127
+        v[block], vs[block] = 0, 0
+        q = rng.standard_normal((q_len, 2, dim)).astype(np.float32)
+        q[:, :, 0] = gap * dim ** 0.5
+        q = torch.from_numpy(q).to(dtype).cuda()
+        got = attend(ops, q, cache, q_len, kv, dim ** -0.5).double().cpu().numpy()
+        want, allowed = plain(q, cache, q_len, kv, dim ** -0.5)
+        # below 2^-126 of the row's largest a probability is nothing
+        allowed += 2.0 ** -126 * kv * vs.max() * 127
+        bad = np.abs(got - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
+        assert np.isfinite(got).all() and not bad.any(), (q_len, kv, np.abs(got - want)[bad].max(), np.abs(want).max())
