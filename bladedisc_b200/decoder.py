@@ -236,6 +236,8 @@ class QuantDecoder:
         if cache.rope is None:
             raise RuntimeError("the paged cache has no rotation tables: start_paged makes one that has")
         total = ids.numel()
+        if total == 0:  # no rows: no request gets tokens
+            return self.embed.new_empty(0, self.cfg.hidden)
         plan = cache.extend(tokens, total)
 
         def attention(L: _Layer, idx: int, qkv: torch.Tensor) -> torch.Tensor:

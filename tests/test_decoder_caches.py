@@ -32,7 +32,7 @@ class Recorder:
 def decoder(monkeypatch):
     d = object.__new__(QuantDecoder)  # no weights: those are made on a GPU
     d.cfg, d.world, d.device = DecoderConfig.tiny(), 1, torch.device("cpu")
-    d.kv, d.pos, d.paged = None, 0, None
+    d.kv, d.pos, d.paged, d.embed = None, 0, None, torch.zeros(1, 1)
     d._cos = d._sin = None
     monkeypatch.setattr(d, "_run_layers", lambda ids, attention: attention(None, 0, torch.zeros(ids.numel(), 4)))
     return d
@@ -90,3 +90,10 @@ def test_a_cache_without_tables_is_refused(decoder):
     cache.rope = None
     with pytest.raises(RuntimeError, match="start_paged"):
         tables_of_a_step(decoder, cache)
+
+
+def test_a_step_without_tokens_touches_nothing(decoder):
+    cache = decoder.start_paged(requests=1, num_blocks=3, max_seq=50)
+    decoder.paged = rec = Recorder(cache)
+    y = decoder.forward_paged(torch.zeros(0, dtype=torch.int64), None, 0)
+    assert y.shape == (0, decoder.cfg.hidden) and rec.tables is None

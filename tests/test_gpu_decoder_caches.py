@@ -149,3 +149,13 @@ def test_two_ranks_have_half_of_the_heads_each(decoder):
         # the same integers, scales and heads; sums over a row of the norms may be added in another order, which can turn
         # an int8 rounding: as far as two runs of a quantized net differ
         assert (a.float() - w.float()).abs().mean() < 0.01 * w.float().abs().mean()
+
+
+def test_steps_without_tokens(decoder):
+    """Rows of no request, a batch of such rows only, and an empty batch."""
+    cache = decoder.start_paged(requests=2, num_blocks=20, max_seq=100, block_size=16)
+    for rows, tokens, lens in ((7, [3, 0], [3, 0]), (4, [0, 0], [3, 0]), (0, [0, 0], [3, 0]), (0, [1, 0], [3, 0])):
+        y = decoder.forward_paged(_ids(5, rows), i32(tokens), max(tokens))
+        assert y.shape == (rows, decoder.cfg.hidden) and torch.isfinite(y).all()
+        assert cache.lens.tolist() == lens
+    decoder.paged = None
