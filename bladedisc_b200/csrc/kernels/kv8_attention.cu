@@ -22,8 +22,8 @@ namespace {
 // per SM: ragged lengths balance to one step.  A share that ends inside an item leaves its partial maximum, sum and
 // output in the workspace, and a second small kernel joins them.  Short caches (max_kv <= kKv8DirectKeys) take one CTA
 // per item and need neither, and so do those up to kDirectMost keys when there are items for two rounds of CTAs: 32
-// requests of up to 2048 tokens and 32 heads take 65 us that way and 73 in shares; 8 requests of up to 32700 tokens and
-// 8 kv heads take 252 us that way and 61 in shares.
+// requests of up to 2048 tokens and 32 heads took 61 us that way and 73 in shares (before the second product below); 8
+// requests of up to 32700 tokens and 8 kv heads 252 us that way and 61 in shares.
 //
 // Inside a CTA a warp runs by itself: it fetches its steps with 16-byte asynchronous copies into its own ring (TMA
 // boxes of 2 to 4 KB cost the warp 170 cycles each, a quarter of a step), multiplies with mma.sync m16n8k16, keeps
@@ -38,20 +38,26 @@ namespace {
 // P, a probability times its value scale, goes to f16 as 2^11 for a row's largest, so that it keeps its 11 bits down to
 // 2^-25 of that; a row of O is in units of the largest so far.  With f16 results what the
 // rounding of P leaves out is multiplied too: over values of either sign it weighs as much as the rounding of the result
-// (error 0.00021, that of one rounding, instead of 0.00025 to 0.00031; 61 -> 64.6 us for the 32 requests).  In bf16 results
+// (error 0.00021, that of one rounding, instead of 0.00025 to 0.00031; 61 -> 65 us for the 32 requests).  In bf16 results
 // (0.0017) it does not show.
 // Rows in the ring are swizzled (16-byte chunk c of row r at c ^ (r & 7), for dim 64 c ^ (r / 2 & 3)); that and the key
 // order perm(n) = n ^ ((n & 1) << 2) make the 16-byte shared-memory reads free of bank conflicts.
 //
-// What bounds it: 270 MB of levels in 61 us (4.4 TB/s, 0.67 of the measured copy rate); the copies alone take 54, of
-// which 10 are the start of a share (sums, table, scales, first copy one after the other) and the join.  Measured and
-// not kept: four CTAs per SM with a ring of three tiles (65 us), levels as f16 subnormals in the first product (64).
+// What bounds it: the cache's bytes.  On the GPU the 32 requests, 330 MB, take 65 us (5.1 TB/s, 0.77 of the measured copy
+// rate); long contexts of 270 MB, 8 requests of up to 32700 tokens or one of 131072, 8 kv heads, 59 and 63 us (4.6 and
+// 4.3 TB/s).  Without any arithmetic the copies of those took 54 and 57, of which 10 are the start of a share (sums, table,
+// scales, first copy one after the other) and the join.  Measured for the 32 requests, then at 61 us, and not kept: four
+// CTAs per SM with a ring of three tiles (65 us), levels as f16 subnormals in the first product (64).
 constexpr int kStep = 32;         // keys per step of a warp
 constexpr int kSplitWarps = 4;
 constexpr int kSplitThreads = kSplitWarps * 32;
-constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one,
+constexpr int kSplitRows = 64;    // query rows per request and kv head up to which this kernel is the faster one
 constexpr int kDirectMost = 4096;  // longest cache that is not cut when there are items for two rounds of CTAs
-constexpr int kSplitRowsMixed = 8;  // and with prompts in the batch: what fits one tile of eight rows
+// The same with prompts in the batch: one tile of eight rows.  Requests of 9 to 64 rows go to the prompts' CTAs, one for
+// all their keys.  Beside 3 prompts of 511 over 2 000 keys, 32 over 8 heads, that is right for 20 requests of 16 tokens
+// (136 us; here 223) and even for 20 of 4 (156; 151), but not over long caches: one request of 4 tokens over 32 000 keys
+// beside a prompt of 500 takes 263 us (here 93), a single token with 16 query heads per kv head 448 (78).
+constexpr int kSplitRowsMixed = 8;
 constexpr float kPScaleLog2 = 11.f;
 constexpr float kMaxSlack = 2.f;  // maxima may be stale by this much (in log2) before O is rescaled: P < 2^14
 constexpr float kNone = -3.4028235e38f;  // maximum of a row that has seen no key: below it, -infinity alone

@@ -5,9 +5,9 @@
 // new scale: level' = rne(level * (s_old / s)); the error that adds is at most half a level each time the maximum
 // grows.  Keys are rotated (pairs (i, i + dim / 2)) in fp32 and quantized without a rounding in between.
 //
-// Bound by memory for prompts: 9815 tokens with 32 query and 8 + 8 key / value heads of 128 values in bf16 move 225 MB
-// in 52 us (0.66 of the measured copy rate), reading 315 blocks back 65 MB in 14 us; by latency for decode steps: 64
-// tokens with 32 + 32 + 32 heads 10 us.
+// Prompts: 9815 tokens with 32 query and 8 + 8 key / value heads of 128 values in bf16 move 225 MB in 54 us (0.63 of the
+// measured copy rate), issue slots half busy: memory latency at 35 % of the warps, and every run is rotated twice.  Reading
+// 315 blocks back moves 65 MB in 12.4 us (0.80).  Decode steps are latency: 64 tokens with 32 + 32 + 32 heads 7.4 us.
 #include "kv8.h"
 
 #include "device_info.h"

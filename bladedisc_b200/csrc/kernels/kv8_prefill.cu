@@ -15,10 +15,13 @@
 // Key scales multiply the scores of their 16 keys.  Value scales multiply P: a row of O is in units of the largest
 // product of a probability and its value scale so far, so that P stays in the range of f16 and keeps its bits whatever
 // scales the blocks have that have little part in it; see kPScaleLog2.
-// What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all): shared memory 3070 cycles (levels in
-// and out 512, operands out 512, Q and K into S 1536 at 64 keys a product, V into O 512), exp2 2048 at 16 a cycle less
-// the quarter that goes to the FMA pipe, products 2560.  Measured at 4095 tokens behind 12289, 32 over 8 heads: 0.95 ms
-// (0.90 to 1.0 as the card's power allows) = 1010 TFLOP/s, 0.61 of the measured bf16 rate.  What was measured on the way
+// What bounds it, at dim 128 per 256 rows and 128 keys (about 3950 cycles in all), by count: shared memory 3070 cycles
+// (levels in and out 512, operands out 512, Q and K into S 1536 at 64 keys a product, V into O 512), exp2 2048 at 16 a
+// cycle less the quarter that goes to the FMA pipe, products 2560 (a product of 64 keys takes 49 cycles, not 32).  Of a
+// profiled call the tensor pipe was active 0.48, instructions were issued 0.57 and the conversion and exp2 pipe was busy
+// 0.37 of the time: no unit is at its end, the chain from scores to P to products goes through all of them in turn.
+// Measured at 4095 tokens behind 12289, 32 over 8 heads in bf16: 0.91 to 1.03 ms by card and clock = 930 to 1060 TFLOP/s,
+// 0.57 to 0.64 of the measured bf16 rate.  What was measured on the way
 // there, in the order of the steps, beside 0.98: scores of 128 keys in one buffer 1.07 ms (the chain softmax, P V, S is
 // exposed), one issuer for both tiles 1.44,
 // products issued behind `lane == 0` 1.20, levels to registers instead of TMA 1.40, exp2 all on the MUFU 1.01, half of
@@ -208,8 +211,8 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
 constexpr uint32_t kOnFma = 0x22;  // of the eight pairs of a group, those whose exp2 is a polynomial
 // ROUNDED: the row's sum is that of P as f16 holds it (divided by its value scale again), so that the rounding of the
 // largest ones cancels where the output is divided by it.  For f16 results only: their error falls from 0.00029 (up to
-// 0.00032, 1.5 roundings, in batches with few prompts) to 0.00025, for 10 % of the time (4 prompts 127 -> 140 us, mixed
-// 67 -> 72 us); with the sum corrected by what the rounding took, at edges too, 148 us.
+// 0.00032, 1.5 roundings, in batches with few prompts) to 0.00024, for 10 % of the time (4 prompts 127 -> 140 us); with the
+// sum corrected by what the rounding took, at edges too, 148 us.
 template <bool EDGE, bool ROUNDED>
 __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back, float rmul, float off, float unit,
                                              float per_unit, uint32_t t_p, int left, uint32_t present, uint64_t* sum) {
@@ -949,11 +952,18 @@ struct Launch {
 };
 // The grid, and which items' keys are cut into shares: all of them, so that few rows over long caches fill the GPU, or
 // those that would not fill the last round of CTAs.  As many shares as make one to three full rounds, where the rounds
-// (as measured 2.1 us per key tile and 8 per CTA) and the join (5 us, and its bytes at 6 TB/s) come to 6 % less than they
-// do without shares.  The host has bounds only: the rows of the batch, and the longest cache.  (8 kv heads of 128 with 4
-// query heads each, one request: 64 tokens over 8 000 139 -> 33 us, 100 over 30 000 492 -> 82 us, 512 over 8 192
-// 146 -> 94 us; 4095 over 16 384, 3.46 rounds: the last round alone, 0.99 -> 0.95 ms; 1500 over 12 000, 1.3 rounds:
-// 339 -> 295 us.  In f16, before its sums were those of P as rounded, which adds up to 10 % to both sides.)
+// (2.1 us per key tile and 8 per CTA) and the join (5 us, and its bytes at 6 TB/s) come to 6 % less than they do without
+// shares.  A round of 148 equal CTAs takes 2.6 us per key tile in f16 and 2.3 in bf16 at heads of 128, 2.3 and 2.0 at heads
+// of 64: one pair of figures serves both.  The host has bounds only: the rows of the batch, and the longest cache.
+// One request, 8 kv heads with 4 query heads each, us without shares -> as chosen:
+//                       128, f16        128, bf16       64, f16         64, bf16
+//   64 over  8 000     162 ->   36     143 ->   35     155 ->   30     129 ->   26
+//  100 over 30 000     579 ->   92     490 ->   83     559 ->   84     466 ->   68
+//  200 over  3 000      70 ->   36      66 ->   37      62 ->   31      54 ->   29
+//  512 over  8 192     167 ->  106     145 ->   95     156 ->   99     133 ->   85
+//  700 over  2 500      61 ->   61      56 ->   61      54 ->   54      48 ->   48
+// 1500 over 12 000     441 ->  365     377 ->  298     409 ->  324     350 ->  263
+// 2048 over 30 000    1127 -> 1174     990 ->  995    1058 -> 1010     902 ->  826
 Launch launch_of(const Kv8AttentionParams& p, void* workspace) {
   Launch l = {};
   const int64_t G = p.q_heads / p.cache.kv_heads, KH = p.cache.kv_heads, sms = device_sm_count();
