@@ -214,8 +214,9 @@ constexpr uint32_t kOnFma = 0x22;  // of the eight pairs of a group, those whose
 // 0.00032, 1.5 roundings, in batches with few prompts) to 0.00024, for 10 % of the time (4 prompts 127 -> 140 us); with the
 // sum corrected by what the rounding took, at edges too, 148 us.
 template <bool EDGE, bool ROUNDED>
-__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back, float rmul, float off, float unit,
-                                             float per_unit, uint32_t t_p, int left, uint32_t present, uint64_t* sum) {
+__device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back,
+                                             float rmul, float off, float unit, float per_unit, uint32_t t_p, int left,
+                                             uint32_t present, uint64_t* sum) {
   const uint64_t off2 = pair(off, off);
 #pragma unroll
   for (int cc = 0; cc < kKeys / 32; ++cc) {
@@ -813,7 +814,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
         in.lw[lane] = vs > 0.f && vs < INFINITY ? fminf(fmaxf(__log2f(vs), kLeastLog2), kMostLog2) : -INFINITY;
       }
       if (kRoundedSum) {
-        float least = vs >= 0.f ? vs : 0.f;
+        float least = vs >= 0.f && vs < INFINITY ? vs : 0.f;
         least = fminf(least, __shfl_xor_sync(~0u, least, 1));
         least = fminf(least, __shfl_xor_sync(~0u, least, 2));
         if (lane < kGroups) {
@@ -821,9 +822,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ C
           if (lane % kStepGroups == 0) in.least[lane / kStepGroups] = least;
         }
       }
-      if (lane == 0) {
-        in.there = there;
-      }
+      if (lane == 0) in.there = there;
       __syncwarp();
       if (lane == 0) mbar_arrive(info_full(t % kInfo));
       id = id_next;

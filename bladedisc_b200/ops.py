@@ -753,7 +753,7 @@ def kv8_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_scale: to
     are int32 and stay on the device; ``max_q`` bounds ``q_lens`` and shapes the launch (rows behind it are not
     computed), ``max_kv`` bounds ``kv_lens`` and only steers how the work is split (default: the table's width).
     Query heads are a multiple of the kv heads.  ``scale`` defaults to ``head size ** -0.5``.  Rows that belong to
-    no request are left as ``out`` had them; a row that sees no key gives zeros."""
+    no request are left as ``out`` had them; a row that sees no key gives zeros.  ``out`` may not overlap ``q``."""
     dev = _one_device(q, k, v, k_scale, v_scale, table, q_start, q_lens, kv_lens, out)
     cache = _kv8_cache(k, v, k_scale, v_scale)
     kind = _kv_type("q", q.dtype)

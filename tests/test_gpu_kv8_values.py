@@ -229,3 +229,21 @@ def test_the_largest_probabilities_belong_to_a_block_without_values(ops, where, 
         allowed += 2.0 ** -126 * kv * vs.max() * 127
         bad = np.abs(got - want) > allowed * 1.001 + HALF_STEP[dtype] * np.abs(want) + SMALLEST[dtype]
         assert np.isfinite(got).all() and not bad.any(), (q_len, kv, np.abs(got - want)[bad].max(), np.abs(want).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("which", ["first", "last", "all"])
+def test_value_scales_that_are_not_finite_show(ops, which, bad, dtype):
+    """In every value of the rows that see such a block, and in no other."""
+    rng = np.random.default_rng(8)
+    dim, size = 64, 16
+    for q_len, kv in ((1, 400), (20, 3000), (80, 700), (300, 2000), (70, 5000)):
+        cache = k, v, ks, vs, table = cache_of(rng, kv, size, 1, dim)
+        blocks = k.shape[0]
+        begin = {"first": 0, "last": blocks - 1, "all": 0}[which]
+        vs[table[0, begin:] if which == "all" else table[0, begin]] = bad
+        q = torch.from_numpy(rng.standard_normal((q_len, 2, dim)).astype(np.float32)).to(dtype).cuda()
+        got = attend(ops, q, cache, q_len, kv, dim ** -0.5).double().cpu().numpy()
+        see = kv - q_len + np.arange(q_len) >= begin * size
+        assert see.any() and not np.isfinite(got[see]).any() and np.isfinite(got[~see]).all(), (q_len, kv)
