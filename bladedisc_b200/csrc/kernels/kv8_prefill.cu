@@ -20,8 +20,8 @@
 // cycle less the quarter that goes to the FMA pipe, products 2560 (a product of 64 keys takes 49 cycles, not 32).  Of a
 // profiled call the tensor pipe was active 0.48, instructions were issued 0.57 and the conversion and exp2 pipe was busy
 // 0.37 of the time: no unit is at its end, the chain from scores to P to products goes through all of them in turn.
-// Measured at 4095 tokens behind 12289, 32 over 8 heads in bf16: 0.91 to 1.03 ms by card and clock = 930 to 1060 TFLOP/s,
-// 0.57 to 0.64 of the measured bf16 rate.  What was measured on the way
+// Measured at 4095 tokens behind 12289, 32 over 8 heads in bf16: 0.91 to 1.05 ms by card and clock = 920 to 1060 TFLOP/s,
+// 0.56 to 0.64 of the measured bf16 rate.  What was measured on the way
 // there, in the order of the steps, beside 0.98: scores of 128 keys in one buffer 1.07 ms (the chain softmax, P V, S is
 // exposed), one issuer for both tiles 1.44,
 // products issued behind `lane == 0` 1.20, levels to registers instead of TMA 1.40, exp2 all on the MUFU 1.01, half of
@@ -211,7 +211,7 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
 constexpr uint32_t kOnFma = 0x22;  // of the eight pairs of a group, those whose exp2 is a polynomial
 // ROUNDED: the row's sum is that of P as f16 holds it (divided by its value scale again), so that the rounding of the
 // largest ones cancels where the output is divided by it.  For f16 results only: their error falls from 0.00029 (up to
-// 0.00032, 1.5 roundings, in batches with few prompts) to 0.00024, for 10 % of the time (4 prompts 127 -> 140 us); with the
+// 0.00032, 1.5 roundings, in batches with few prompts) to 0.00023 - 0.00025, for 10 % of the time (4 prompts 127 -> 140 us); with the
 // sum corrected by what the rounding took, at edges too, 148 us.
 template <bool EDGE, bool ROUNDED>
 __device__ __forceinline__ void softmax_step(const uint32_t* s, const float* fs, const float* ws, const float* back,
